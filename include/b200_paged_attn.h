@@ -69,8 +69,9 @@ enum {
   B200_DEV_BAD_LENGTH = 2,   /* context length < 1 or > M*S                */
   B200_DEV_BAD_SLOT = 4,     /* slot outside [0, P*S)                      */
   B200_DEV_WAIT_TIMEOUT = 8, /* a bounded pipeline wait gave up            */
-  B200_DEV_SLOT_MISMATCH = 16 /* fused write: slot is not the slot of the
+  B200_DEV_SLOT_MISMATCH = 16, /* fused write: slot is not the slot of the
                                  sequence's last context position           */
+  B200_DEV_BAD_POSITION = 32 /* position outside the rotation table          */
 };
 
 /* Paged KV pool descriptor: two contiguous [L, P, S, H, D] tensors. */
@@ -275,6 +276,74 @@ B200_API int b200_qkv_kv_write(const b200_qkv_kv_write_args_t* args, void* strea
  * CTAs (128 x *tile_n tiles).  A diagnostic with no counterpart in the reference. */
 B200_API int b200_qkv_kv_write_plan(int64_t num_tokens, int64_t hidden, int32_t* kind,
                                     int32_t* tile_n, int32_t* splits);
+
+/*
+ * Norm and rotation of the query and key heads (no counterpart in the
+ * reference, whose model has learned positions).  For every token t and head
+ * row x = q[t, h, :] or k[t, h, :]:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight      (y = x without a weight)
+ *   (y_a, y_b) -> (y_a c_i - y_b s_i, y_a s_i + y_b c_i),  i < R / 2
+ * with c_i = cos_sin[positions[t], i], s_i = cos_sin[positions[t], R/2 + i],
+ * pairs (a, b) = (i, i + R/2), or (2i, 2i + 1) when `interleaved`; elements
+ * from R on are not rotated.  Computed in f32, rounded once.  q_out / k_out
+ * may be q / k themselves (same pointer and strides), else must not overlap
+ * the inputs.  A token whose position lies outside [0, table_rows) gets zero
+ * rows and sets B200_DEV_BAD_POSITION.
+ */
+typedef struct {
+  int64_t num_tokens;               /* T (0 is a no-op)                     */
+  int64_t num_q_heads;
+  int64_t num_kv_heads;
+  int64_t head_dim;                 /* D <= 256                             */
+  const void* q;                    /* [T, Hq, D], strides in elements      */
+  int64_t q_stride[3];
+  const void* k;                    /* [T, Hkv, D]                          */
+  int64_t k_stride[3];
+  void* q_out;                      /* [T, Hq, D]                           */
+  int64_t q_out_stride[3];
+  void* k_out;                      /* [T, Hkv, D] (NULL for the KV append) */
+  int64_t k_out_stride[3];
+  const void* q_weight;             /* [D] contiguous, or NULL: no norm     */
+  const void* k_weight;
+  const float* cos_sin;             /* [table_rows, R] contiguous           */
+  int64_t table_rows;
+  int64_t rotary_dim;               /* R: even, 2 <= R <= D                 */
+  const void* positions;            /* device [T]                           */
+  int64_t position_stride;
+  int32_t* status;                  /* optional device word (may be NULL)   */
+  b200_dtype_t dtype;               /* of q, k, q_out, k_out (and v)        */
+  b200_dtype_t weight_dtype;
+  b200_index_t position_dtype;
+  int32_t interleaved;
+  float eps;                        /* > 0                                  */
+  int32_t reserved;
+} b200_qk_norm_rope_args_t;
+
+B200_API int b200_qk_norm_rope(const b200_qk_norm_rope_args_t* args, void* stream);
+
+/*
+ * The same pass with the KV append of b200_kv_scatter: the normed and rotated
+ * k and the unchanged v are stored at the tokens' slots
+ *   pool.{k,v}[layer, slot[t] / S, slot[t] % S, :, :]
+ * (rounded once to the pool's dtype) and only q_out is written besides.
+ * rope.k_out must be NULL; the pool's num_heads and head_dim are the keys'.
+ * A slot outside [0, P*S) skips that token's k and v and sets
+ * B200_DEV_BAD_SLOT; a bad position skips them too.  Where several tokens
+ * have one slot, any of them may be the one that stays, element by element.
+ */
+typedef struct {
+  b200_qk_norm_rope_args_t rope;
+  b200_kv_pool_t pool;
+  int64_t layer_idx;
+  const void* v;                    /* [T, Hkv, D]                          */
+  int64_t v_stride[3];
+  const void* slot_mapping;         /* device [T]                           */
+  int64_t slot_stride;
+  b200_index_t slot_dtype;
+  int32_t reserved;
+} b200_rope_kv_append_args_t;
+
+B200_API int b200_rope_kv_append(const b200_rope_kv_append_args_t* args, void* stream);
 
 /* Workspace bytes the decode launch needs for these sizes. */
 B200_API size_t b200_paged_decode_workspace_size(int64_t batch, int64_t num_heads,

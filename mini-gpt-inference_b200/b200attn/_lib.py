@@ -27,6 +27,7 @@ DEV_BAD_LENGTH = 2
 DEV_BAD_SLOT = 4
 DEV_WAIT_TIMEOUT = 8
 DEV_SLOT_MISMATCH = 16
+DEV_BAD_POSITION = 32
 
 # Static split-K scratch of b200_paged_decode_no_alloc (B200_NO_ALLOC_SCRATCH_BYTES).
 NO_ALLOC_SCRATCH_BYTES = 4 << 20
@@ -79,6 +80,28 @@ class QkvKvWriteArgs(ctypes.Structure):
                 ("slot_dtype", ctypes.c_int), ("status", _p)]
 
 
+class QkNormRopeArgs(ctypes.Structure):
+    # The [3] stride arrays are written as three fields each: the same layout,
+    # and one positional constructor call fills the struct.
+    _fields_ = [("num_tokens", _i64), ("num_q_heads", _i64), ("num_kv_heads", _i64),
+                ("head_dim", _i64),
+                ("q", _p), ("q_s0", _i64), ("q_s1", _i64), ("q_s2", _i64),
+                ("k", _p), ("k_s0", _i64), ("k_s1", _i64), ("k_s2", _i64),
+                ("q_out", _p), ("q_out_s0", _i64), ("q_out_s1", _i64), ("q_out_s2", _i64),
+                ("k_out", _p), ("k_out_s0", _i64), ("k_out_s1", _i64), ("k_out_s2", _i64),
+                ("q_weight", _p), ("k_weight", _p), ("cos_sin", _p), ("table_rows", _i64),
+                ("rotary_dim", _i64), ("positions", _p), ("position_stride", _i64),
+                ("status", _p), ("dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int),
+                ("position_dtype", ctypes.c_int), ("interleaved", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class RopeKvAppendArgs(ctypes.Structure):
+    _fields_ = [("rope", QkNormRopeArgs), ("pool", KVPool), ("layer_idx", _i64), ("v", _p),
+                ("v_s0", _i64), ("v_s1", _i64), ("v_s2", _i64), ("slot_mapping", _p),
+                ("slot_stride", _i64), ("slot_dtype", ctypes.c_int), ("reserved", ctypes.c_int32)]
+
+
 class PrefillBatchArgs(ctypes.Structure):
     _fields_ = [("num_seqs", _i64), ("seqs", ctypes.POINTER(PrefillArgs))]
 
@@ -94,6 +117,8 @@ SIGNATURES = {
     "b200_qkv_kv_write_plan": (ctypes.c_int, [_i64, _i64, ctypes.POINTER(ctypes.c_int32),
                                               ctypes.POINTER(ctypes.c_int32),
                                               ctypes.POINTER(ctypes.c_int32)]),
+    "b200_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), _p]),
+    "b200_rope_kv_append": (ctypes.c_int, [ctypes.POINTER(RopeKvAppendArgs), _p]),
     "b200_paged_decode_workspace_size": (
         ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int32]),
     "b200_chunked_prefill_workspace_size": (

@@ -15,6 +15,13 @@ C-ABI entry points as :mod:`b200attn.ops`.
                               int prefix_len, int layer_idx) -> Tensor
     b200attn::qkv_kv_write(Tensor x, Tensor weight, Tensor(a!) k_pool, Tensor(b!) v_pool,
                            Tensor slot_mapping, int layer_idx) -> Tensor
+    b200attn::qk_norm_rope(Tensor q, Tensor k, Tensor positions, Tensor cos_sin,
+                           Tensor? q_weight, Tensor? k_weight, float eps,
+                           bool interleaved) -> (Tensor, Tensor)
+    b200attn::rope_kv_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_pool, Tensor(b!) v_pool,
+                             Tensor slot_mapping, Tensor positions, Tensor cos_sin,
+                             int layer_idx, Tensor? q_weight, Tensor? k_weight, float eps,
+                             bool interleaved) -> Tensor
 
 The pools are the KVBlockPool tensors ``[L, P, S, H, D]`` (S = block size).
 ``paged_decode`` writes k_new/v_new into the pools when they are given
@@ -23,7 +30,8 @@ at ``slot_mapping`` (attention.py:193-208) and returns the prefix-aware
 attention of the chunk (attention.py:215-299). ``qkv_kv_write`` is the bf16
 QKV projection (attention.py:79-83) that stores k and v at ``slot_mapping``
 from its epilogue and returns q as [T, H, D] (attention.py:177-208,
-:360-392). Importing this module registers the ops.
+:360-392). ``qk_norm_rope`` and ``rope_kv_append`` are the head norms and the
+rotation of :mod:`b200attn.rope`. Importing this module registers the ops.
 """
 from __future__ import annotations
 
@@ -32,9 +40,10 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import ops, rope
 
-__all__ = ["paged_decode", "kv_scatter", "chunked_prefill", "qkv_kv_write"]
+__all__ = ["paged_decode", "kv_scatter", "chunked_prefill", "qkv_kv_write", "qk_norm_rope",
+           "rope_kv_append"]
 
 
 def _pool(k_pool: torch.Tensor, v_pool: torch.Tensor) -> SimpleNamespace:
@@ -96,3 +105,36 @@ def qkv_kv_write(x: torch.Tensor, weight: torch.Tensor, k_pool: torch.Tensor,
 @qkv_kv_write.register_fake
 def _(x, weight, k_pool, v_pool, slot_mapping, layer_idx):
     return x.new_empty((x.shape[0], k_pool.shape[3], k_pool.shape[4]))
+
+
+@torch.library.custom_op("b200attn::qk_norm_rope", mutates_args=())
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    return rope.qk_norm_rope_b200(q, k, positions, cos_sin, q_weight=q_weight, k_weight=k_weight,
+                                  eps=eps, interleaved=interleaved)
+
+
+@qk_norm_rope.register_fake
+def _(q, k, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            torch.empty_like(k, memory_format=torch.contiguous_format))
+
+
+@torch.library.custom_op("b200attn::rope_kv_append", mutates_args=("k_pool", "v_pool"))
+def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
+                   v_pool: torch.Tensor, slot_mapping: torch.Tensor, positions: torch.Tensor,
+                   cos_sin: torch.Tensor, layer_idx: int,
+                   q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   interleaved: bool = False) -> torch.Tensor:
+    return rope.rope_kv_append_b200(q, k, v, _pool(k_pool, v_pool), slot_mapping, positions,
+                                    cos_sin, layer_idx, q_weight=q_weight, k_weight=k_weight,
+                                    eps=eps, interleaved=interleaved)
+
+
+@rope_kv_append.register_fake
+def _(q, k, v, k_pool, v_pool, slot_mapping, positions, cos_sin, layer_idx, q_weight=None,
+      k_weight=None, eps=1e-6, interleaved=False):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)

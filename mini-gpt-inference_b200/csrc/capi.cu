@@ -132,6 +132,31 @@ b200_decode_args_t prefill_as_decode(const b200_prefill_args_t& a) {
   return d;
 }
 
+int check_rope(const b200_qk_norm_rope_args_t& a) {
+  B200_CHECK(a.num_q_heads >= 1 && a.num_kv_heads >= 1 && a.head_dim >= 2, B200_ERR_INVALID_ARGUMENT,
+             "q and k dimensions must be nonzero");
+  B200_CHECK(a.head_dim <= 256 && a.num_q_heads + 2 * a.num_kv_heads < (int64_t(1) << 20),
+             B200_ERR_UNSUPPORTED, "rotation: head_dim must be <= 256 (and heads < 2^20)");
+  // One CTA per token: the grid's x extent bounds T.
+  B200_CHECK(a.num_tokens < (int64_t(1) << 31) - 1, B200_ERR_UNSUPPORTED,
+             "rotation: num_tokens must be < 2^31 - 1");
+  B200_CHECK(a.q != nullptr && a.k != nullptr && a.q_out != nullptr && a.cos_sin != nullptr &&
+                 a.positions != nullptr,
+             B200_ERR_INVALID_ARGUMENT, "q, k, q_out, cos_sin and positions must be non-null");
+  B200_CHECK(valid_dtype(a.dtype), B200_ERR_INVALID_ARGUMENT,
+             "q/k dtype must be float32, bfloat16 or float16");
+  B200_CHECK((a.q_weight == nullptr && a.k_weight == nullptr) || valid_dtype(a.weight_dtype),
+             B200_ERR_INVALID_ARGUMENT, "norm weights must be float32, bfloat16 or float16");
+  B200_CHECK(valid_index(a.position_dtype), B200_ERR_INVALID_ARGUMENT, "positions must be integer");
+  B200_CHECK(a.rotary_dim >= 2 && a.rotary_dim % 2 == 0 && a.rotary_dim <= a.head_dim,
+             B200_ERR_INVALID_ARGUMENT, "rotary_dim must be even and in [2, head_dim]");
+  B200_CHECK(a.table_rows >= 1, B200_ERR_INVALID_ARGUMENT, "cos_sin must have at least one row");
+  B200_CHECK(a.eps > 0.f, B200_ERR_INVALID_ARGUMENT, "eps must be positive");
+  B200_CHECK(reinterpret_cast<uintptr_t>(a.cos_sin) % 4 == 0, B200_ERR_INVALID_ARGUMENT,
+             "cos_sin must be 4-byte aligned");
+  return B200_OK;
+}
+
 int sm_count() {
   DeviceInfo dev;
   if (current_device_info(&dev) != B200_OK) return 148;
@@ -220,6 +245,38 @@ int b200_qkv_kv_write(const b200_qkv_kv_write_args_t* args, void* stream) {
              B200_ERR_UNSUPPORTED, "qkv projection: x, weight and q_out must be 16-byte aligned");
   B200_CHECK(valid_index(a.slot_dtype), B200_ERR_INVALID_ARGUMENT, "slot_mapping must be integer");
   return launch_qkv_kv_write(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200_qk_norm_rope(const b200_qk_norm_rope_args_t* args, void* stream) {
+  clear_error();
+  if (args == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "null arguments");
+  const b200_qk_norm_rope_args_t& a = *args;
+  if (a.num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (a.num_tokens == 0) return B200_OK;
+  int rc = check_rope(a);
+  if (rc != B200_OK) return rc;
+  if (a.k_out == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "k_out must be non-null");
+  return launch_qk_norm_rope(a, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+int b200_rope_kv_append(const b200_rope_kv_append_args_t* args, void* stream) {
+  clear_error();
+  if (args == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "null arguments");
+  const b200_rope_kv_append_args_t& a = *args;
+  int rc = check_pool(a.pool, a.layer_idx);
+  if (rc != B200_OK) return rc;
+  if (a.rope.num_tokens < 0) return fail(B200_ERR_INVALID_ARGUMENT, "num_tokens must be >= 0");
+  if (a.rope.num_tokens == 0) return B200_OK;
+  rc = check_rope(a.rope);
+  if (rc != B200_OK) return rc;
+  B200_CHECK(a.rope.k_out == nullptr, B200_ERR_INVALID_ARGUMENT,
+             "KV append: the keys go to the pool, k_out must be null");
+  B200_CHECK(a.pool.num_heads == a.rope.num_kv_heads && a.pool.head_dim == a.rope.head_dim,
+             B200_ERR_INVALID_ARGUMENT, "k/v head dimensions do not match the KV pool");
+  B200_CHECK(a.v != nullptr && a.slot_mapping != nullptr, B200_ERR_INVALID_ARGUMENT,
+             "v and slot_mapping must be non-null");
+  B200_CHECK(valid_index(a.slot_dtype), B200_ERR_INVALID_ARGUMENT, "slot_mapping must be integer");
+  return launch_qk_norm_rope(a.rope, &a, static_cast<cudaStream_t>(stream));
 }
 
 int b200_qkv_kv_write_plan(int64_t num_tokens, int64_t hidden, int32_t* kind, int32_t* tile_n,

@@ -37,6 +37,9 @@ struct QkvPlan {
 int launch_qkv_kv_write(const b200_qkv_kv_write_args_t& a, cudaStream_t stream);
 struct DeviceInfo;
 QkvPlan qkv_plan(int64_t T, int64_t C, const DeviceInfo& dev);
+// Head norms + rotation, and the same with the KV append (pool == nullptr: none).
+int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_append_args_t* append,
+                        cudaStream_t stream);
 int launch_bounded_wait_selftest(int32_t* status, int64_t limit_ns, cudaStream_t stream);
 
 // Split-K planning shared by the launcher and the workspace query.
