@@ -345,6 +345,58 @@ typedef struct {
 
 B200_API int b200_rope_kv_append(const b200_rope_kv_append_args_t* args, void* stream);
 
+/*
+ * Paged decode attention of a batch whose sequences share a prefix, which is
+ * read once for all of them (no counterpart in the reference):
+ *   out[b, h, :] = softmax(q[b, h, :] . K^T / sqrt(D)) V
+ * over positions 0 .. context_lengths[b] - 1 of sequence b.  Position n <
+ * prefix_len is row n % S of block prefix_table[n / S]; from prefix_len on it
+ * is row n % S of block block_tables[b, n / S] (entries before
+ * prefix_len / S are not read, so a block table of the whole sequence serves).
+ * Query head h reads key/value head h / (Hq / H): Hq is a multiple of the
+ * pool's num_heads.  prefix_len 0 is a plain paged decode.
+ * A sequence whose length is < 1, < prefix_len or > M*S gets zero rows and
+ * sets B200_DEV_BAD_LENGTH (a padding row of a fixed-size batch, say).
+ * `workspace`: b200_shared_prefix_decode_workspace_size() bytes, 256-byte
+ * aligned; its contents need not be initialised and are the call's own until
+ * it has run.
+ */
+typedef struct {
+  b200_kv_pool_t pool;
+  int64_t layer_idx;
+  int64_t batch;                    /* B >= 1                               */
+  int64_t num_q_heads;              /* Hq                                   */
+  int64_t prefix_len;               /* >= 0                                 */
+  int64_t table_width;              /* M >= 1 (columns of block_tables)     */
+  const void* q;                    /* [B, Hq, D] any strides               */
+  int64_t q_stride[3];
+  void* out;                        /* [B, Hq, D] strides                   */
+  int64_t out_stride[3];
+  const void* prefix_table;         /* device [>= ceil(prefix_len / S)]     */
+  int64_t prefix_table_len;
+  int64_t prefix_table_stride;
+  const void* block_tables;         /* device [B, M]                        */
+  int64_t block_table_stride[2];
+  const void* context_lengths;      /* device [B]                           */
+  int64_t context_length_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status;                  /* optional device word (may be NULL)   */
+  b200_dtype_t q_dtype;             /* f32 / bf16 / f16                     */
+  b200_dtype_t out_dtype;
+  b200_index_t prefix_table_dtype;
+  b200_index_t block_table_dtype;
+  b200_index_t context_length_dtype;
+  int32_t reserved;
+} b200_shared_prefix_args_t;
+
+B200_API int b200_shared_prefix_decode(const b200_shared_prefix_args_t* args, void* stream);
+B200_API size_t b200_shared_prefix_decode_workspace_size(int64_t batch, int64_t num_q_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t prefix_len, int64_t table_width,
+                                                int64_t block_size, b200_dtype_t kv_dtype,
+                                                b200_dtype_t q_dtype);
+
 /* Workspace bytes the decode launch needs for these sizes. */
 B200_API size_t b200_paged_decode_workspace_size(int64_t batch, int64_t num_heads,
                                         int64_t head_dim, int64_t table_width,

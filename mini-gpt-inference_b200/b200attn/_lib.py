@@ -102,6 +102,20 @@ class RopeKvAppendArgs(ctypes.Structure):
                 ("slot_stride", _i64), ("slot_dtype", ctypes.c_int), ("reserved", ctypes.c_int32)]
 
 
+class SharedPrefixArgs(ctypes.Structure):
+    _fields_ = [("pool", KVPool), ("layer_idx", _i64), ("batch", _i64), ("num_q_heads", _i64),
+                ("prefix_len", _i64), ("table_width", _i64),
+                ("q", _p), ("q_s0", _i64), ("q_s1", _i64), ("q_s2", _i64),
+                ("out", _p), ("out_s0", _i64), ("out_s1", _i64), ("out_s2", _i64),
+                ("prefix_table", _p), ("prefix_table_len", _i64), ("prefix_table_stride", _i64),
+                ("block_tables", _p), ("block_table_s0", _i64), ("block_table_s1", _i64),
+                ("context_lengths", _p), ("context_length_stride", _i64),
+                ("workspace", _p), ("workspace_bytes", ctypes.c_size_t), ("status", _p),
+                ("q_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int),
+                ("prefix_table_dtype", ctypes.c_int), ("block_table_dtype", ctypes.c_int),
+                ("context_length_dtype", ctypes.c_int), ("reserved", ctypes.c_int32)]
+
+
 class PrefillBatchArgs(ctypes.Structure):
     _fields_ = [("num_seqs", _i64), ("seqs", ctypes.POINTER(PrefillArgs))]
 
@@ -119,6 +133,9 @@ SIGNATURES = {
                                               ctypes.POINTER(ctypes.c_int32)]),
     "b200_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), _p]),
     "b200_rope_kv_append": (ctypes.c_int, [ctypes.POINTER(RopeKvAppendArgs), _p]),
+    "b200_shared_prefix_decode": (ctypes.c_int, [ctypes.POINTER(SharedPrefixArgs), _p]),
+    "b200_shared_prefix_decode_workspace_size": (
+        ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "b200_paged_decode_workspace_size": (
         ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int32]),
     "b200_chunked_prefill_workspace_size": (

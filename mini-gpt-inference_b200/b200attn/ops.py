@@ -121,6 +121,27 @@ class PreparedCall:
         return self._result
 
 
+def _launch(fn, args, device: torch.device, what: str) -> None:
+    """Calls a C entry on the current stream of ``device``, whichever device
+    is the current one."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
+class _DeviceCall(PreparedCall):
+    """A prepared call that may be made while another device is current."""
+
+    def __call__(self):
+        _launch(self._fn, self._args, self._device, self._what)
+        return self._result
+
+
 def _workspace(device: torch.device, stream: int, nbytes: int, private: bool):
     if private:
         return torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device) if nbytes else None

@@ -17,17 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _INDEX, PreparedCall, _index_tensor, _inference_only, _pool_struct
-
-
-class _Call(PreparedCall):
-    """A prepared call that launches on its own device, whichever is current."""
-
-    def __call__(self):
-        if self._device.index != torch.cuda.current_device():
-            with torch.cuda.device(self._device):
-                return super().__call__()
-        return super().__call__()
+from .ops import _DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch, _pool_struct
 
 
 def rope_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0,
@@ -173,9 +163,12 @@ def qk_norm_rope_b200(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     lib = _lib.load()
     args, q_out, k_out = _rope_args(q, k, None, positions, cos_sin, q_weight, k_weight, eps,
                                     interleaved, q_out, k_out, True, status)
-    call = _Call(lib.b200_qk_norm_rope, args, q.device, (q_out, k_out), "head norm and rotation",
-                 (q, k, positions, cos_sin, q_weight, k_weight, status))
-    return call if prepare else call()
+    if prepare:
+        return _DeviceCall(lib.b200_qk_norm_rope, args, q.device, (q_out, k_out),
+                           "head norm and rotation",
+                           (q, k, positions, cos_sin, q_weight, k_weight, status))
+    _launch(lib.b200_qk_norm_rope, args, q.device, "head norm and rotation")
+    return q_out, k_out
 
 
 def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool, slot_mapping,
@@ -215,6 +208,9 @@ def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool,
         raise ValueError("slot_mapping must have shape [T]")
     args = _lib.RopeKvAppendArgs(rope, pstruct, layer_idx, v.data_ptr(), *v.stride(),
                                  slots.data_ptr(), slots.stride(0), _INDEX[slots.dtype], 0)
-    call = _Call(lib.b200_rope_kv_append, args, dev, q_out, "rotary KV append",
-                 (q, k, v, pool.k, pool.v, slots, positions, cos_sin, q_weight, k_weight, status))
-    return call if prepare else call()
+    if prepare:
+        return _DeviceCall(lib.b200_rope_kv_append, args, dev, q_out, "rotary KV append",
+                           (q, k, v, pool.k, pool.v, slots, positions, cos_sin, q_weight, k_weight,
+                            status))
+    _launch(lib.b200_rope_kv_append, args, dev, "rotary KV append")
+    return q_out

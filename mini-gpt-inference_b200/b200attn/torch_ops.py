@@ -22,6 +22,9 @@ C-ABI entry points as :mod:`b200attn.ops`.
                              Tensor slot_mapping, Tensor positions, Tensor cos_sin,
                              int layer_idx, Tensor? q_weight, Tensor? k_weight, float eps,
                              bool interleaved) -> Tensor
+    b200attn::shared_prefix_decode(Tensor q, Tensor k_pool, Tensor v_pool, Tensor prefix_table,
+                                   int prefix_len, Tensor block_tables,
+                                   Tensor context_lengths, int layer_idx) -> Tensor
 
 The pools are the KVBlockPool tensors ``[L, P, S, H, D]`` (S = block size).
 ``paged_decode`` writes k_new/v_new into the pools when they are given
@@ -31,7 +34,8 @@ attention of the chunk (attention.py:215-299). ``qkv_kv_write`` is the bf16
 QKV projection (attention.py:79-83) that stores k and v at ``slot_mapping``
 from its epilogue and returns q as [T, H, D] (attention.py:177-208,
 :360-392). ``qk_norm_rope`` and ``rope_kv_append`` are the head norms and the
-rotation of :mod:`b200attn.rope`. Importing this module registers the ops.
+rotation of :mod:`b200attn.rope`, ``shared_prefix_decode`` the decode of
+:mod:`b200attn.shared_prefix`.  Importing this module registers the ops.
 """
 from __future__ import annotations
 
@@ -41,9 +45,10 @@ from typing import Optional
 import torch
 
 from . import ops, rope
+from .shared_prefix import shared_prefix_decode_b200
 
 __all__ = ["paged_decode", "kv_scatter", "chunked_prefill", "qkv_kv_write", "qk_norm_rope",
-           "rope_kv_append"]
+           "rope_kv_append", "shared_prefix_decode"]
 
 
 def _pool(k_pool: torch.Tensor, v_pool: torch.Tensor) -> SimpleNamespace:
@@ -137,4 +142,17 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: to
 @rope_kv_append.register_fake
 def _(q, k, v, k_pool, v_pool, slot_mapping, positions, cos_sin, layer_idx, q_weight=None,
       k_weight=None, eps=1e-6, interleaved=False):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("b200attn::shared_prefix_decode", mutates_args=())
+def shared_prefix_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                         prefix_table: torch.Tensor, prefix_len: int, block_tables: torch.Tensor,
+                         context_lengths: torch.Tensor, layer_idx: int) -> torch.Tensor:
+    return shared_prefix_decode_b200(q, _pool(k_pool, v_pool), prefix_table, prefix_len,
+                                     block_tables, context_lengths, layer_idx)
+
+
+@shared_prefix_decode.register_fake
+def _(q, k_pool, v_pool, prefix_table, prefix_len, block_tables, context_lengths, layer_idx):
     return torch.empty_like(q, memory_format=torch.contiguous_format)

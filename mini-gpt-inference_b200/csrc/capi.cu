@@ -157,6 +157,43 @@ int check_rope(const b200_qk_norm_rope_args_t& a) {
   return B200_OK;
 }
 
+int check_shared(const b200_shared_prefix_args_t& a) {
+  int rc = check_pool(a.pool, a.layer_idx);
+  if (rc != B200_OK) return rc;
+  B200_CHECK(a.batch >= 1 && a.num_q_heads >= 1, B200_ERR_INVALID_ARGUMENT,
+             "q dimensions must be nonzero");
+  B200_CHECK(a.num_q_heads % a.pool.num_heads == 0, B200_ERR_INVALID_ARGUMENT,
+             "the query heads must be a multiple of the pool's heads");
+  B200_CHECK(a.batch < (int64_t(1) << 24) && a.num_q_heads < (int64_t(1) << 16) &&
+                 a.batch * a.num_q_heads < (int64_t(1) << 26),
+             B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
+  B200_CHECK(a.table_width >= 1, B200_ERR_INVALID_ARGUMENT,
+             "block_tables need at least one block column");
+  B200_CHECK(a.prefix_len >= 0, B200_ERR_INVALID_ARGUMENT, "prefix_len must be >= 0");
+  B200_CHECK(a.prefix_len < (int64_t(1) << 30) && a.table_width < (int64_t(1) << 30),
+             B200_ERR_UNSUPPORTED, "shared prefix: contexts too long");
+  B200_CHECK(a.q != nullptr && a.out != nullptr, B200_ERR_INVALID_ARGUMENT,
+             "q and out must be non-null");
+  B200_CHECK(valid_dtype(a.q_dtype) && valid_dtype(a.out_dtype), B200_ERR_INVALID_ARGUMENT,
+             "q/out dtype must be float32, bfloat16 or float16");
+  if (a.prefix_len > 0) {
+    B200_CHECK(a.prefix_table != nullptr, B200_ERR_INVALID_ARGUMENT, "prefix_table must be non-null");
+    B200_CHECK(valid_index(a.prefix_table_dtype), B200_ERR_INVALID_ARGUMENT,
+               "prefix_table must contain integer indices");
+    B200_CHECK(a.prefix_table_len >= ceil_div(a.prefix_len, a.pool.block_size),
+               B200_ERR_INVALID_ARGUMENT, "incomplete KV block table for prefix");
+  }
+  B200_CHECK(a.block_tables != nullptr && a.context_lengths != nullptr, B200_ERR_INVALID_ARGUMENT,
+             "block_tables and context_lengths must be non-null");
+  B200_CHECK(valid_index(a.block_table_dtype), B200_ERR_INVALID_ARGUMENT,
+             "block_tables must contain integer indices");
+  B200_CHECK(valid_index(a.context_length_dtype), B200_ERR_INVALID_ARGUMENT,
+             "context_lengths must be integer");
+  B200_CHECK(reinterpret_cast<uintptr_t>(a.workspace) % 256 == 0, B200_ERR_WORKSPACE,
+             "shared prefix: the workspace must be 256-byte aligned");
+  return B200_OK;
+}
+
 int sm_count() {
   DeviceInfo dev;
   if (current_device_info(&dev) != B200_OK) return 148;
@@ -302,6 +339,27 @@ int b200_paged_decode(const b200_decode_args_t* args, void* stream) {
   int rc = check_decode(*args);
   if (rc != B200_OK) return rc;
   return launch_paged_decode(*args, static_cast<cudaStream_t>(stream));
+}
+
+int b200_shared_prefix_decode(const b200_shared_prefix_args_t* args, void* stream) {
+  clear_error();
+  if (args == nullptr) return fail(B200_ERR_INVALID_ARGUMENT, "null arguments");
+  int rc = check_shared(*args);
+  if (rc != B200_OK) return rc;
+  return launch_shared_prefix(*args, static_cast<cudaStream_t>(stream));
+}
+
+size_t b200_shared_prefix_decode_workspace_size(int64_t batch, int64_t num_q_heads,
+                                                int64_t num_kv_heads, int64_t head_dim,
+                                                int64_t prefix_len, int64_t table_width,
+                                                int64_t block_size, b200_dtype_t kv_dtype,
+                                                b200_dtype_t q_dtype) {
+  (void)kv_dtype, (void)q_dtype;
+  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1 || prefix_len < 0 ||
+      table_width < 1 || block_size < 1)
+    return 0;
+  return shared_prefix_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, prefix_len,
+                                       table_width, block_size, sm_count());
 }
 
 int b200_chunked_prefill(const b200_prefill_args_t* args, void* stream) {

@@ -1,0 +1,440 @@
+// shared_prefix.cu -- paged decode attention of a batch whose sequences share
+// a prefix: the prefix's keys and values are read once for the whole batch.
+//
+//   out[b, h] = sum_j softmax_j(q[b, h].k_j / sqrt(D)) v_j
+// over the prefix's keys (prefix_table) and the sequence's own (positions
+// prefix .. context_length - 1 of its block table).  The softmax splits: the
+// prefix's part is one product of all B * rep query rows of a key head with
+// the prefix (arithmetic grows with the batch, bytes do not); the own parts
+// are a matrix-vector product per sequence; parts are joined by their running
+// maximum and sum.
+//
+// Element kernels (any pool and query type, exact f32): a tile of R query
+// rows in shared memory, key tiles of 32, thread tiles of scores and outputs
+// in registers, online softmax in the log2 domain.
+#include <math.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "common.cuh"
+#include "host_util.h"
+#include "kernels.h"
+#include "shared_prefix.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kKeys = 32;  // keys per tile of the element kernels
+
+// Thread tile: TR x TC threads, RT rows and kKeys / TC keys (then DP / TC
+// output columns, in float4 groups) each.
+template <int R>
+struct ElemTile;
+template <>
+struct ElemTile<64> {
+  static constexpr int RT = 4, TR = 16, TC = 8;
+};
+template <>
+struct ElemTile<8> {
+  static constexpr int RT = 1, TR = 8, TC = 16;
+};
+
+template <int R, int DP>
+struct ElemSmem {
+  static constexpr int LD = DP + 4;  // row pitch: float4 reads of 8 rows spread over the banks
+  static constexpr int Q = 0, K = Q + R * LD, V = K + kKeys * LD, P = V + kKeys * LD;
+  static constexpr int LP = kKeys + 1;
+  static constexpr int FLOATS = P + R * LP;
+  static constexpr int BYTES = FLOATS * 4;
+};
+
+// One part: R rows (row i of the tile is query row row0 + i of key head g,
+// those from nrows on are empty) over keys [k0, k1) of a page list.
+template <typename KV, int R, int DP>
+struct ElemAttend {
+  using T = ElemTile<R>;
+  using L = ElemSmem<R, DP>;
+  static constexpr int RT = T::RT, TC = T::TC, KPT = kKeys / TC;
+  static constexpr int NG = (DP / 4 + TC - 1) / TC;  // float4 column groups per thread
+  float m[RT], l[RT];
+  float4 o[RT][NG];
+
+  __device__ void run(const SharedParams& p, float* sm, int g, int row0, int nrows, int64_t k0,
+                      int64_t k1, const void* table, int64_t tstride, int ti64, int64_t tlen) {
+    const int tid = threadIdx.x;
+    const int tr = tid / TC, tc = tid % TC;
+    float* Q = sm + L::Q;
+    float* K = sm + L::K;
+    float* V = sm + L::V;
+    float* Pm = sm + L::P;
+    for (int i = tid; i < R * DP; i += 128) {
+      const int r = i / DP, d = i % DP;
+      float x = 0.f;
+      if (r < nrows && d < p.D) {
+        const int row = row0 + r;
+        x = load_elem(p.q, (row / p.rep) * p.qs0 + (g * p.rep + row % p.rep) * p.qs1 + d * p.qs2,
+                      p.q_dtype) * p.qscale;
+      }
+      Q[r * L::LD + d] = x;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NG; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const KV* kp = static_cast<const KV*>(p.k_pool);
+    const KV* vp = static_cast<const KV*>(p.v_pool);
+    constexpr int E = 16 / sizeof(KV);  // elements per 16-byte chunk
+    constexpr int CH = DP / E;          // chunks per row
+
+    for (int64_t key0 = k0; key0 < k1; key0 += kKeys) {
+      __syncthreads();  // the tile before is done with K and V (and Q is there)
+      for (int i = tid; i < kKeys * CH; i += 128) {
+        const int r = i / CH, d0 = (i % CH) * E;
+        const int64_t key = key0 + r;
+        float fk[E], fv[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) fk[e] = fv[e] = 0.f;  // keys past the end, columns past D
+        if (key < k1 && d0 < p.D) {
+          const int64_t page = key >> p.s_shift;
+          int64_t phys = page < tlen ? load_index(table, page * tstride, ti64) : -1;
+          if (phys < 0 || phys >= p.P) {
+            report(p.status, B200_DEV_BAD_BLOCK);
+            phys = 0;  // an in-bounds page; the status word tells
+          }
+          const int64_t at =
+              ((p.layer_row0 + phys * p.S + (key & (p.S - 1))) * p.Hkv + g) * p.D + d0;
+          Elem<KV>::unpack(*reinterpret_cast<const uint4*>(kp + at), fk);
+          Elem<KV>::unpack(*reinterpret_cast<const uint4*>(vp + at), fv);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          *reinterpret_cast<float4*>(K + r * L::LD + d0 + e) =
+              make_float4(fk[e], fk[e + 1], fk[e + 2], fk[e + 3]);
+          *reinterpret_cast<float4*>(V + r * L::LD + d0 + e) =
+              make_float4(fv[e], fv[e + 1], fv[e + 2], fv[e + 3]);
+        }
+      }
+      __syncthreads();
+      // Scores: rows tr * RT + i, keys tc + TC * j.
+      float2 s2[RT][KPT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) s2[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 4
+      for (int d = 0; d < DP; d += 4) {
+        float4 a[RT], b[KPT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          a[i] = *reinterpret_cast<const float4*>(Q + (tr * RT + i) * L::LD + d);
+#pragma unroll
+        for (int j = 0; j < KPT; ++j)
+          b[j] = *reinterpret_cast<const float4*>(K + (tc + TC * j) * L::LD + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < KPT; ++j) {
+            s2[i][j] = ffma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y), s2[i][j]);
+            s2[i][j] = ffma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]);
+          }
+      }
+      const int nkeys = static_cast<int>(min(k1 - key0, static_cast<int64_t>(kKeys)));
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float s[KPT], mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          s[j] = tc + TC * j < nkeys ? s2[i][j].x + s2[i][j].y : -INFINITY;
+          mx = fmaxf(mx, s[j]);
+        }
+#pragma unroll
+        for (int w = TC / 2; w >= 1; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float mn = fmaxf(m[i], mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;  // all scores -inf: p = 0, not NaN
+        const float alpha = exp2f(m[i] - ref);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          const float e = exp2f(s[j] - ref);
+          sum += e;
+          Pm[(tr * RT + i) * L::LP + tc + TC * j] = e;
+        }
+#pragma unroll
+        for (int w = TC / 2; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        l[i] = l[i] * alpha + sum;
+        m[i] = mn;
+#pragma unroll
+        for (int c = 0; c < NG; ++c) {
+          o[i][c].x *= alpha;
+          o[i][c].y *= alpha;
+          o[i][c].z *= alpha;
+          o[i][c].w *= alpha;
+        }
+      }
+      __syncwarp();  // a row's probabilities stay within its warp
+#pragma unroll 4
+      for (int j = 0; j < kKeys; ++j) {
+        float4 v[NG];
+#pragma unroll
+        for (int c = 0; c < NG; ++c)
+          if ((tc + TC * c) * 4 < DP)
+            v[c] = *reinterpret_cast<const float4*>(V + j * L::LD + (tc + TC * c) * 4);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const float pr = Pm[(tr * RT + i) * L::LP + j];
+          const float2 p2 = make_float2(pr, pr);
+#pragma unroll
+          for (int c = 0; c < NG; ++c) {
+            if ((tc + TC * c) * 4 >= DP) continue;
+            const float2 lo = ffma2(p2, make_float2(v[c].x, v[c].y), make_float2(o[i][c].x, o[i][c].y));
+            const float2 hi = ffma2(p2, make_float2(v[c].z, v[c].w), make_float2(o[i][c].z, o[i][c].w));
+            o[i][c] = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
+        }
+      }
+    }
+  }
+
+  // The rows' parts into slot `slot`.
+  __device__ void write(const SharedParams& p, int g, int row0, int nrows, int slot) {
+    const int tr = threadIdx.x / TC, tc = threadIdx.x % TC;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int r = tr * RT + i;
+      if (r >= nrows) continue;
+      const int64_t at = (static_cast<int64_t>(g) * p.rows + row0 + r) * p.ns + slot;
+#pragma unroll
+      for (int c = 0; c < NG; ++c) {
+        const int d = (tc + TC * c) * 4;
+        if (d < p.D) *reinterpret_cast<float4*>(p.acc + at * p.D + d) = o[i][c];
+      }
+      if (tc == 0) {
+        p.ml[at * 2] = m[i];
+        p.ml[at * 2 + 1] = l[i];
+      }
+    }
+  }
+};
+
+// Prefix: CTA (part, row tile, key head).
+template <typename KV, int R, int DP>
+__global__ void __launch_bounds__(128) shared_prefix_elem_kernel(const __grid_constant__ SharedParams p) {
+  extern __shared__ float4 sm4[];
+  float* sm = reinterpret_cast<float*>(sm4);
+  const int part = blockIdx.x, row0 = blockIdx.y * R, g = blockIdx.z;
+  const int64_t k0 = static_cast<int64_t>(part) * p.prefix_per;
+  const int64_t k1 = min(p.prefix, k0 + p.prefix_per);
+  const int nrows = min(R, p.rows - row0);
+  ElemAttend<KV, R, DP> a;
+  a.run(p, sm, g, row0, nrows, k0, k1, p.prefix_table, p.pt_stride, p.pt_i64,
+        (p.prefix + p.S - 1) >> p.s_shift);
+  a.write(p, g, row0, nrows, part);
+}
+
+// Own keys and the join: CTA ((sequence, key head, chunk of 8 rows), part).
+template <typename KV, int DP>
+__global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_constant__ SharedParams p) {
+  constexpr int R = 8;
+  extern __shared__ float4 sm4[];
+  float* sm = reinterpret_cast<float*>(sm4);
+  __shared__ int last;
+  int64_t idx = blockIdx.x;
+  const int split = static_cast<int>(idx % p.own_splits);
+  idx /= p.own_splits;
+  const int64_t unit = idx;
+  const int chunk = static_cast<int>(idx % p.row_chunks);
+  idx /= p.row_chunks;
+  const int g = static_cast<int>(idx % p.Hkv);
+  const int b = static_cast<int>(idx / p.Hkv);
+  const int row0 = b * p.rep + chunk * R;
+  const int nrows = min(R, p.rep - chunk * R);
+  const int64_t ctx = load_index(p.lens, b * p.len_stride, p.lens_i64);
+  if (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S) {
+    if (split == 0) {
+      if (threadIdx.x == 0) report(p.status, B200_DEV_BAD_LENGTH);
+      for (int i = threadIdx.x; i < nrows * p.D; i += 128)
+        store_elem(p.out, b * p.os0 + (g * p.rep + chunk * R + i / p.D) * p.os1 + (i % p.D) * p.os2,
+                   p.out_dtype, 0.f);
+    }
+    return;
+  }
+  int64_t k0, k1;
+  const int parts = own_range(p, ctx - p.prefix, split, &k0, &k1);
+  if (split >= parts) return;
+  ElemAttend<KV, R, DP> a;
+  const int64_t row_bytes = p.tables_i64 ? 8 : 4;
+  a.run(p, sm, g, row0, nrows, p.prefix + k0, p.prefix + k1,
+        static_cast<const char*>(p.tables) + b * p.ts0 * row_bytes, p.ts1, p.tables_i64,
+        p.table_width);
+  a.write(p, g, row0, nrows, p.np + split);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&p.cnt[unit], 1) == parts - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int r = threadIdx.x >> 5; r < nrows; r += 4)
+    join_row(p, g, row0 + r, parts, threadIdx.x & 31, 32);
+}
+
+// ------------------------------------------------------------------ host
+struct SharedPlan {
+  int np, own_splits, own_min, row_chunks;
+  int64_t prefix_per;
+  size_t acc_bytes, ml_bytes, cnt_bytes;
+  size_t bytes() const { return acc_bytes + ml_bytes + cnt_bytes; }
+};
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// The parts of a call, from its sizes alone.
+SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix, int64_t max_own,
+                     int num_sms) {
+  SharedPlan pl{};
+  const int64_t rep = Hq / Hkv, rows = B * rep;
+  // Prefix: parts of whole key tiles that give about two CTAs per SM.
+  pl.np = 0;
+  pl.prefix_per = 0;
+  if (prefix > 0) {
+    const int64_t units = ceil_div(rows, 64) * Hkv;
+    int64_t parts = std::min<int64_t>(ceil_div(2 * num_sms, units), ceil_div(prefix, 4 * kKeys));
+    parts = std::max<int64_t>(1, std::min<int64_t>(parts, 64));
+    pl.prefix_per = ceil_div(ceil_div(prefix, parts), kKeys) * kKeys;
+    pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
+  }
+  // Own keys: enough parts to fill the GPU, none much longer than 1024 keys.
+  pl.row_chunks = static_cast<int>(ceil_div(rep, 8));
+  pl.own_min = 64;
+  const int64_t units = B * Hkv * pl.row_chunks;
+  int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));
+  splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(32)});
+  pl.own_splits = static_cast<int>(std::max<int64_t>(splits, 1));
+  const size_t slots = static_cast<size_t>(Hkv * rows) * (pl.np + pl.own_splits);
+  pl.acc_bytes = round256(slots * D * sizeof(float));
+  pl.ml_bytes = round256(slots * 2 * sizeof(float));
+  pl.cnt_bytes = round256(static_cast<size_t>(units) * sizeof(int32_t));
+  return pl;
+}
+
+// Raises the kernel's shared memory limit once per device (`state` is the
+// kernel's own).
+template <typename Kernel>
+int allow_smem(Kernel kern, int bytes, int device, std::atomic<int>* state) {
+  if (bytes <= 48 * 1024 || device >= 64 || state[device].load(std::memory_order_acquire)) return B200_OK;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
+  state[device].store(1, std::memory_order_release);
+  return B200_OK;
+}
+
+template <typename KV, int DP>
+int launch_elem(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
+  if (pl.np > 0) {
+    const int64_t tiles = ceil_div(p.rows, 64);
+    if (tiles > 65535) return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
+    auto kern = shared_prefix_elem_kernel<KV, 64, DP>;
+    static std::atomic<int> state[64];
+    int rc = allow_smem(kern, ElemSmem<64, DP>::BYTES, device, state);
+    if (rc != B200_OK) return rc;
+    const dim3 grid(static_cast<unsigned>(pl.np), static_cast<unsigned>(tiles),
+                    static_cast<unsigned>(p.Hkv));
+    kern<<<grid, 128, ElemSmem<64, DP>::BYTES, stream>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "shared prefix launch");
+  }
+  const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_chunks * p.own_splits;
+  if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  auto kern = shared_own_elem_kernel<KV, DP>;
+  static std::atomic<int> state[64];
+  int rc = allow_smem(kern, ElemSmem<8, DP>::BYTES, device, state);
+  if (rc != B200_OK) return rc;
+  kern<<<static_cast<unsigned>(grid), 128, ElemSmem<8, DP>::BYTES, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
+}
+
+template <typename KV>
+int launch_elem_d(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
+  if (p.D <= 32) return launch_elem<KV, 32>(p, pl, device, stream);
+  if (p.D <= 64) return launch_elem<KV, 64>(p, pl, device, stream);
+  return launch_elem<KV, 128>(p, pl, device, stream);
+}
+
+}  // namespace
+
+size_t shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix,
+                                     int64_t table_width, int64_t S, int num_sms) {
+  const int64_t own = std::max<int64_t>(table_width * S - prefix, 0);
+  return make_plan(B, Hq, Hkv, D, prefix, own, num_sms).bytes();
+}
+
+int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc != B200_OK) return rc;
+  const int64_t B = a.batch, Hq = a.num_q_heads, Hkv = a.pool.num_heads, D = a.pool.head_dim;
+  const int64_t S = a.pool.block_size;
+  const int64_t own = std::max<int64_t>(a.table_width * S - a.prefix_len, 0);
+  const SharedPlan pl = make_plan(B, Hq, Hkv, D, a.prefix_len, own, dev.num_sms);
+  if (a.workspace == nullptr || a.workspace_bytes < pl.bytes()) {
+    char buf[160];
+    snprintf(buf, sizeof(buf), "shared prefix decode needs %zu workspace bytes, got %zu", pl.bytes(),
+             a.workspace_bytes);
+    return fail(B200_ERR_WORKSPACE, buf);
+  }
+  SharedParams p{};
+  p.q = a.q;
+  p.out = a.out;
+  p.qs0 = a.q_stride[0], p.qs1 = a.q_stride[1], p.qs2 = a.q_stride[2];
+  p.os0 = a.out_stride[0], p.os1 = a.out_stride[1], p.os2 = a.out_stride[2];
+  p.k_pool = a.pool.k;
+  p.v_pool = a.pool.v;
+  p.P = a.pool.num_blocks;
+  p.S = S;
+  p.layer_row0 = a.layer_idx * p.P * S;
+  p.prefix_table = a.prefix_table;
+  p.pt_stride = a.prefix_table_stride;
+  p.pt_i64 = a.prefix_table_dtype == B200_INDEX_I64;
+  p.tables = a.block_tables;
+  p.ts0 = a.block_table_stride[0];
+  p.ts1 = a.block_table_stride[1];
+  p.tables_i64 = a.block_table_dtype == B200_INDEX_I64;
+  p.table_width = a.table_width;
+  p.lens = a.context_lengths;
+  p.len_stride = a.context_length_stride;
+  p.lens_i64 = a.context_length_dtype == B200_INDEX_I64;
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  p.acc = reinterpret_cast<float*>(ws);
+  p.ml = reinterpret_cast<float*>(ws + pl.acc_bytes);
+  p.cnt = reinterpret_cast<int32_t*>(ws + pl.acc_bytes + pl.ml_bytes);
+  p.status = a.status;
+  p.prefix = a.prefix_len;
+  p.B = static_cast<int32_t>(B);
+  p.Hq = static_cast<int32_t>(Hq);
+  p.Hkv = static_cast<int32_t>(Hkv);
+  p.D = static_cast<int32_t>(D);
+  p.rep = static_cast<int32_t>(Hq / Hkv);
+  p.rows = p.B * p.rep;
+  p.s_shift = log2i(S);
+  p.np = pl.np;
+  p.ns = pl.np + pl.own_splits;
+  p.prefix_per = static_cast<int32_t>(pl.prefix_per);
+  p.own_splits = pl.own_splits;
+  p.own_min = pl.own_min;
+  p.row_chunks = pl.row_chunks;
+  p.q_dtype = a.q_dtype;
+  p.out_dtype = a.out_dtype;
+  p.qscale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
+  cudaError_t e = cudaMemsetAsync(p.cnt, 0, pl.cnt_bytes, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(shared prefix counters)");
+  if (a.pool.dtype == B200_DTYPE_F32) return launch_elem_d<float>(p, pl, dev.device, stream);
+  return launch_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
+}
+
+}  // namespace b200
