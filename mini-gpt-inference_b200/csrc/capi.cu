@@ -354,12 +354,11 @@ size_t b200_shared_prefix_decode_workspace_size(int64_t batch, int64_t num_q_hea
                                                 int64_t prefix_len, int64_t table_width,
                                                 int64_t block_size, b200_dtype_t kv_dtype,
                                                 b200_dtype_t q_dtype) {
-  (void)kv_dtype, (void)q_dtype;
   if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1 || prefix_len < 0 ||
       table_width < 1 || block_size < 1)
     return 0;
   return shared_prefix_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, prefix_len,
-                                       table_width, block_size, sm_count());
+                                       table_width, block_size, kv_dtype, q_dtype, sm_count());
 }
 
 int b200_chunked_prefill(const b200_prefill_args_t* args, void* stream) {

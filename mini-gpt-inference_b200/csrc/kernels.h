@@ -43,7 +43,8 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
 // Decode attention with a prefix shared by the batch.
 int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream);
 size_t shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix,
-                                     int64_t table_width, int64_t S, int num_sms);
+                                     int64_t table_width, int64_t S, int kv_dtype, int q_dtype,
+                                     int num_sms);
 int launch_bounded_wait_selftest(int32_t* status, int64_t limit_ns, cudaStream_t stream);
 
 // Split-K planning shared by the launcher and the workspace query.

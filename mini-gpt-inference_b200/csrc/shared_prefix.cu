@@ -295,7 +295,7 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // The parts of a call, from its sizes alone.
 SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix, int64_t max_own,
-                     int num_sms) {
+                     bool mma, int num_sms) {
   SharedPlan pl{};
   const int64_t rep = Hq / Hkv, rows = B * rep;
   // Prefix: parts of whole key tiles that give about two CTAs per SM.
@@ -309,8 +309,8 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   }
   // Own keys: enough parts to fill the GPU, none much longer than 1024 keys.
-  pl.row_chunks = static_cast<int>(ceil_div(rep, 8));
-  pl.own_min = 64;
+  pl.row_chunks = static_cast<int>(ceil_div(rep, mma ? shared_own_rows(rep) : 8));
+  pl.own_min = mma ? 128 : 64;
   const int64_t units = B * Hkv * pl.row_chunks;
   int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));
   splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(32)});
@@ -334,20 +334,22 @@ int allow_smem(Kernel kern, int bytes, int device, std::atomic<int>* state) {
 }
 
 template <typename KV, int DP>
-int launch_elem(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
-  if (pl.np > 0) {
-    const int64_t tiles = ceil_div(p.rows, 64);
-    if (tiles > 65535) return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
-    auto kern = shared_prefix_elem_kernel<KV, 64, DP>;
-    static std::atomic<int> state[64];
-    int rc = allow_smem(kern, ElemSmem<64, DP>::BYTES, device, state);
-    if (rc != B200_OK) return rc;
-    const dim3 grid(static_cast<unsigned>(pl.np), static_cast<unsigned>(tiles),
-                    static_cast<unsigned>(p.Hkv));
-    kern<<<grid, 128, ElemSmem<64, DP>::BYTES, stream>>>(p);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "shared prefix launch");
-  }
+int launch_prefix_elem(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
+  const int64_t tiles = ceil_div(p.rows, 64);
+  if (tiles > 65535) return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
+  auto kern = shared_prefix_elem_kernel<KV, 64, DP>;
+  static std::atomic<int> state[64];
+  int rc = allow_smem(kern, ElemSmem<64, DP>::BYTES, device, state);
+  if (rc != B200_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(pl.np), static_cast<unsigned>(tiles),
+                  static_cast<unsigned>(p.Hkv));
+  kern<<<grid, 128, ElemSmem<64, DP>::BYTES, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix launch");
+}
+
+template <typename KV, int DP>
+int launch_own_elem(const SharedParams& p, int device, cudaStream_t stream) {
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_chunks * p.own_splits;
   if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
   auto kern = shared_own_elem_kernel<KV, DP>;
@@ -360,18 +362,32 @@ int launch_elem(const SharedParams& p, const SharedPlan& pl, int device, cudaStr
 }
 
 template <typename KV>
-int launch_elem_d(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
-  if (p.D <= 32) return launch_elem<KV, 32>(p, pl, device, stream);
-  if (p.D <= 64) return launch_elem<KV, 64>(p, pl, device, stream);
-  return launch_elem<KV, 128>(p, pl, device, stream);
+int launch_prefix_elem_d(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
+  if (p.D <= 32) return launch_prefix_elem<KV, 32>(p, pl, device, stream);
+  if (p.D <= 64) return launch_prefix_elem<KV, 64>(p, pl, device, stream);
+  return launch_prefix_elem<KV, 128>(p, pl, device, stream);
+}
+
+template <typename KV>
+int launch_own_elem_d(const SharedParams& p, int device, cudaStream_t stream) {
+  if (p.D <= 32) return launch_own_elem<KV, 32>(p, device, stream);
+  if (p.D <= 64) return launch_own_elem<KV, 64>(p, device, stream);
+  return launch_own_elem<KV, 128>(p, device, stream);
+}
+
+// bf16 throughout: the products may run on tensor cores.  Queries of other
+// types, and f32 pools, would lose bits there.
+bool use_mma(int kv_dtype, int q_dtype) {
+  return kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16;
 }
 
 }  // namespace
 
 size_t shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix,
-                                     int64_t table_width, int64_t S, int num_sms) {
+                                     int64_t table_width, int64_t S, int kv_dtype, int q_dtype,
+                                     int num_sms) {
   const int64_t own = std::max<int64_t>(table_width * S - prefix, 0);
-  return make_plan(B, Hq, Hkv, D, prefix, own, num_sms).bytes();
+  return make_plan(B, Hq, Hkv, D, prefix, own, use_mma(kv_dtype, q_dtype), num_sms).bytes();
 }
 
 int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream) {
@@ -381,7 +397,8 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   const int64_t B = a.batch, Hq = a.num_q_heads, Hkv = a.pool.num_heads, D = a.pool.head_dim;
   const int64_t S = a.pool.block_size;
   const int64_t own = std::max<int64_t>(a.table_width * S - a.prefix_len, 0);
-  const SharedPlan pl = make_plan(B, Hq, Hkv, D, a.prefix_len, own, dev.num_sms);
+  const bool mma = use_mma(a.pool.dtype, a.q_dtype);
+  const SharedPlan pl = make_plan(B, Hq, Hkv, D, a.prefix_len, own, mma, dev.num_sms);
   if (a.workspace == nullptr || a.workspace_bytes < pl.bytes()) {
     char buf[160];
     snprintf(buf, sizeof(buf), "shared prefix decode needs %zu workspace bytes, got %zu", pl.bytes(),
@@ -433,8 +450,15 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   p.qscale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
   cudaError_t e = cudaMemsetAsync(p.cnt, 0, pl.cnt_bytes, stream);
   if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(shared prefix counters)");
-  if (a.pool.dtype == B200_DTYPE_F32) return launch_elem_d<float>(p, pl, dev.device, stream);
-  return launch_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
+  const bool f32 = a.pool.dtype == B200_DTYPE_F32;
+  if (pl.np > 0) {
+    rc = f32 ? launch_prefix_elem_d<float>(p, pl, dev.device, stream)
+             : launch_prefix_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
+    if (rc != B200_OK) return rc;
+  }
+  if (mma) return launch_shared_own_mma(p, stream);
+  return f32 ? launch_own_elem_d<float>(p, dev.device, stream)
+             : launch_own_elem_d<__nv_bfloat16>(p, dev.device, stream);
 }
 
 }  // namespace b200

@@ -46,6 +46,10 @@ struct SharedParams {
   float qscale;  // log2(e) / sqrt(D)
 };
 
+// Own keys and join, bf16 pool and queries; the rows of a key head one CTA takes.
+int launch_shared_own_mma(const SharedParams& p, cudaStream_t stream);
+int shared_own_rows(int64_t rep);
+
 // Keys [*k0, *k1) of part `split` of a sequence with n own keys; returns the
 // number of parts (at least 1, also for n = 0).
 __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int split, int64_t* k0,
