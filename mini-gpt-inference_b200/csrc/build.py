@@ -24,7 +24,8 @@ BUILD_DIR = PKG_ROOT / "_build"
 
 SOURCES = ["host_util.cu", "capi.cu", "kv_scatter.cu", "paged_decode.cu", "paged_decode_no_alloc.cu",
            "prefill_tc.cu", "qkv_proj.cu", "rope.cu",
-           "shared_prefix.cu", "shared_prefix_own.cu", "selftest.cu"]
+           "shared_prefix.cu", "shared_prefix_own.cu",
+           "shared_prefix_tc.cu", "selftest.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

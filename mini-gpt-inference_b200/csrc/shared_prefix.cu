@@ -285,6 +285,8 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
 
 // ------------------------------------------------------------------ host
 struct SharedPlan {
+  bool mma, tc;  // own keys by warp-level products, prefix on tcgen05
+  TcSplit split;
   int np, own_splits, own_min, row_chunks;
   int64_t prefix_per;
   size_t acc_bytes, ml_bytes, cnt_bytes;
@@ -295,13 +297,21 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // The parts of a call, from its sizes alone.
 SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix, int64_t max_own,
-                     bool mma, int num_sms) {
+                     int64_t S, int kv_dtype, int q_dtype, int num_sms) {
   SharedPlan pl{};
+  // bf16 throughout: the products may run on tensor cores.  Queries of other
+  // types, and f32 pools, would lose bits there.
+  pl.mma = kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16;
+  pl.tc = pl.mma && shared_tc_supported(S) && prefix > 0;
+  const bool mma = pl.mma;
   const int64_t rep = Hq / Hkv, rows = B * rep;
   // Prefix: parts of whole key tiles that give about two CTAs per SM.
   pl.np = 0;
   pl.prefix_per = 0;
-  if (prefix > 0) {
+  if (pl.tc) {
+    pl.split = shared_tc_split(rows, Hkv, prefix, num_sms);
+    pl.np = pl.split.np;
+  } else if (prefix > 0) {
     const int64_t units = ceil_div(rows, 64) * Hkv;
     int64_t parts = std::min<int64_t>(ceil_div(2 * num_sms, units), ceil_div(prefix, 4 * kKeys));
     parts = std::max<int64_t>(1, std::min<int64_t>(parts, 64));
@@ -375,19 +385,13 @@ int launch_own_elem_d(const SharedParams& p, int device, cudaStream_t stream) {
   return launch_own_elem<KV, 128>(p, device, stream);
 }
 
-// bf16 throughout: the products may run on tensor cores.  Queries of other
-// types, and f32 pools, would lose bits there.
-bool use_mma(int kv_dtype, int q_dtype) {
-  return kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16;
-}
-
 }  // namespace
 
 size_t shared_prefix_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix,
                                      int64_t table_width, int64_t S, int kv_dtype, int q_dtype,
                                      int num_sms) {
   const int64_t own = std::max<int64_t>(table_width * S - prefix, 0);
-  return make_plan(B, Hq, Hkv, D, prefix, own, use_mma(kv_dtype, q_dtype), num_sms).bytes();
+  return make_plan(B, Hq, Hkv, D, prefix, own, S, kv_dtype, q_dtype, num_sms).bytes();
 }
 
 int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream) {
@@ -397,8 +401,8 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   const int64_t B = a.batch, Hq = a.num_q_heads, Hkv = a.pool.num_heads, D = a.pool.head_dim;
   const int64_t S = a.pool.block_size;
   const int64_t own = std::max<int64_t>(a.table_width * S - a.prefix_len, 0);
-  const bool mma = use_mma(a.pool.dtype, a.q_dtype);
-  const SharedPlan pl = make_plan(B, Hq, Hkv, D, a.prefix_len, own, mma, dev.num_sms);
+  const SharedPlan pl = make_plan(B, Hq, Hkv, D, a.prefix_len, own, S, a.pool.dtype, a.q_dtype,
+                                  dev.num_sms);
   if (a.workspace == nullptr || a.workspace_bytes < pl.bytes()) {
     char buf[160];
     snprintf(buf, sizeof(buf), "shared prefix decode needs %zu workspace bytes, got %zu", pl.bytes(),
@@ -448,15 +452,23 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   p.q_dtype = a.q_dtype;
   p.out_dtype = a.out_dtype;
   p.qscale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
-  cudaError_t e = cudaMemsetAsync(p.cnt, 0, pl.cnt_bytes, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(shared prefix counters)");
+  // The parts of a sequence's own keys count themselves; the tensor-core
+  // kernel clears the counters on its way.
+  const int counters = pl.mma && pl.own_splits == 1 ? 0 : static_cast<int>(pl.cnt_bytes / sizeof(int32_t));
+  if (counters > 0 && !pl.tc) {
+    cudaError_t e = cudaMemsetAsync(p.cnt, 0, pl.cnt_bytes, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(shared prefix counters)");
+  }
   const bool f32 = a.pool.dtype == B200_DTYPE_F32;
-  if (pl.np > 0) {
+  if (pl.tc) {
+    rc = launch_shared_prefix_tc(p, a.pool, pl.split, counters, stream);
+    if (rc != B200_OK) return rc;
+  } else if (pl.np > 0) {
     rc = f32 ? launch_prefix_elem_d<float>(p, pl, dev.device, stream)
              : launch_prefix_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
     if (rc != B200_OK) return rc;
   }
-  if (mma) return launch_shared_own_mma(p, stream);
+  if (pl.mma) return launch_shared_own_mma(p, stream);
   return f32 ? launch_own_elem_d<float>(p, dev.device, stream)
              : launch_own_elem_d<__nv_bfloat16>(p, dev.device, stream);
 }

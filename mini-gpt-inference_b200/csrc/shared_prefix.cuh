@@ -50,6 +50,19 @@ struct SharedParams {
 int launch_shared_own_mma(const SharedParams& p, cudaStream_t stream);
 int shared_own_rows(int64_t rep);
 
+// The prefix on tensor cores: how its key tiles are cut.
+struct TcSplit {
+  int64_t total;   // key tiles of all units
+  int unit_tiles;  // of one unit (up to 256 rows of a key head)
+  int unit_pairs;  // units per key head
+  int ctas;
+  int np;          // most CTAs that share a unit
+};
+bool shared_tc_supported(int64_t S);
+TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms);
+int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, const TcSplit& t,
+                            int zero_count, cudaStream_t stream);
+
 // Keys [*k0, *k1) of part `split` of a sequence with n own keys; returns the
 // number of parts (at least 1, also for n = 0).
 __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int split, int64_t* k0,

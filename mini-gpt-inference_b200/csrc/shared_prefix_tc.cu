@@ -1,0 +1,659 @@
+// shared_prefix_tc.cu -- the prefix's part of the shared-prefix decode on
+// tcgen05 tensor cores (bf16 pools and queries, block size >= 8).
+//
+// For a key head g the rows q[b, h] of all sequences and of g's query heads
+// form one matrix of B * rep rows: S = Q K^T, P = 2^(S - max), O = P V over
+// the prefix.  A unit is up to 256 of these rows (two tiles of 128) of one key
+// head; its key tiles of 128 are read once for both.  The units' key tiles,
+// end to end, are cut into equal runs, one per CTA and SM, so that every CTA
+// has the same work whatever the batch, heads and prefix are; a run that
+// crosses units is worked off in segments, each of which leaves its rows'
+// unnormalised O, maximum and sum in a slot of the workspace.
+//
+// Roles (12 warps):
+//   warp 0      loads K and V tiles by TMA, page by page, into one ring
+//               (K of a tile, then its V);
+//   warp 1      issues every product.  The tensor pipe runs the products of
+//               one thread in order, so S of the next tile may follow P V of
+//               this one into the same TMEM columns without a wait, and the
+//               barrier that announces S(k + 1) also says that P V(k) is done;
+//   warps 4-7, 8-11  softmax of row tile 0 / 1: thread r owns row r = TMEM
+//               lane r; reads its scores, writes its weights as bf16 over them.
+// While one tile's softmax runs, the tensor pipe works on the other's S and
+// P V.  With at most 128 rows there is one row tile and the two softmax groups
+// take its key tiles in turn, each with its own O; group 0 adds them up.
+//
+// TMEM (512 columns): S_w / P_w at 128 w, O_w at 256 + 128 w.
+// V rows behind the prefix are cleared in shared memory before they are
+// used: unwritten pool rows can hold NaN, and 0 * NaN is NaN.
+// Every wait is bounded; after one runs out all roles leave.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "common.cuh"
+#include "host_util.h"
+#include "kernels.h"
+#include "shared_prefix.cuh"
+#include "tcgen05.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kBM = 128, kBN = 128;
+constexpr int kThreads = 384;
+
+struct TcParams {
+  SharedParams s;
+  int64_t total;    // key tiles of all units
+  int32_t unit_tiles;  // key tiles per unit
+  int32_t unit_pairs;  // units per key head
+  int32_t one_tile;    // at most 128 rows per key head
+  int32_t rbox, rb_shift;
+  int32_t q_vec;
+  int32_t zero_count;  // counters to clear for the own-key kernel
+};
+
+template <int DP>
+struct TcSmem {
+  static constexpr int HALVES = DP / 64;
+  static constexpr int HALF = 128 * 128;       // 128 rows of 128 bytes
+  static constexpr int TILE = HALVES * HALF;   // a row or key tile
+  static constexpr int STAGES = DP == 128 ? 5 : 10;
+  static constexpr int Q0 = 0;
+  static constexpr int RING = 2 * TILE;
+  static constexpr int BAR = RING + STAGES * TILE;
+  static constexpr int ML = BAR + 512;  // float2 [128]: group 1's maximum and sum
+  static constexpr int BYTES = ML + 128 * 8;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Stops the compiler from moving what is computed from x out of a loop.
+__device__ __forceinline__ void keep_here(uint64_t& x) { asm volatile("" : "+l"(x)); }
+
+// Byte offset of 16-byte chunk ch of row r in a 128-byte-swizzled half tile.
+__device__ __forceinline__ uint32_t sw128(int r, int ch) {
+  return static_cast<uint32_t>(r) * 128u + (static_cast<uint32_t>(ch ^ (r & 7)) << 4);
+}
+
+// A CTA's run of key tiles, segment by segment.
+struct Segments {
+  int64_t pos, end;
+  int tiles_per_unit;
+  int unit, j0, n;  // this segment: key tiles [j0, j0 + n) of a unit
+  __device__ Segments(const TcParams& p) {
+    pos = p.total * blockIdx.x / gridDim.x;
+    end = p.total * (blockIdx.x + 1) / gridDim.x;
+    tiles_per_unit = p.unit_tiles;
+  }
+  __device__ bool next() {
+    if (pos >= end) return false;
+    unit = static_cast<int>(pos / tiles_per_unit);
+    j0 = static_cast<int>(pos - static_cast<int64_t>(unit) * tiles_per_unit);
+    n = static_cast<int>(min(static_cast<int64_t>(tiles_per_unit - j0), end - pos));
+    pos += n;
+    return true;
+  }
+};
+
+// The query row `row` of key head g (zeros from `rows` on) into row r of a
+// swizzled tile.
+template <int DP>
+__device__ __forceinline__ void load_q_row(uint8_t* tile, int r, const SharedParams& s, int row, int g,
+                                           int q_vec) {
+  const bool live = row < s.rows;
+  const int b = live ? row / s.rep : 0;
+  const int64_t base = b * s.qs0 + static_cast<int64_t>(g * s.rep + (live ? row - b * s.rep : 0)) * s.qs1;
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q) + base;
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (live && c * 8 < s.D) {
+      if (q_vec) {
+        w = *reinterpret_cast<const uint4*>(q + c * 8);
+      } else {
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 h =
+              __halves2bfloat162(q[(c * 8 + 2 * e) * s.qs2], q[(c * 8 + 2 * e + 1) * s.qs2]);
+          x[e] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        w = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+    }
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * (128 * 128) + sw128(r, c & 7)) = w;
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk,
+                            const __grid_constant__ CUtensorMap tmv, const __grid_constant__ TcParams p) {
+  using L = TcSmem<DP>;
+  constexpr int NS = L::STAGES;
+  const SharedParams& s = p.s;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [NS]
+  uint64_t* empty = full + NS;                                  // [NS]
+  uint64_t* q_full = empty + NS;                                // [2]
+  uint64_t* s_full = q_full + 2;                                // [2]
+  uint64_t* p_full = s_full + 2;                                // [2]
+  uint64_t* o_full = p_full + 2;                                // [2]
+  uint64_t* merge_full = o_full + 2;
+  uint64_t* merge_done = merge_full + 1;
+  uint64_t* idle = merge_done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
+  volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(idle + 2);
+  static_assert((2 * NS + 13) * 8 <= 512, "barrier area too small");
+  float2* ml1 = reinterpret_cast<float2*>(smem + L::ML);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&q_full[w], 128);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_full[w], 1);
+    }
+    mbar_init(merge_full, 128);
+    mbar_init(merge_done, 128);
+    mbar_init(idle, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const bool one = p.one_tile != 0;
+  auto unit_rows = [&](int unit) { return (unit % p.unit_pairs) * 2 * kBM; };  // its first row
+  auto give_up = [&]() {
+    report(s.status, B200_DEV_WAIT_TIMEOUT);
+    *abort_flag = 1;
+  };
+
+  // Registers: 384 threads start with 168 each (64512 in all); 128 x 72 +
+  // 256 x 216 is the same sum.  A softmax thread holds a row of 128 scores.
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    const int box_bytes = 64 * p.rbox * 2;
+    const int boxes_per_tile = kBN / p.rbox;  // <= 16
+    const int64_t table_len = (s.prefix + s.S - 1) >> s.s_shift;
+    uint32_t it = 0;
+    bool ok = true;
+    Segments sg(p);
+    while (ok && sg.next()) {
+      const int g = sg.unit / p.unit_pairs;
+      // Lane i looks up block i of a tile (16 at most), one tile ahead.
+      auto blocks = [&](int j) {
+        return static_cast<int>(min(static_cast<int64_t>(boxes_per_tile),
+                                    (s.prefix - static_cast<int64_t>(j) * kBN + p.rbox - 1) >> p.rb_shift));
+      };
+      auto entry = [&](int j) -> int64_t {
+        if (j >= sg.j0 + sg.n || lane >= blocks(j)) return 0;
+        const int64_t page = (static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift)) >> s.s_shift;
+        return page < table_len ? load_index(s.prefix_table, page * s.pt_stride, s.pt_i64) : -1;
+      };
+      int64_t next = entry(sg.j0);
+      for (int j = sg.j0; ok && j < sg.j0 + sg.n; ++j) {
+        const int nb = blocks(j);
+        int64_t phys = next;
+        next = entry(j + 1);
+        if (lane < nb && (phys < 0 || phys >= s.P)) {
+          report(s.status, B200_DEV_BAD_BLOCK);
+          phys = 0;  // an in-bounds page; the status word tells
+        }
+        const int64_t key = static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift);
+        const int row = static_cast<int>(s.layer_row0 + phys * s.S + (key & (s.S - 1)));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int st = static_cast<int>(it % NS);
+          int good = 1;
+          if (lane == 0) good = mbar_wait(&empty[st], ((it / NS) & 1u) ^ 1u) ? 1 : 0;
+          good = __shfl_sync(0xffffffffu, good, 0);
+          if (!good || *abort_flag) {
+            if (!good && lane == 0) give_up();
+            ok = false;
+            break;
+          }
+          if (lane == 0)
+            mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(nb * L::HALVES * box_bytes));
+          __syncwarp();
+          if (lane < nb) {
+            uint8_t* dst = smem + L::RING + st * L::TILE + lane * p.rbox * 128;
+#pragma unroll
+            for (int h = 0; h < L::HALVES; ++h)
+              tma_load_3d(dst + h * L::HALF, kv == 0 ? &tmk : &tmv, &full[st], h * 64, g, row);
+          }
+        }
+      }
+    }
+    // Copies in flight land before the CTA ends.
+    if (lane == 0) {
+      for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i)
+        if (!mbar_wait(&full[i % NS], (i / NS) & 1u)) {
+          give_up();
+          break;
+        }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ products
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0 && *abort_flag == 0;
+    };
+    constexpr uint32_t idesc_s = idesc_bf16(128, kBN, false);
+    constexpr uint32_t idesc_o = idesc_bf16(128, DP, true);
+    const uint64_t dq0 = smem_desc_sw128(smem_u32(smem + L::Q0), 16, 1024);
+    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::RING), 16, 1024);
+    const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::RING), L::HALF, 1024);
+    uint32_t first = 0;           // ring entry of the segment's first K
+    uint32_t np[2] = {0, 0};      // P tiles of group w awaited so far
+    uint32_t nq[2] = {0, 0};      // Q tiles awaited so far
+    bool ok = true;
+    auto issue_s = [&](int w, int qt, uint32_t entry) {
+      uint64_t dq = dq0 + static_cast<uint64_t>(qt * (L::TILE >> 4));
+      uint64_t dk = dk0 + static_cast<uint64_t>((entry % NS) * (L::TILE >> 4));
+      keep_here(dq);  // the steps' descriptors are not worth registers over the loop
+      keep_here(dk);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * L::HALF + (kk & 3) * 32) >> 4);
+        mma_bf16(tmem + w * 128, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
+      }
+      mma_commit(&s_full[w]);
+    };
+    auto issue_pv = [&](int w, uint32_t entry, bool accumulate) {
+      uint64_t dv = dv0 + static_cast<uint64_t>((entry % NS) * (L::TILE >> 4));
+      keep_here(dv);
+#pragma unroll
+      for (int kk = 0; kk < kBN / 16; ++kk)
+        mma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, dv + static_cast<uint64_t>(kk * 128),
+                    idesc_o, accumulate || kk > 0 ? 1u : 0u);
+    };
+    auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
+    Segments sg(p);
+    while (ok && sg.next()) {
+      const int n = sg.n;
+      const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
+      ok = wait_all(&q_full[0], nq[0]++ & 1u) && (!two || wait_all(&q_full[1], nq[1]++ & 1u));
+      if (!ok) break;
+      tc_fence_after();
+      if (one) {
+        // Group w takes the tiles k = w, w + 2, ...
+        for (int k = 0; ok && k < min(n, 2); ++k) {
+          ok = wait_entry(first + 2 * k);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(k, 0, first + 2 * k);
+          mma_commit(&empty[(first + 2 * k) % NS]);
+        }
+        for (int k = 0; ok && k < n; ++k) {
+          const int w = k & 1;
+          ok = wait_all(&p_full[w], np[w] & 1u) && wait_entry(first + 2 * k + 1);
+          if (!ok) break;
+          ++np[w];
+          tc_fence_after();
+          issue_pv(w, first + 2 * k + 1, k >= 2);
+          mma_commit(&empty[(first + 2 * k + 1) % NS]);
+          if (k + 2 >= n) {
+            mma_commit(&o_full[w]);
+          } else {
+            const uint32_t e = first + 2 * (k + 2);
+            ok = wait_entry(e);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(w, 0, e);
+            mma_commit(&empty[e % NS]);
+          }
+        }
+      } else {
+        const int groups = two ? 2 : 1;
+        ok = wait_entry(first);
+        if (!ok) break;
+        tc_fence_after();
+        for (int w = 0; w < groups; ++w) issue_s(w, w, first);
+        mma_commit(&empty[first % NS]);
+        for (int k = 0; ok && k < n; ++k) {
+          const uint32_t ev = first + 2 * k + 1, ek = ev + 1;
+          for (int w = 0; ok && w < groups; ++w) {
+            ok = wait_all(&p_full[w], np[w] & 1u) && (w > 0 || wait_entry(ev));
+            if (!ok) break;
+            ++np[w];
+            tc_fence_after();
+            issue_pv(w, ev, k > 0);
+            if (w == groups - 1) mma_commit(&empty[ev % NS]);
+            if (k + 1 == n) {
+              mma_commit(&o_full[w]);
+            } else {
+              ok = w > 0 || wait_entry(ek);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(w, w, ek);
+              if (w == groups - 1) mma_commit(&empty[ek % NS]);
+            }
+          }
+        }
+      }
+      first += 2 * n;
+    }
+    if (!ok && lane == 0) give_up();
+    mma_commit(idle);  // every product issued has ended before TMEM is freed
+    if (!__all_sync(0xffffffffu, mbar_wait(idle, 0)) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
+    __syncwarp();
+  } else {
+    // Counters of the kernel that follows on the stream.
+    for (int i = blockIdx.x * 64 + threadIdx.x - 64; i < p.zero_count; i += gridDim.x * 64) s.cnt[i] = 0;
+  }
+  } else {
+    // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int w = (warp - 4) >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
+    const float scale = s.qscale;
+    uint32_t tiles = 0, oseg = 0, mseg = 0;
+    uint32_t first = 0;
+    bool ok = true;
+    Segments sg(p);
+    while (ok && sg.next()) {
+      const int n = sg.n;
+      const int g = sg.unit / p.unit_pairs;
+      const int tile_row0 = unit_rows(sg.unit) + (one ? 0 : w * kBM);
+      const int row = tile_row0 + r;
+      const bool group_live = tile_row0 < s.rows;  // uniform over the group
+      const bool warp_live = tile_row0 + (warp & 3) * 32 < s.rows;
+      const int cnt = one ? (n + 1 - w) / 2 : group_live ? n : 0;
+      // Q: the last segment's S products have all ended (s_full, o_full).
+      if (one ? w == 0 : group_live) {
+        load_q_row<DP>(smem + L::Q0 + w * L::TILE, r, s, row, g, p.q_vec);
+        fence_proxy_async_shared();
+        mbar_arrive(&q_full[w]);
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int k = 0; k < cnt; ++k, ++tiles) {
+        const int jj = one ? 2 * k + w : k;  // tile within the segment
+        if (!mbar_wait(&s_full[w], tiles & 1u) || *abort_flag) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int left = static_cast<int>(  // keys from here on
+            min(s.prefix - static_cast<int64_t>(sg.j0 + jj) * kBN, static_cast<int64_t>(kBN)));
+        if (warp_live) {
+          float v[kBN];
+#pragma unroll
+          for (int c = 0; c < kBN; c += 32) tmem_ld32(ts + c, v + c);
+          tmem_wait_ld();
+          if (left < kBN) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c)
+              if (c >= left) v[c] = -INFINITY;
+          }
+          float mp[8];
+#pragma unroll
+          for (int a = 0; a < 8; ++a) mp[a] = fmaxf(v[2 * a], v[2 * a + 1]);
+#pragma unroll
+          for (int c = 16; c < kBN; c += 16)
+#pragma unroll
+            for (int a = 0; a < 8; ++a) mp[a] = max3(mp[a], v[c + 2 * a], v[c + 2 * a + 1]);
+          const float mx =
+              scale * max3(max3(mp[0], mp[1], mp[2]), max3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
+          // The reference point moves only when the maximum exceeds it by
+          // more than 2^8; O follows (P V of the tile before has ended).
+          float m_new = m, alpha = 1.f;
+          if (mx > m + 8.f) {
+            m_new = mx;
+            alpha = m == -INFINITY ? 0.f : ex2(m - mx);
+          }
+          if (k > 0 && __any_sync(0xffffffffu, m_new != m)) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              tmem_ld32(to + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              tmem_st32(to + c, o);
+            }
+          }
+          m = m_new;
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-ref, -ref);
+          const float2 one2 = make_float2(1.f, 1.f);
+          float2 sum[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) sum[a] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < kBN; c += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 x = ffma2(make_float2(v[c + e], v[c + e + 1]), sc2, nm2);
+              const float2 q = make_float2(ex2(x.x), ex2(x.y));
+              sum[(e >> 1) & 3] = ffma2(q, one2, sum[(e >> 1) & 3]);
+              // bf16 for the product alone; the sum keeps the weights whole.
+              pk[e >> 1] = pack_bf16(q.x, q.y);
+            }
+            tmem_st16(ts + (c >> 1), pk);
+          }
+          const float add = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
+                            ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+          l = l * alpha + add;
+          tmem_wait_st();
+        }
+        if (left < kBN && (one || w == 0)) {
+          const uint32_t e = first + 2 * jj + 1;
+          if (!mbar_wait(&full[e % NS], (e / NS) & 1u)) {
+            ok = false;
+            break;
+          }
+          if (r >= left) {
+            uint8_t* vrow = smem + L::RING + (e % NS) * L::TILE + r * 128;
+#pragma unroll
+            for (int h = 0; h < L::HALVES; ++h)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(vrow + h * L::HALF + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_shared();
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+      }
+      if (ok && cnt > 0) {
+        ok = mbar_wait(&o_full[w], oseg & 1u) && *abort_flag == 0;
+        ++oseg;
+        tc_fence_after();
+      }
+      if (!ok) break;
+      // Slot of this CTA among those that share the unit.
+      const int64_t a = static_cast<int64_t>(sg.unit) * p.unit_tiles;
+      const int slot = static_cast<int>(blockIdx.x - ((a + 1) * gridDim.x - 1) / p.total);
+      float f0 = 1.f, f1 = 0.f;
+      if (one && n >= 2) {
+        // Group 1's O, maximum and sum are added to group 0's.
+        if (w == 1) {
+          ml1[r] = make_float2(m, l);
+          mbar_arrive(merge_full);
+        } else {
+          ok = mbar_wait(merge_full, mseg & 1u) && *abort_flag == 0;
+          if (!ok) break;
+          const float2 o = ml1[r];
+          const float mm = fmaxf(m, o.x);
+          f0 = m == -INFINITY ? 0.f : ex2(m - mm);
+          f1 = o.x == -INFINITY ? 0.f : ex2(o.x - mm);
+          m = mm;
+          l = l * f0 + o.y * f1;
+        }
+      }
+      if (warp_live && (one ? w == 0 : group_live)) {
+        const int64_t at = (static_cast<int64_t>(g) * s.rows + row) * s.ns + slot;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          tmem_ld32(to + c, o);
+          if (one && n >= 2) {
+            float o1[32];
+            tmem_ld32(to + 128 + c, o1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
+          } else {
+            tmem_wait_ld();
+          }
+          if (row < s.rows) {
+            float* dst = s.acc + at * s.D + c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < s.D) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (row < s.rows) {
+          s.ml[at * 2] = m;
+          s.ml[at * 2 + 1] = l;
+          // The unit's last segment also marks the slots that stay unused.
+          if (sg.j0 + n == p.unit_tiles)
+            for (int i = slot + 1; i < s.np; ++i) {
+              s.ml[(at + i - slot) * 2] = -INFINITY;
+              s.ml[(at + i - slot) * 2 + 1] = 0.f;
+            }
+        }
+      }
+      if (one && n >= 2) {
+        // Group 1 may write its O again once group 0 has read it.
+        if (w == 0) {
+          tc_fence_before();
+          mbar_arrive(merge_done);
+        } else {
+          ok = mbar_wait(merge_done, mseg & 1u) && *abort_flag == 0;
+          tc_fence_after();
+        }
+        ++mseg;
+      }
+      first += 2 * n;
+    }
+    if (!ok) {
+      report(s.status, B200_DEV_WAIT_TIMEOUT);
+      *abort_flag = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+template <int DP>
+int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const DeviceInfo& dev,
+           cudaStream_t stream) {
+  const int smem = TcSmem<DP>::BYTES + 1024;
+  if (smem > dev.max_smem_optin)
+    return fail(B200_ERR_UNSUPPORTED, "shared prefix: not enough shared memory");
+  CUtensorMap tk, tv;
+  const uint64_t dims[3] = {static_cast<uint64_t>(pool.head_dim), static_cast<uint64_t>(pool.num_heads),
+                            static_cast<uint64_t>(pool.num_layers * pool.num_blocks * pool.block_size)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(pool.head_dim * 2),
+                               static_cast<uint64_t>(pool.num_heads * pool.head_dim * 2)};
+  const uint32_t box[3] = {64u, 1u, static_cast<uint32_t>(p.rbox)};
+  int rc = encode_tensor_map(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.k, dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != B200_OK) return rc;
+  rc = encode_tensor_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.v, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != B200_OK) return rc;
+  static std::atomic<int> configured[64];
+  if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(shared_prefix_tc_kernel<DP>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
+    if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
+  }
+  shared_prefix_tc_kernel<DP><<<static_cast<unsigned>(ctas), kThreads, smem, stream>>>(tk, tv, p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix launch");
+}
+
+}  // namespace
+
+bool shared_tc_supported(int64_t S) { return S >= 8; }
+
+// One CTA per SM, at least two key tiles and at most kMaxParts CTAs to a unit
+// (each leaves a part that the join reads).
+TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) {
+  constexpr int64_t kMinTiles = 2, kMaxParts = 32;
+  TcSplit t{};
+  t.unit_pairs = static_cast<int>(ceil_div(rows, 2 * kBM));
+  t.unit_tiles = static_cast<int>(ceil_div(prefix, kBN));
+  const int64_t units = Hkv * t.unit_pairs;
+  t.total = units * t.unit_tiles;
+  const int64_t ctas = std::min<int64_t>({static_cast<int64_t>(num_sms), ceil_div(t.total, kMinTiles),
+                                          units * kMaxParts});
+  t.ctas = static_cast<int>(std::max<int64_t>(ctas, 1));
+  // Parts of a unit: each of its CTAs but the first and last has at least
+  // total / ctas of its tiles.
+  const int64_t least = t.total / t.ctas;
+  t.np = static_cast<int>(std::min<int64_t>(ceil_div(t.unit_tiles - 1, least) + 1, t.ctas));
+  if (units <= 1024) {
+    int64_t most = 1;
+    for (int64_t u = 0; u < units; ++u) {
+      const int64_t c0 = ((u * t.unit_tiles + 1) * t.ctas - 1) / t.total;
+      const int64_t c1 = ((u + 1) * t.unit_tiles * t.ctas - 1) / t.total;
+      most = std::max(most, c1 - c0 + 1);
+    }
+    t.np = static_cast<int>(most);
+  }
+  return t;
+}
+
+int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, const TcSplit& t,
+                            int zero_count, cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc != B200_OK) return rc;
+  TcParams p{};
+  p.s = s;
+  p.total = t.total;
+  p.unit_tiles = t.unit_tiles;
+  p.unit_pairs = t.unit_pairs;
+  p.one_tile = s.rows <= kBM;
+  p.rbox = static_cast<int32_t>(std::min<int64_t>(s.S, kBN));
+  p.rb_shift = log2i(p.rbox);
+  p.q_vec = s.qs2 == 1 && reinterpret_cast<uintptr_t>(s.q) % 16 == 0 && s.qs0 % 8 == 0 && s.qs1 % 8 == 0;
+  p.zero_count = zero_count;
+  if (s.D <= 64) return launch<64>(p, pool, t.ctas, dev, stream);
+  return launch<128>(p, pool, t.ctas, dev, stream);
+}
+
+}  // namespace b200
