@@ -301,8 +301,9 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
   SharedPlan pl{};
   // bf16 throughout: the products may run on tensor cores.  Queries of other
   // types, and f32 pools, would lose bits there.
-  pl.mma = kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16;
-  pl.tc = pl.mma && shared_tc_supported(S) && prefix > 0;
+  // (Pages of fewer than 8 tokens would make swizzled boxes of less than 1 KB.)
+  pl.mma = kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16 && S >= 8;
+  pl.tc = pl.mma && prefix > 0;
   const bool mma = pl.mma;
   const int64_t rep = Hq / Hkv, rows = B * rep;
   // Prefix: parts of whole key tiles that give about two CTAs per SM.
@@ -468,7 +469,7 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
              : launch_prefix_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
     if (rc != B200_OK) return rc;
   }
-  if (pl.mma) return launch_shared_own_mma(p, stream);
+  if (pl.mma) return launch_shared_own_mma(p, a.pool, stream);
   return f32 ? launch_own_elem_d<float>(p, dev.device, stream)
              : launch_own_elem_d<__nv_bfloat16>(p, dev.device, stream);
 }

@@ -47,7 +47,7 @@ struct SharedParams {
 };
 
 // Own keys and join, bf16 pool and queries; the rows of a key head one CTA takes.
-int launch_shared_own_mma(const SharedParams& p, cudaStream_t stream);
+int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, cudaStream_t stream);
 int shared_own_rows(int64_t rep);
 
 // The prefix on tensor cores: how its key tiles are cut.
@@ -58,7 +58,6 @@ struct TcSplit {
   int ctas;
   int np;          // most CTAs that share a unit
 };
-bool shared_tc_supported(int64_t S);
 TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms);
 int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, const TcSplit& t,
                             int zero_count, cudaStream_t stream);

@@ -3,22 +3,20 @@
 //
 // For the rep query rows of one (sequence, key head) this is a matrix-vector
 // product per row: bound by the bytes of K and V, each read once for all rep
-// rows.  Warp-level matrix products keep the arithmetic out of the way with
-// few instructions per byte, and are arranged so that every operand comes from
-// global memory straight into registers, 16 bytes a load, with no staging:
-//   S^T = K Q^T   (16 keys x 8 rows): the sum over d may run in any order, so
-//       a lane takes 16-byte chunks of a key's row as they lie; the query's
-//       fragment holds the same chunks.
-//   O^T = V^T P^T (16 d x 8 rows): a lane loads the same 8 d of four keys and
-//       pairs them up with byte permutes; the rows of an O^T tile are those d.
-// P^T comes from S^T by an 8x8 transpose within the warp.  Rows from rep on
-// are zero queries whose results are dropped.
+// rows.  Warp-level matrix products keep the arithmetic out of the way:
+//   S^T = K Q^T   (16 keys x 8 rows),   O^T = V^T P^T  (16 d x 8 rows)
+// have the keys and the d on the 16-wide side, so that a group of 8 rows
+// fills the other; rows from rep on are zero queries whose results are
+// dropped.  P^T comes from S^T by an 8x8 transpose within the warp.
 //
-// A warp works on 16 keys at a time, four warps side by side; the next step's
-// K is requested when this step's scores are done, its V when the outputs
-// are, its table entries a step earlier, so that loads are in flight all the
-// time (8 KB a warp at D = 128).
+// What bounds it is the bytes in flight: a row of one head is 256 bytes in a
+// place of its own.  Each of the four warps takes every fourth step of 16
+// keys, has its own ring of stages (K and V of a step, 8 KB at D = 128) filled
+// by TMA page by page, and needs no other warp until the end.  A first version
+// that loaded its operands straight into registers had no room for more than
+// one step a warp: 2.5 TB/s at 64 sequences of 32 heads, against <ring> here.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -30,7 +28,8 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStep = 16;  // keys a warp takes at a time
+constexpr int kStep = 16;      // keys a warp takes at a time
+constexpr int kMaxSlots = 72;  // parts of a row: 33 of the prefix, 32 own ones, 4 warps
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -39,13 +38,25 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // c += a b: 16 x 16 by 16 x 8, bf16 with f32 sums.
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -54,32 +65,45 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint4 load_chunk(const uint8_t* p, bool ok) {
-  return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-}
-
 struct OwnParams {
   SharedParams s;
-  int32_t q_vec, out_vec;  // 16-byte access to rows of q / bf16 out is legal
+  int32_t rbox, rb_shift;  // rows per TMA box: min(S, 16)
+  int32_t q_vec;           // 4-byte access to pairs of q is legal
+  int32_t out_vec;         // 8-byte access to four elements of bf16 out is legal
+};
+
+template <int DP, int NQ>
+struct OwnSmem {
+  static constexpr int HALVES = DP / 64;
+  static constexpr int HALF = kStep * 128;        // 16 keys x 64 d
+  static constexpr int TILE = HALVES * HALF;      // K or V of a step
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int STAGES = DP == 128 ? 3 : 6;
+  static constexpr int RING = kWarps * STAGES * STAGE;
+  static constexpr int R = 8 * NQ;
+  static constexpr int LD = DP + 4;               // 2 LD = 8 mod 32: no bank is hit twice
+  static constexpr int MERGE = kWarps * R * LD * 4;  // the warps' O, over the ring
+  static constexpr int BAR = RING > MERGE ? RING : MERGE;
+  static constexpr int ML = BAR + kWarps * STAGES * 8;  // float2 [kMaxSlots][R]
+  static constexpr int BYTES = ML + kMaxSlots * R * 8 + 16;
+  static_assert(RING % 1024 == 0 && STAGE % 1024 == 0, "swizzled tiles start on 1024 bytes");
 };
 
 // NQ groups of 8 query rows; DP: head dimension rounded up to 64 or 128.
 template <int DP, int NQ>
-__global__ void __launch_bounds__(kWarps * 32, NQ == 1 ? 3 : 2)
-    shared_own_mma_kernel(const __grid_constant__ OwnParams op) {
-  constexpr int KC = DP / 32;  // K chunks per lane and row
-  constexpr int VH = DP / 64;  // V chunks per lane and key
-  constexpr int R = 8 * NQ;
-  constexpr int LD = DP + 8;
-  __shared__ float s_o[kWarps][R][LD];
-  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
-  __shared__ int s_last;
+__global__ void __launch_bounds__(kWarps * 32)
+    shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
+                          const __grid_constant__ CUtensorMap tmv, const __grid_constant__ OwnParams op) {
+  using L = OwnSmem<DP, NQ>;
+  constexpr int NS = L::STAGES, R = L::R;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const SharedParams& p = op.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gq = lane >> 2, t = lane & 3;  // fragment row and column pair
 
-  // Heads fastest, then parts: CTAs that run together read neighbouring
-  // columns of the same pages.
+  // Heads fastest: CTAs that run together read neighbouring columns of the
+  // same pages.
   int64_t idx = blockIdx.x;
   const int g = static_cast<int>(idx % p.Hkv);
   idx /= p.Hkv;
@@ -89,349 +113,383 @@ __global__ void __launch_bounds__(kWarps * 32, NQ == 1 ? 3 : 2)
   const int b = static_cast<int>(idx / p.own_splits);
   const int row0 = b * p.rep + chunk * R;
   const int nrows = min(R, p.rep - chunk * R);
+  const int head0 = g * p.rep + chunk * R;
   const int64_t ctx = load_index(p.lens, b * p.len_stride, p.lens_i64);
   if (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S) {
     if (split == 0) {
       if (threadIdx.x == 0) report(p.status, B200_DEV_BAD_LENGTH);
       for (int i = threadIdx.x; i < nrows * p.D; i += kWarps * 32)
-        store_elem(p.out, b * p.os0 + (g * p.rep + chunk * R + i / p.D) * p.os1 + (i % p.D) * p.os2,
-                   p.out_dtype, 0.f);
+        store_elem(p.out, b * p.os0 + (head0 + i / p.D) * p.os1 + (i % p.D) * p.os2, p.out_dtype, 0.f);
     }
     return;
   }
-  int64_t k0, k1;
-  const int parts = own_range(p, ctx - p.prefix, split, &k0, &k1);
+  // Steps lie on multiples of 16 positions, so that no step's box leaves its
+  // page; the keys outside [lo, hi) of the first and last one are masked.
+  const int64_t origin = p.prefix & ~int64_t(kStep - 1);
+  int64_t k0, hi;
+  const int parts = own_range(p, ctx > p.prefix ? ctx - origin : 0, split, &k0, &hi);
   if (split >= parts) return;
-  k0 += p.prefix;
-  k1 += p.prefix;
+  k0 += origin;
+  hi += origin;
+  const int64_t lo = max(k0, p.prefix);
+  const int steps = static_cast<int>((hi - k0 + kStep - 1) / kStep);
+  const int mine = (steps - warp + kWarps - 1) / kWarps;  // of this warp: warp, warp + 4, ...
 
-  // Table entry -> pool row of key base + lane (lanes 0..15), -1 past the end.
-  auto entry = [&](int64_t base) -> int64_t {
-    const int64_t key = base + lane;
-    if (lane >= kStep || key >= k1) return -1;
-    return load_index(p.tables, b * p.ts0 + (key >> p.s_shift) * p.ts1, p.tables_i64);
-  };
-  auto row_of = [&](int64_t base, int64_t e) -> int {
-    const int64_t key = base + lane;
-    if (lane >= kStep || key >= k1) return -1;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR) + warp * NS;
+  uint8_t* ring = smem + warp * (NS * L::STAGE);
+  if (lane < NS) mbar_init(&full[lane], 1);
+  fence_mbar_init();
+  __syncwarp();
+
+  // Boxes of step n: nb of them, box i holding keys first + i * rbox.  A lane
+  // keeps the pool row of box (lane % nb) of step (batch + lane / nb).
+  const int nb = kStep >> op.rb_shift;
+  const int per_batch = 32 / nb;
+  auto lookup = [&](int n) -> int {  // for lane's step n + lane / nb
+    const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * (n + lane / nb)) * kStep +
+                        ((lane % nb) << op.rb_shift);
+    if (n + lane / nb >= mine || key >= hi || key + op.rbox <= lo) return -1;
+    int64_t e = load_index(p.tables, b * p.ts0 + (key >> p.s_shift) * p.ts1, p.tables_i64);
     if (e < 0 || e >= p.P) {
       report(p.status, B200_DEV_BAD_BLOCK);
       e = 0;  // an in-bounds page; the status word tells
     }
     return static_cast<int>(p.layer_row0 + e * p.S + (key & (p.S - 1)));
   };
-  const int64_t row_bytes = static_cast<int64_t>(p.Hkv) * p.D * 2;
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k_pool) + static_cast<int64_t>(g) * p.D * 2;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v_pool) + static_cast<int64_t>(g) * p.D * 2;
-  const int nchunks = p.D / 8;
-
-  uint4 kf[2][KC], vf[4][VH];
-  auto load_k = [&](int row) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = __shfl_sync(0xffffffffu, row, gq + 8 * h);
-      const uint8_t* src = kbase + r * row_bytes + t * 16;
-#pragma unroll
-      for (int i = 0; i < KC; ++i) kf[h][i] = load_chunk(src + i * 64, r >= 0 && t + 4 * i < nchunks);
+  int rows = lookup(0);
+  int rows_next = mine > per_batch ? lookup(per_batch) : -1;
+  int batch = 0;
+  auto issue = [&](int n) {
+    if (n >= batch + per_batch) {
+      batch += per_batch;
+      rows = rows_next;
+      rows_next = batch + per_batch < mine ? lookup(batch + per_batch) : -1;
     }
+    const int st = n % NS;
+    // Lane: box, half, K or V.
+    const int box = lane % nb, rest = lane / nb;
+    const int half = rest % L::HALVES, kv = rest / L::HALVES;
+    const int row = __shfl_sync(0xffffffffu, rows, (n - batch) * nb + box);
+    const unsigned there = __ballot_sync(0xffffffffu, lane < nb && row >= 0);
+    if (lane == 0)
+      mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(__popc(there) * 2 * L::HALVES * op.rbox * 128));
+    __syncwarp();
+    if (kv < 2 && row >= 0)
+      tma_load_3d(ring + st * L::STAGE + kv * L::TILE + half * L::HALF + box * op.rbox * 128,
+                  kv == 0 ? &tmk : &tmv, &full[st], half * 64, g, row);
   };
-  auto load_v = [&](int row) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = __shfl_sync(0xffffffffu, row, 2 * t + (j & 1) + 8 * (j >> 1));
-      const uint8_t* src = vbase + r * row_bytes + gq * 16;
-#pragma unroll
-      for (int h = 0; h < VH; ++h) vf[j][h] = load_chunk(src + h * 128, r >= 0 && gq + 8 * h < nchunks);
-    }
-  };
+  int issued = min(mine, NS);
+  for (int n = 0; n < issued; ++n) issue(n);
 
-  int64_t base = k0 + warp * kStep;
-  int row = -1;
-  int64_t e_next = -1;
-  if (base < k1) {
-    row = row_of(base, entry(base));
-    load_k(row);
-    load_v(row);
-    e_next = entry(base + kWarps * kStep);
-  }
-
-  // Query fragments: row 8n + gq, the chunks t + 4i.
-  uint4 qf[NQ][KC];
+  // Query fragments: row 8n + gq, d = 16 i + 2t + {0, 1} and + 8.
+  uint32_t qf[NQ][DP / 16][2];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = 8 * n + gq;
+  for (int n = 0; n < NQ; ++n)
 #pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const int c = t + 4 * i;
-      qf[n][i] = make_uint4(0, 0, 0, 0);
-      if (r < nrows && c < nchunks) {
-        const int64_t at = b * p.qs0 + (g * p.rep + chunk * R + r) * p.qs1 + c * 8 * p.qs2;
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q);
-        if (op.q_vec) {
-          qf[n][i] = *reinterpret_cast<const uint4*>(q + at);
-        } else {
-          uint32_t w[4];
+    for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __nv_bfloat162 x = __halves2bfloat162(q[at + 2 * e * p.qs2], q[at + (2 * e + 1) * p.qs2]);
-            w[e] = *reinterpret_cast<const uint32_t*>(&x);
+      for (int u = 0; u < 2; ++u) {
+        const int r = 8 * n + gq, d = 16 * i + 2 * t + 8 * u;
+        uint32_t x = 0;
+        if (r < nrows && d < p.D) {
+          const __nv_bfloat16* q =
+              static_cast<const __nv_bfloat16*>(p.q) + b * p.qs0 + (head0 + r) * p.qs1 + d * p.qs2;
+          if (op.q_vec) {
+            x = *reinterpret_cast<const uint32_t*>(q);
+          } else {
+            const __nv_bfloat162 h = __halves2bfloat162(q[0], q[p.qs2]);
+            x = *reinterpret_cast<const uint32_t*>(&h);
           }
-          qf[n][i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        qf[n][i][u] = x;
       }
-    }
-  }
 
-  // Row 8n + 2t + u: m[n][u] (the same in its 8 lanes) and this lane's l.
-  float m[NQ][2], l[NQ][2], o[NQ][VH][4][4];
+  // Row 8n + 2t + u: m[n][u] (the same in its 8 lanes) and this lane's l;
+  // o[n][i]: d = 16 i + gq (+ 8) of rows 2t, 2t + 1.
+  float m[NQ][2], l[NQ][2], o[NQ][DP / 16][4];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     m[n][0] = m[n][1] = -INFINITY;
     l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-    for (int h = 0; h < VH; ++h)
+    for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][h][j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
   }
-  // New maxima mn for the rows of group n: l and o follow.
-  auto rescale = [&](int n, float mn0, float mn1) {
-    const float a0 = m[n][0] == -INFINITY ? 0.f : ex2(m[n][0] - mn0);
-    const float a1 = m[n][1] == -INFINITY ? 0.f : ex2(m[n][1] - mn1);
-    m[n][0] = mn0;
-    m[n][1] = mn1;
-    l[n][0] *= a0;
-    l[n][1] *= a1;
-#pragma unroll
-    for (int h = 0; h < VH; ++h)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[n][h][j][0] *= a0;
-        o[n][h][j][1] *= a1;
-        o[n][h][j][2] *= a0;
-        o[n][h][j][3] *= a1;
-      }
-  };
+  // Byte offsets of this lane's ldmatrix row and its chunk's swizzle.  K: keys
+  // (lane & 15), chunks 2 i + (lane >> 4); V: keys (lane & 7) + 8 (lane >> 4),
+  // chunks 2 i + (lane >> 3 & 1).
+  const uint32_t k_row = (lane & 15) * 128, k_hi = lane >> 4;
+  const uint32_t v_row = ((lane & 7) + 8 * (lane >> 4)) * 128, v_hi = (lane >> 3) & 1;
+  const uint32_t sw = lane & 7;
 
-  for (; base < k1; base += kWarps * kStep) {
-    float s[NQ][4];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        mma16816(s[n], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, qf[n][i].x, qf[n][i].y);
-        mma16816(s[n], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, qf[n][i].z, qf[n][i].w);
-      }
+  bool ok = true;
+  for (int n = 0; n < mine; ++n) {
+    const int st = n % NS;
+    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], static_cast<uint32_t>(n / NS) & 1u))) {
+      ok = false;
+      break;
     }
-    const int64_t next = base + kWarps * kStep;
-    int row_next = -1;
-    if (next < k1) {
-      row_next = row_of(next, e_next);
-      load_k(row_next);
-      e_next = entry(next + kWarps * kStep);
+    const uint32_t kt = smem_u32(ring + st * L::STAGE), vt = kt + L::TILE;
+    float s[NQ][2][4];  // two chains of products
+#pragma unroll
+    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[c][e >> 2][e & 3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      uint32_t a[4];
+      const uint32_t ch = (2 * i + k_hi) & 7;
+      ldmatrix4(a, kt + (i / 4) * L::HALF + k_row + ((ch ^ sw) << 4));
+#pragma unroll
+      for (int c = 0; c < NQ; ++c) mma16816(s[c][i & 1], a, qf[c][i][0], qf[c][i][1]);
     }
-    const bool in0 = base + gq < k1, in1 = base + gq + 8 < k1;
+    const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * n) * kStep;
+    const bool edge = key < lo || key + kStep > hi;
+    const bool in0 = !edge || (key + gq >= lo && key + gq < hi);
+    const bool in1 = !edge || (key + gq + 8 >= lo && key + gq + 8 < hi);
     uint32_t pb[NQ][2];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
+    for (int c = 0; c < NQ; ++c) {
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (e < 2 ? in0 : in1) ? s[n][e] * p.qscale : -INFINITY;
+      for (int e = 0; e < 4; ++e)
+        x[e] = (e < 2 ? in0 : in1) ? (s[c][0][e] + s[c][1][e]) * p.qscale : -INFINITY;
       const float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
       // The reference point moves only when a score exceeds it by more than
-      // 2^8: weights stay below 2^8 and the parts' exact l and o follow it.
-      if (__any_sync(0xffffffffu, mx0 > m[n][0] + 8.f || mx1 > m[n][1] + 8.f)) {
+      // 2^8: weights stay below 2^8 and l and o stay exact relative to it.
+      if (__any_sync(0xffffffffu, mx0 > m[c][0] + 8.f || mx1 > m[c][1] + 8.f)) {
         float r0 = mx0, r1 = mx1;
 #pragma unroll
         for (int w = 4; w <= 16; w <<= 1) {
           r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, w));
           r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, w));
         }
-        rescale(n, fmaxf(m[n][0], r0), fmaxf(m[n][1], r1));
+        r0 = fmaxf(m[c][0], r0);
+        r1 = fmaxf(m[c][1], r1);
+        const float a0 = m[c][0] == -INFINITY ? 0.f : ex2(m[c][0] - r0);
+        const float a1 = m[c][1] == -INFINITY ? 0.f : ex2(m[c][1] - r1);
+        m[c][0] = r0;
+        m[c][1] = r1;
+        l[c][0] *= a0;
+        l[c][1] *= a1;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          o[c][i][0] *= a0;
+          o[c][i][1] *= a1;
+          o[c][i][2] *= a0;
+          o[c][i][3] *= a1;
+        }
       }
-      const float ref0 = m[n][0] == -INFINITY ? 0.f : m[n][0];
-      const float ref1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+      const float ref0 = m[c][0] == -INFINITY ? 0.f : m[c][0];
+      const float ref1 = m[c][1] == -INFINITY ? 0.f : m[c][1];
       const float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
       const float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
-      l[n][0] += p0 + p2;
-      l[n][1] += p1 + p3;
+      l[c][0] += p0 + p2;
+      l[c][1] += p1 + p3;
       // The weights are rounded to bf16 for the product alone; l keeps them whole.
-      pb[n][0] = transpose8x8(pack_bf16(p0, p1));
-      pb[n][1] = transpose8x8(pack_bf16(p2, p3));
+      pb[c][0] = transpose8x8(pack_bf16(p0, p1));
+      pb[c][1] = transpose8x8(pack_bf16(p2, p3));
+    }
+    // V rows of masked keys may hold anything, and 0 * NaN is NaN.
+    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+    if (edge) {
+      auto in = [&](int j) { return key + j >= lo && key + j < hi; };
+      keep0 = (in(2 * t) ? 0xffffu : 0u) | (in(2 * t + 1) ? 0xffff0000u : 0u);
+      keep1 = (in(2 * t + 8) ? 0xffffu : 0u) | (in(2 * t + 9) ? 0xffff0000u : 0u);
     }
 #pragma unroll
-    for (int h = 0; h < VH; ++h) {
-      const uint32_t* x = reinterpret_cast<const uint32_t*>(&vf[0][h]);
-      const uint32_t* y = reinterpret_cast<const uint32_t*>(&vf[1][h]);
-      const uint32_t* z = reinterpret_cast<const uint32_t*>(&vf[2][h]);
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(&vf[3][h]);
+    for (int i = 0; i < DP / 16; ++i) {
+      uint32_t a[4];
+      const uint32_t ch = (2 * i + v_hi) & 7;
+      ldmatrix4_trans(a, vt + (i / 4) * L::HALF + v_row + ((ch ^ sw) << 4));
+      a[0] &= keep0;
+      a[1] &= keep0;
+      a[2] &= keep1;
+      a[3] &= keep1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t a0 = __byte_perm(x[j], y[j], 0x5410), a1 = __byte_perm(x[j], y[j], 0x7632);
-        const uint32_t a2 = __byte_perm(z[j], w[j], 0x5410), a3 = __byte_perm(z[j], w[j], 0x7632);
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) mma16816(o[n][h][j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-      }
+      for (int c = 0; c < NQ; ++c) mma16816(o[c][i], a, pb[c][0], pb[c][1]);
     }
-    if (next < k1) load_v(row_next);
+    __syncwarp();  // every lane has read the stage
+    if (issued < mine) issue(issued++);
+  }
+  if (!ok) {
+    if (lane == 0) report(p.status, B200_DEV_WAIT_TIMEOUT);
+    for (int n = max(0, issued - NS); n < issued; ++n) mbar_wait(&full[n % NS], static_cast<uint32_t>(n / NS) & 1u);
   }
 
-  // Whole sums of the rows' weights.
+  // Whole sums of the rows' weights; the warps' states meet in shared memory.
+  __syncthreads();  // the ring is free
+  float* s_o = reinterpret_cast<float*>(smem);
+  float2* s_ml = reinterpret_cast<float2*>(smem + L::ML);
+  int* s_last = reinterpret_cast<int*>(smem + L::ML + kMaxSlots * R * 8);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int w = 4; w <= 16; w <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], w);
-
-  // The only part of its row also takes in the prefix's parts, dealt out to
-  // the warps: lane (gq, t) holds d = 64h + 8 gq .. + 7 of rows 2t, 2t + 1.
-  if (parts == 1) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int r = 8 * n + 2 * t;
-      for (int slot = warp; slot < p.np; slot += kWarps) {
-        float pm[2], pl[2], v[2][VH][8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          pm[u] = -INFINITY;
-          pl[u] = 0.f;
-          const int64_t at = (static_cast<int64_t>(g) * p.rows + row0 + r + u) * p.ns + slot;
-          const bool ok = r + u < nrows;
-          if (ok) {
-            pm[u] = p.ml[at * 2];
-            pl[u] = p.ml[at * 2 + 1];
-          }
-#pragma unroll
-          for (int h = 0; h < VH; ++h)
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-              float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (ok && gq + 8 * h < nchunks)
-                f = *reinterpret_cast<const float4*>(p.acc + at * p.D + 64 * h + 8 * gq + e);
-              v[u][h][e] = f.x, v[u][h][e + 1] = f.y, v[u][h][e + 2] = f.z, v[u][h][e + 3] = f.w;
-            }
-        }
-        if (pm[0] > m[n][0] || pm[1] > m[n][1])
-          rescale(n, fmaxf(m[n][0], pm[0]), fmaxf(m[n][1], pm[1]));
-        const float f0 = pm[0] == -INFINITY ? 0.f : ex2(pm[0] - m[n][0]);
-        const float f1 = pm[1] == -INFINITY ? 0.f : ex2(pm[1] - m[n][1]);
-        l[n][0] += f0 * pl[0];
-        l[n][1] += f1 * pl[1];
-#pragma unroll
-        for (int h = 0; h < VH; ++h)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o[n][h][j][0] += f0 * v[0][h][2 * j];
-            o[n][h][j][1] += f1 * v[1][h][2 * j];
-            o[n][h][j][2] += f0 * v[0][h][2 * j + 1];
-            o[n][h][j][3] += f1 * v[1][h][2 * j + 1];
-          }
-      }
-    }
-  }
-
-  // The warps' states meet in shared memory.
-#pragma unroll
-  for (int n = 0; n < NQ; ++n)
+  for (int c = 0; c < NQ; ++c)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int r = 8 * n + 2 * t + u;
-      if (gq == 0) {
-        s_m[warp][r] = m[n][u];
-        s_l[warp][r] = l[n][u];
-      }
 #pragma unroll
-      for (int h = 0; h < VH; ++h) {
-        float* dst = &s_o[warp][r][64 * h + 8 * gq];
-        *reinterpret_cast<float4*>(dst) =
-            make_float4(o[n][h][0][u], o[n][h][0][u + 2], o[n][h][1][u], o[n][h][1][u + 2]);
-        *reinterpret_cast<float4*>(dst + 4) =
-            make_float4(o[n][h][2][u], o[n][h][2][u + 2], o[n][h][3][u], o[n][h][3][u + 2]);
+      for (int w = 4; w <= 16; w <<= 1) l[c][u] += __shfl_xor_sync(0xffffffffu, l[c][u], w);
+      const int r = 8 * c + 2 * t + u;
+      if (gq == 0) s_ml[warp * R + r] = make_float2(m[c][u], l[c][u]);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        s_o[(warp * R + r) * L::LD + 16 * i + gq] = o[c][i][u];
+        s_o[(warp * R + r) * L::LD + 16 * i + gq + 8] = o[c][i][u + 2];
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < nrows * nchunks; i += kWarps * 32) {
-    const int r = i / nchunks, d0 = (i % nchunks) * 8;
+
+  const int64_t slot_row = (static_cast<int64_t>(g) * p.rows + row0) * p.ns;
+  int warps = kWarps, slots = p.np;  // what is joined: the warps' states, slots of the workspace
+  if (parts > 1) {
+    // This part goes to its slot; the last one to arrive joins all.
+    for (int i = threadIdx.x; i < nrows * (p.D / 4); i += kWarps * 32) {
+      const int r = i / (p.D / 4), d = (i % (p.D / 4)) * 4;
+      float M = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w * R + r].x);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = s_ml[w * R + r];
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - M);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * R + r) * L::LD + d);
+        sum = fmaf(f, ml.y, sum);
+        a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+      }
+      const int64_t at = slot_row + static_cast<int64_t>(r) * p.ns + p.np + split;
+      *reinterpret_cast<float4*>(p.acc + at * p.D + d) = a;
+      if (d == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(M, sum);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int64_t unit = (static_cast<int64_t>(b) * p.Hkv + g) * p.row_chunks + chunk;
+      *s_last = atomicAdd(&p.cnt[unit], 1) == parts - 1;
+    }
+    __syncthreads();
+    if (!*s_last) return;
+    __threadfence();
+    warps = 0;
+    slots = p.np + parts;
+  }
+
+  // Factors 2^(m - M) / L of every part of every row, a warp per row.
+  const int total = warps + slots;
+  for (int i = threadIdx.x; i < slots * nrows; i += kWarps * 32) {
+    const int j = i / nrows, r = i % nrows;
+    s_ml[(warps + j) * R + r] = __ldcg(
+        reinterpret_cast<const float2*>(p.ml + (slot_row + static_cast<int64_t>(r) * p.ns + j) * 2));
+  }
+  __syncthreads();
+  for (int r = warp; r < nrows; r += kWarps) {
     float M = -INFINITY;
+    for (int j = lane; j < total; j += 32) M = fmaxf(M, s_ml[j * R + r].x);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][r]);
-    float L = 0.f, a[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = s_m[w][r] == -INFINITY ? (s_l[w][r] == 0.f ? 0.f : 1.f) : ex2(s_m[w][r] - M);
-      L = fmaf(f, s_l[w][r], L);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = fmaf(f, s_o[w][r][d0 + e], a[e]);
+    for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    float sum = 0.f;
+    for (int j = lane; j < total; j += 32) {
+      const float2 ml = s_ml[j * R + r];
+      // An empty part (no key, or a slot that stays unused) has no factor.
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - M);
+      s_ml[j * R + r].x = f;
+      sum = fmaf(f, ml.y, sum);
     }
-    if (parts == 1) {
-      const float inv = 1.0f / L;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] *= inv;
-      const int64_t at = b * p.os0 + (g * p.rep + chunk * R + r) * p.os1 + d0 * p.os2;
-      if (op.out_vec) {
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) =
-            make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]),
-                       pack_bf16(a[6], a[7]));
-      } else {
+    for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    const float inv = 1.0f / sum;
+    for (int j = lane; j < total; j += 32) s_ml[j * R + r].x *= inv;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nrows * (p.D / 4); i += kWarps * 32) {
+    const int r = i / (p.D / 4), d = (i % (p.D / 4)) * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, const float4& v) {
+      a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+    };
+    for (int j = 0; j < warps; ++j)
+      add(s_ml[j * R + r].x, *reinterpret_cast<const float4*>(s_o + (j * R + r) * L::LD + d));
+    const float* acc = p.acc + (slot_row + static_cast<int64_t>(r) * p.ns) * p.D + d;
+    for (int j0 = 0; j0 < slots; j0 += 8) {  // eight loads on their way together
+      float4 v[8];
+      float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) store_elem(p.out, at + e * p.os2, p.out_dtype, a[e]);
+      for (int k = 0; k < 8; ++k) {
+        const int j = j0 + k;
+        f[k] = j < slots ? s_ml[(warps + j) * R + r].x : 0.f;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (f[k] != 0.f) v[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(j) * p.D));
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) add(f[k], v[k]);
+    }
+    const int64_t at = b * p.os0 + (head0 + r) * p.os1 + d * p.os2;
+    if (op.out_vec) {
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+          make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
     } else {
-      const int64_t at = (static_cast<int64_t>(g) * p.rows + row0 + r) * p.ns + p.np + split;
-      float4* dst = reinterpret_cast<float4*>(p.acc + at * p.D + d0);
-      dst[0] = make_float4(a[0], a[1], a[2], a[3]);
-      dst[1] = make_float4(a[4], a[5], a[6], a[7]);
-      if (d0 == 0) {
-        p.ml[at * 2] = M;
-        p.ml[at * 2 + 1] = L;
-      }
+      store_elem(p.out, at, p.out_dtype, a.x);
+      store_elem(p.out, at + p.os2, p.out_dtype, a.y);
+      store_elem(p.out, at + 2 * p.os2, p.out_dtype, a.z);
+      store_elem(p.out, at + 3 * p.os2, p.out_dtype, a.w);
     }
   }
-  if (parts == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int64_t unit = (static_cast<int64_t>(b) * p.Hkv + g) * p.row_chunks + chunk;
-    s_last = atomicAdd(&p.cnt[unit], 1) == parts - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  for (int r = warp; r < nrows; r += kWarps) join_row(p, g, row0 + r, parts, lane, 32);
 }
 
 template <int DP, int NQ>
-int launch(const OwnParams& op, cudaStream_t stream) {
+int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(p.B) * p.own_splits * p.row_chunks * p.Hkv;
   if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
-  shared_own_mma_kernel<DP, NQ><<<static_cast<unsigned>(grid), kWarps * 32, 0, stream>>>(op);
+  if (p.np + p.own_splits + kWarps > kMaxSlots)
+    return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
+  const int smem = OwnSmem<DP, NQ>::BYTES + 1024;
+  CUtensorMap tk, tv;
+  const uint64_t dims[3] = {static_cast<uint64_t>(pool.head_dim), static_cast<uint64_t>(pool.num_heads),
+                            static_cast<uint64_t>(pool.num_layers * pool.num_blocks * pool.block_size)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(pool.head_dim * 2),
+                               static_cast<uint64_t>(pool.num_heads * pool.head_dim * 2)};
+  const uint32_t box[3] = {64u, 1u, static_cast<uint32_t>(op.rbox)};
+  int rc = encode_tensor_map(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.k, dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != B200_OK) return rc;
+  rc = encode_tensor_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.v, dims, strides, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != B200_OK) return rc;
+  auto kern = shared_own_mma_kernel<DP, NQ>;
+  static std::atomic<int> configured[64];
+  if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
+    if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
+  }
+  kern<<<static_cast<unsigned>(grid), kWarps * 32, smem, stream>>>(tk, tv, op);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
 }
 
-bool vec16(const void* p, int64_t s0, int64_t s1, int64_t s2) {
-  return s2 == 1 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0;
+bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
+  return s2 == 1 && reinterpret_cast<uintptr_t>(p) % bytes == 0 && s0 % (bytes / 2) == 0 &&
+         s1 % (bytes / 2) == 0;
 }
 
 }  // namespace
 
 int shared_own_rows(int64_t rep) { return rep <= 8 ? 8 : 16; }
 
-int launch_shared_own_mma(const SharedParams& p, cudaStream_t stream) {
+int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc != B200_OK) return rc;
   OwnParams op;
   op.s = p;
-  op.q_vec = vec16(p.q, p.qs0, p.qs1, p.qs2);
-  op.out_vec = p.out_dtype == B200_DTYPE_BF16 && vec16(p.out, p.os0, p.os1, p.os2);
+  op.rbox = static_cast<int32_t>(std::min<int64_t>(p.S, kStep));
+  op.rb_shift = log2i(op.rbox);
+  op.q_vec = aligned(p.q, p.qs0, p.qs1, p.qs2, 4);
+  op.out_vec = p.out_dtype == B200_DTYPE_BF16 && aligned(p.out, p.os0, p.os1, p.os2, 8);
   const bool wide = shared_own_rows(p.rep) == 16;
-  if (p.D <= 64) return wide ? launch<64, 2>(op, stream) : launch<64, 1>(op, stream);
-  return wide ? launch<128, 2>(op, stream) : launch<128, 1>(op, stream);
+  if (p.D <= 64) return wide ? launch<64, 2>(op, pool, dev, stream) : launch<64, 1>(op, pool, dev, stream);
+  return wide ? launch<128, 2>(op, pool, dev, stream) : launch<128, 1>(op, pool, dev, stream);
 }
 
 }  // namespace b200

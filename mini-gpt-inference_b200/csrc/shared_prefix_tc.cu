@@ -607,8 +607,6 @@ int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const Device
 
 }  // namespace
 
-bool shared_tc_supported(int64_t S) { return S >= 8; }
-
 // One CTA per SM, at least two key tiles and at most kMaxParts CTAs to a unit
 // (each leaves a part that the join reads).
 TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) {
