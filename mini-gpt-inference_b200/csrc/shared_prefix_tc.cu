@@ -65,8 +65,7 @@ struct TcSmem {
   static constexpr int Q0 = 0;
   static constexpr int RING = 2 * TILE;
   static constexpr int BAR = RING + STAGES * TILE;
-  static constexpr int ML = BAR + 512;  // float2 [128]: group 1's maximum and sum
-  static constexpr int BYTES = ML + 128 * 8;
+  static constexpr int BYTES = BAR + 512;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -109,35 +108,83 @@ struct Segments {
   }
 };
 
-// The query row `row` of key head g (zeros from `rows` on) into row r of a
-// swizzled tile.
+// The 32 query rows from row0 on of key head g (zeros from `rows` on) into
+// rows r0 .. r0 + 31 of a swizzled tile, by one warp: whole rows by neighbouring
+// lanes, all loads on their way before the first store.  (A row per lane, 32
+// lines to a load, took 7 us for a tile; this takes <q>.)
 template <int DP>
-__device__ __forceinline__ void load_q_row(uint8_t* tile, int r, const SharedParams& s, int row, int g,
-                                           int q_vec) {
-  const bool live = row < s.rows;
-  const int b = live ? row / s.rep : 0;
-  const int64_t base = b * s.qs0 + static_cast<int64_t>(g * s.rep + (live ? row - b * s.rep : 0)) * s.qs1;
-  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q) + base;
+__device__ __forceinline__ void load_q_rows(uint8_t* tile, int r0, const SharedParams& s, int row0, int g,
+                                            int q_vec) {
+  constexpr int CH = DP / 8;       // chunks per row
+  constexpr int RPI = 32 / CH;     // rows per load
+  constexpr int IT = 32 / RPI;
+  const int lane = threadIdx.x & 31;
+  const int mine = min(row0 + lane, s.rows - 1);
+  const int b = mine / s.rep;
+  const int64_t off = b * s.qs0 + static_cast<int64_t>(g * s.rep + mine - b * s.rep) * s.qs1;
+  const int c = lane % CH;
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(s.q);
+  uint4 w[IT];
 #pragma unroll
-  for (int c = 0; c < DP / 8; ++c) {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (live && c * 8 < s.D) {
+  for (int i = 0; i < IT; ++i) {
+    const int r = i * RPI + lane / CH;
+    const __nv_bfloat16* src = q + __shfl_sync(0xffffffffu, off, r);
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (row0 + r < s.rows && c * 8 < s.D) {
       if (q_vec) {
-        w = *reinterpret_cast<const uint4*>(q + c * 8);
+        w[i] = *reinterpret_cast<const uint4*>(src + c * 8);
       } else {
         uint32_t x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const __nv_bfloat162 h =
-              __halves2bfloat162(q[(c * 8 + 2 * e) * s.qs2], q[(c * 8 + 2 * e + 1) * s.qs2]);
+              __halves2bfloat162(src[(c * 8 + 2 * e) * s.qs2], src[(c * 8 + 2 * e + 1) * s.qs2]);
           x[e] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        w = make_uint4(x[0], x[1], x[2], x[3]);
+        w[i] = make_uint4(x[0], x[1], x[2], x[3]);
       }
     }
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * (128 * 128) + sw128(r, c & 7)) = w;
   }
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+    *reinterpret_cast<uint4*>(tile + (c >> 3) * (128 * 128) + sw128(r0 + i * RPI + lane / CH, c & 7)) = w[i];
 }
+
+// W columns (32 or 64) of a warp's 32 rows, a row per lane, to global rows of
+// `pitch` floats through shared memory (32 x W floats, 16-byte chunks permuted
+// by row so that neither side meets a bank twice): W / 4 neighbouring lanes
+// write consecutive bytes of a row.  (16 bytes a lane, straight from the
+// lane's row, took 9 us for a tile; this takes <w>.)
+template <int W>
+struct RowWriter {
+  static constexpr int CH = W / 4;
+  float* stage;
+  float* dst;  // row 0, column 0
+  int64_t pitch;
+  int rows, cols;  // that exist
+  __device__ __forceinline__ void put(int c0, const float* o) {  // columns c0 .. c0 + 31 of this row
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const int ch = (c0 % W + e) >> 2;
+      *reinterpret_cast<float4*>(stage + lane * W + ((ch ^ (lane & (CH - 1))) << 2)) =
+          make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+    }
+  }
+  __device__ __forceinline__ void flush(int c0) {  // columns c0 .. c0 + W - 1
+    const int lane = threadIdx.x & 31;
+    const int ch = lane % CH;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int r = i * (32 / CH) + lane / CH;
+      const float4 v = *reinterpret_cast<const float4*>(stage + r * W + ((ch ^ (r & (CH - 1))) << 2));
+      if (r < rows && c0 + ch * 4 < cols)
+        *reinterpret_cast<float4*>(dst + r * pitch + c0 + ch * 4) = v;
+    }
+    __syncwarp();
+  }
+};
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -156,11 +203,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_full = p_full + 2;                                // [2]
   uint64_t* merge_full = o_full + 2;
   uint64_t* merge_done = merge_full + 1;
-  uint64_t* idle = merge_done + 1;
+  uint64_t* drained = merge_done + 1;                           // [2]
+  uint64_t* idle = drained + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(idle + 2);
-  static_assert((2 * NS + 13) * 8 <= 512, "barrier area too small");
-  float2* ml1 = reinterpret_cast<float2*>(smem + L::ML);
+  static_assert((2 * NS + 15) * 8 <= 512, "barrier area too small");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -173,9 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s_full[w], 1);
       mbar_init(&p_full[w], 128);
       mbar_init(&o_full[w], 1);
+      mbar_init(&drained[w], 128);
     }
-    mbar_init(merge_full, 128);
-    mbar_init(merge_done, 128);
+    mbar_init(merge_full, 256);
+    mbar_init(merge_done, 256);
     mbar_init(idle, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -380,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const float scale = s.qscale;
-    uint32_t tiles = 0, oseg = 0, mseg = 0;
+    uint32_t tiles = 0, oseg = 0, mseg = 0, dseg = 0;
     uint32_t first = 0;
     bool ok = true;
     Segments sg(p);
@@ -392,9 +440,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool group_live = tile_row0 < s.rows;  // uniform over the group
       const bool warp_live = tile_row0 + (warp & 3) * 32 < s.rows;
       const int cnt = one ? (n + 1 - w) / 2 : group_live ? n : 0;
-      // Q: the last segment's S products have all ended (s_full, o_full).
+      // Q: the last segment's S products have all ended (s_full, o_full, and
+      // in the one-tile form merge_done), and so has the use of its memory below.
       if (one ? w == 0 : group_live) {
-        load_q_row<DP>(smem + L::Q0 + w * L::TILE, r, s, row, g, p.q_vec);
+        load_q_rows<DP>(smem + L::Q0 + w * L::TILE, (warp & 3) * 32, s, tile_row0 + (warp & 3) * 32, g,
+                        p.q_vec);
         fence_proxy_async_shared();
         mbar_arrive(&q_full[w]);
       }
@@ -498,66 +548,77 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Slot of this CTA among those that share the unit.
       const int64_t a = static_cast<int64_t>(sg.unit) * p.unit_tiles;
       const int slot = static_cast<int>(blockIdx.x - ((a + 1) * gridDim.x - 1) / p.total);
+      // The groups' columns and factors: group w writes its own tile, or in the
+      // one-tile form half of the columns of f0 O_0 + f1 O_1.
+      const bool both = one && n >= 2;
       float f0 = 1.f, f1 = 0.f;
-      if (one && n >= 2) {
-        // Group 1's O, maximum and sum are added to group 0's.
-        if (w == 1) {
-          ml1[r] = make_float2(m, l);
-          mbar_arrive(merge_full);
-        } else {
-          ok = mbar_wait(merge_full, mseg & 1u) && *abort_flag == 0;
-          if (!ok) break;
-          const float2 o = ml1[r];
-          const float mm = fmaxf(m, o.x);
-          f0 = m == -INFINITY ? 0.f : ex2(m - mm);
-          f1 = o.x == -INFINITY ? 0.f : ex2(o.x - mm);
-          m = mm;
-          l = l * f0 + o.y * f1;
-        }
+      if (both) {
+        // (Maximum, sum) go through the groups' S columns, which are free now.
+        tmem_st2(ts, __float_as_uint(m), __float_as_uint(l));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(merge_full);
+        ok = mbar_wait(merge_full, mseg & 1u) && *abort_flag == 0;
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t x0, y0, x1, y1;
+        tmem_ld2(tmem + lanes, x0, y0);
+        tmem_ld2(tmem + 128 + lanes, x1, y1);
+        tmem_wait_ld();
+        const float2 a0 = make_float2(__uint_as_float(x0), __uint_as_float(y0));
+        const float2 a1 = make_float2(__uint_as_float(x1), __uint_as_float(y1));
+        m = fmaxf(a0.x, a1.x);
+        f0 = a0.x == -INFINITY ? 0.f : ex2(a0.x - m);
+        f1 = a1.x == -INFINITY ? 0.f : ex2(a1.x - m);
+        l = a0.y * f0 + a1.y * f1;
       }
-      if (warp_live && (one ? w == 0 : group_live)) {
+      if (warp_live && (both || (one ? w == 0 : group_live))) {
         const int64_t at = (static_cast<int64_t>(g) * s.rows + row) * s.ns + slot;
+        // This warp's eighth of the Q tiles is free: every S has been computed.
+        constexpr int W = DP / 2;
+        RowWriter<W> out;
+        out.stage = reinterpret_cast<float*>(smem + L::Q0 + (warp - 4) * (L::TILE / 4));
+        out.dst = s.acc + (at - static_cast<int64_t>(lane) * s.ns) * s.D;
+        out.pitch = static_cast<int64_t>(s.ns) * s.D;
+        out.rows = s.rows - (row - lane);
+        out.cols = s.D;
+        const uint32_t o0 = tmem + 256 + lanes;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = both ? w * W : 0; c < (both ? (w + 1) * W : DP); c += 32) {
           float o[32];
-          tmem_ld32(to + c, o);
-          if (one && n >= 2) {
+          tmem_ld32((both ? o0 : to) + c, o);
+          if (both) {
             float o1[32];
-            tmem_ld32(to + 128 + c, o1);
+            tmem_ld32(o0 + 128 + c, o1);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
           } else {
             tmem_wait_ld();
           }
-          if (row < s.rows) {
-            float* dst = s.acc + at * s.D + c;
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c + e < s.D) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
+          out.put(c, o);
+          if ((c + 32) % W == 0) out.flush(c + 32 - W);
         }
-        if (row < s.rows) {
-          s.ml[at * 2] = m;
-          s.ml[at * 2 + 1] = l;
+        if (row < s.rows && (w == 0 || !both)) {
+          float2* dst = reinterpret_cast<float2*>(s.ml) + at;
+          dst[0] = make_float2(m, l);
           // The unit's last segment also marks the slots that stay unused.
           if (sg.j0 + n == p.unit_tiles)
-            for (int i = slot + 1; i < s.np; ++i) {
-              s.ml[(at + i - slot) * 2] = -INFINITY;
-              s.ml[(at + i - slot) * 2 + 1] = 0.f;
-            }
+            for (int i = slot + 1; i < s.np; ++i) dst[i - slot] = make_float2(-INFINITY, 0.f);
         }
       }
-      if (one && n >= 2) {
-        // Group 1 may write its O again once group 0 has read it.
-        if (w == 0) {
-          tc_fence_before();
-          mbar_arrive(merge_done);
-        } else {
-          ok = mbar_wait(merge_done, mseg & 1u) && *abort_flag == 0;
-          tc_fence_after();
-        }
+      if (both) {
+        // O, Q and ml may be written again once both groups are done with them.
+        tc_fence_before();
+        mbar_arrive(merge_done);
+        ok = mbar_wait(merge_done, mseg & 1u) && *abort_flag == 0;
+        tc_fence_after();
         ++mseg;
+      } else if (one ? w == 0 : group_live) {
+        // The next Q goes over what the group's warps stage their rows in.
+        mbar_arrive(&drained[w]);
+        ok = mbar_wait(&drained[w], dseg & 1u) && *abort_flag == 0;
+        ++dseg;
       }
       first += 2 * n;
     }
