@@ -74,14 +74,41 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Waits for this thread's TMEM loads; the 32 values cannot be used earlier.
+__device__ __forceinline__ void wait_ld32(float* v) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+        "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+        "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+        "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
+}
+
+// Weights 2^(v scale - ref) of 32 scores as bf16 pairs; returns their sum
+// before the rounding.
+__device__ __forceinline__ float weights32(const float* v, float scale, float ref, uint32_t* pk) {
+  const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-ref, -ref), one2 = make_float2(1.f, 1.f);
+  float2 q[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) q[e] = ffma2(make_float2(v[2 * e], v[2 * e + 1]), sc2, nm2);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) q[e] = make_float2(ex2(q[e].x), ex2(q[e].y));
+  // bf16 for the product alone; the sum keeps the weights whole.
+#pragma unroll
+  for (int e = 0; e < 16; ++e) pk[e] = pack_bf16(q[e].x, q[e].y);
+#pragma unroll
+  for (int w = 8; w >= 1; w >>= 1)
+#pragma unroll
+    for (int e = 0; e < w; ++e) q[e] = ffma2(q[e], one2, q[e + w]);
+  return q[0].x + q[0].y;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-
-// Stops the compiler from moving what is computed from x out of a loop.
-__device__ __forceinline__ void keep_here(uint64_t& x) { asm volatile("" : "+l"(x)); }
 
 // Byte offset of 16-byte chunk ch of row r in a 128-byte-swizzled half tile.
 __device__ __forceinline__ uint32_t sw128(int r, int ch) {
@@ -204,10 +231,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* merge_full = o_full + 2;
   uint64_t* merge_done = merge_full + 1;
   uint64_t* drained = merge_done + 1;                           // [2]
-  uint64_t* idle = drained + 2;
+  uint64_t* turn = drained + 2;                                 // [2 groups][4 warps]
+  uint64_t* idle = turn + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(idle + 2);
-  static_assert((2 * NS + 15) * 8 <= 512, "barrier area too small");
+  static_assert((2 * NS + 23) * 8 <= 512, "barrier area too small");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -218,9 +246,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&q_full[w], 128);
       mbar_init(&s_full[w], 1);
-      mbar_init(&p_full[w], 128);
+      mbar_init(&p_full[w], 4);  // a lane of each warp
       mbar_init(&o_full[w], 1);
       mbar_init(&drained[w], 128);
+      for (int i = 0; i < 4; ++i) mbar_init(&turn[4 * w + i], 1);
     }
     mbar_init(merge_full, 256);
     mbar_init(merge_done, 256);
@@ -246,10 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 1;
   };
 
-  // Registers: 384 threads start with 168 each (64512 in all); 128 x 72 +
-  // 256 x 216 is the same sum.  A softmax thread holds a row of 128 scores.
+  // Registers: 384 threads start with 168 each (64512 in all); 128 x 56 +
+  // 256 x 224 is the same sum.  A softmax thread works on a row of 128 scores.
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     const int box_bytes = 64 * p.rbox * 2;
@@ -314,120 +343,105 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0 && *abort_flag == 0;
-    };
-    constexpr uint32_t idesc_s = idesc_bf16(128, kBN, false);
-    constexpr uint32_t idesc_o = idesc_bf16(128, DP, true);
-    const uint64_t dq0 = smem_desc_sw128(smem_u32(smem + L::Q0), 16, 1024);
-    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::RING), 16, 1024);
-    const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::RING), L::HALF, 1024);
-    uint32_t first = 0;           // ring entry of the segment's first K
-    uint32_t np[2] = {0, 0};      // P tiles of group w awaited so far
-    uint32_t nq[2] = {0, 0};      // Q tiles awaited so far
-    bool ok = true;
-    auto issue_s = [&](int w, int qt, uint32_t entry) {
-      uint64_t dq = dq0 + static_cast<uint64_t>(qt * (L::TILE >> 4));
-      uint64_t dk = dk0 + static_cast<uint64_t>((entry % NS) * (L::TILE >> 4));
-      keep_here(dq);  // the steps' descriptors are not worth registers over the loop
-      keep_here(dk);
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        const uint64_t off = static_cast<uint64_t>(((kk >> 2) * L::HALF + (kk & 3) * 32) >> 4);
-        mma_bf16(tmem + w * 128, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
-      }
-      mma_commit(&s_full[w]);
-    };
-    auto issue_pv = [&](int w, uint32_t entry, bool accumulate) {
-      uint64_t dv = dv0 + static_cast<uint64_t>((entry % NS) * (L::TILE >> 4));
-      keep_here(dv);
-#pragma unroll
-      for (int kk = 0; kk < kBN / 16; ++kk)
-        mma_bf16_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, dv + static_cast<uint64_t>(kk * 128),
-                    idesc_o, accumulate || kk > 0 ? 1u : 0u);
-    };
-    auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
-    Segments sg(p);
-    while (ok && sg.next()) {
-      const int n = sg.n;
-      const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
-      ok = wait_all(&q_full[0], nq[0]++ & 1u) && (!two || wait_all(&q_full[1], nq[1]++ & 1u));
-      if (!ok) break;
-      tc_fence_after();
-      if (one) {
-        // Group w takes the tiles k = w, w + 2, ...
-        for (int k = 0; ok && k < min(n, 2); ++k) {
-          ok = wait_entry(first + 2 * k);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(k, 0, first + 2 * k);
-          mma_commit(&empty[(first + 2 * k) % NS]);
-        }
-        for (int k = 0; ok && k < n; ++k) {
-          const int w = k & 1;
-          ok = wait_all(&p_full[w], np[w] & 1u) && wait_entry(first + 2 * k + 1);
-          if (!ok) break;
-          ++np[w];
-          tc_fence_after();
-          issue_pv(w, first + 2 * k + 1, k >= 2);
-          mma_commit(&empty[(first + 2 * k + 1) % NS]);
-          if (k + 2 >= n) {
-            mma_commit(&o_full[w]);
-          } else {
-            const uint32_t e = first + 2 * (k + 2);
-            ok = wait_entry(e);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(w, 0, e);
-            mma_commit(&empty[e % NS]);
-          }
-        }
-      } else {
-        const int groups = two ? 2 : 1;
-        ok = wait_entry(first);
-        if (!ok) break;
-        tc_fence_after();
-        for (int w = 0; w < groups; ++w) issue_s(w, w, first);
-        mma_commit(&empty[first % NS]);
-        for (int k = 0; ok && k < n; ++k) {
-          const uint32_t ev = first + 2 * k + 1, ek = ev + 1;
-          for (int w = 0; ok && w < groups; ++w) {
-            ok = wait_all(&p_full[w], np[w] & 1u) && (w > 0 || wait_entry(ev));
-            if (!ok) break;
-            ++np[w];
-            tc_fence_after();
-            issue_pv(w, ev, k > 0);
-            if (w == groups - 1) mma_commit(&empty[ev % NS]);
-            if (k + 1 == n) {
-              mma_commit(&o_full[w]);
-            } else {
-              ok = w > 0 || wait_entry(ek);
+    // The whole warp, so that descriptors stay in uniform registers (one lane
+    // issues), in small loops: this code shares its instruction cache with the
+    // softmax warps, and a step that has to be fetched again is late.
+    {
+      constexpr uint32_t idesc_s = idesc_bf16(128, kBN, false);
+      constexpr uint32_t idesc_o = idesc_bf16(128, DP, true);
+      const uint64_t dq0 = smem_desc_sw128(smem_u32(smem + L::Q0), 16, 1024);
+      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::RING), 16, 1024);
+      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::RING), L::HALF, 1024);
+      uint32_t first = 0;         // ring entry of the segment's first K
+      uint32_t np0 = 0, np1 = 0;  // P tiles of group w awaited so far
+      uint32_t nq0 = 0, nq1 = 0;  // Q tiles awaited so far
+      bool ok = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+      };
+      auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
+      Segments sg(p);
+      while (ok && sg.next()) {
+        const int n = sg.n;
+        const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
+        ok = wait_all(&q_full[0], nq0++ & 1u) && (!two || wait_all(&q_full[1], nq1++ & 1u)) &&
+             *abort_flag == 0;
+        // Step t: P V of tile t, then S of tile t + lead for the same group, which
+        // frees the columns in that order.  Two row tiles: both groups, one tile
+        // ahead; one row tile: the groups alternate, two tiles ahead.
+        const int lead = one ? 2 : 1, groups = two ? 2 : 1;
+#pragma unroll 1
+        for (int t = -lead; ok && t < n; ++t) {
+          const uint32_t ev = first + 2 * t + 1, ek = first + 2 * (t + lead);
+#pragma unroll 1
+          for (int i = 0; ok && i < groups; ++i) {
+            const int w = one ? t & 1 : i;
+            const bool last = i == groups - 1;
+            if (t >= 0) {
+              ok = wait_all(&p_full[w], (w ? np1 : np0) & 1u) && (i > 0 || wait_entry(ev));
+              if (!ok) break;
+              (w ? np1 : np0) += 1;
+              tc_fence_after();
+              uint64_t dv = dv0 + static_cast<uint64_t>((ev % NS) * (L::TILE >> 4));
+              uint32_t tp = tmem + w * 128;
+#pragma unroll 8
+              for (int kk = 0; kk < kBN / 16; ++kk, dv += 128, tp += 8)
+                mma_bf16_ts(tmem + 256 + w * 128, tp, dv, idesc_o, t >= lead || kk > 0 ? 1u : 0u);
+              if (last) mma_commit(&empty[ev % NS]);
+              if (t + lead >= n) mma_commit(&o_full[w]);
+            }
+            if (t + lead < n) {
+              ok = i > 0 || wait_entry(ek);
               if (!ok) break;
               tc_fence_after();
-              issue_s(w, w, ek);
-              if (w == groups - 1) mma_commit(&empty[ek % NS]);
+              uint64_t dq = dq0 + static_cast<uint64_t>(i * (L::TILE >> 4));
+              uint64_t dk = dk0 + static_cast<uint64_t>((ek % NS) * (L::TILE >> 4));
+#pragma unroll 8
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                mma_bf16(tmem + w * 128, dq, dk, idesc_s, kk > 0 ? 1u : 0u);
+                const uint64_t step = kk == 3 ? (L::HALF - 96) >> 4 : 2;  // 16 d on, or the other half
+                dq += step;
+                dk += step;
+              }
+              mma_commit(&s_full[w]);
+              if (last) mma_commit(&empty[ek % NS]);
             }
           }
+          ok = ok && *abort_flag == 0;
         }
+        first += 2 * n;
       }
-      first += 2 * n;
+      if (!ok && lane == 0) give_up();
+      mma_commit(idle);  // every product issued has ended before TMEM is freed
+      if (!wait_all(idle, 0) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
+      __syncwarp();
     }
-    if (!ok && lane == 0) give_up();
-    mma_commit(idle);  // every product issued has ended before TMEM is freed
-    if (!__all_sync(0xffffffffu, mbar_wait(idle, 0)) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
-    __syncwarp();
   } else {
     // Counters of the kernel that follows on the stream.
     for (int i = blockIdx.x * 64 + threadIdx.x - 64; i < p.zero_count; i += gridDim.x * 64) s.cnt[i] = 0;
   }
   } else {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int w = (warp - 4) >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const float scale = s.qscale;
+    // The groups take turns at the exponential unit, which their warps share
+    // pairwise: left to themselves they drift into using it side by side,
+    // each at half the speed, and then wait for the products side by side.
+    uint64_t* my_turn = &turn[4 * w + (warp & 3)];
+    uint64_t* their_turn = &turn[4 * (w ^ 1) + (warp & 3)];
+    uint32_t turns = 0;
+    auto take_turn = [&]() -> bool {  // group 0 begins
+      const uint32_t before = w == 0 ? turns++ : ++turns;  // turns of the other group to await
+      return before == 0 || mbar_wait(my_turn, (before - 1) & 1u);
+    };
+    auto pass_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(their_turn);
+    };
     uint32_t tiles = 0, oseg = 0, mseg = 0, dseg = 0;
     uint32_t first = 0;
     bool ok = true;
@@ -456,69 +470,84 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
+        if (!take_turn()) {
+          ok = false;
+          break;
+        }
         const int left = static_cast<int>(  // keys from here on
             min(s.prefix - static_cast<int64_t>(sg.j0 + jj) * kBN, static_cast<int64_t>(kBN)));
         if (warp_live) {
-          float v[kBN];
+          // The weights are taken relative to the row's reference m as it stands,
+          // and their sum tells whether that was far too low (or a score is not
+          // a number); the rare warp with such a row finds a new one and does
+          // the tile again.  The first tile has no reference yet.  What runs
+          // once or rarely is rolled up: cold instructions cost more than
+          // loops here (unrolled, the first two tiles of a CTA took 11 us).
+          if (left < kBN) {  // the prefix ends in this tile
+#pragma unroll 1
+            for (int c = 0; c < kBN; c += 32) {
+              float v[32];
+              tmem_ld32(ts + c, v);
+              wait_ld32(v);
 #pragma unroll
-          for (int c = 0; c < kBN; c += 32) tmem_ld32(ts + c, v + c);
-          tmem_wait_ld();
-          if (left < kBN) {
-#pragma unroll
-            for (int c = 0; c < kBN; ++c)
-              if (c >= left) v[c] = -INFINITY;
-          }
-          float mp[8];
-#pragma unroll
-          for (int a = 0; a < 8; ++a) mp[a] = fmaxf(v[2 * a], v[2 * a + 1]);
-#pragma unroll
-          for (int c = 16; c < kBN; c += 16)
-#pragma unroll
-            for (int a = 0; a < 8; ++a) mp[a] = max3(mp[a], v[c + 2 * a], v[c + 2 * a + 1]);
-          const float mx =
-              scale * max3(max3(mp[0], mp[1], mp[2]), max3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
-          // The reference point moves only when the maximum exceeds it by
-          // more than 2^8; O follows (P V of the tile before has ended).
-          float m_new = m, alpha = 1.f;
-          if (mx > m + 8.f) {
-            m_new = mx;
-            alpha = m == -INFINITY ? 0.f : ex2(m - mx);
-          }
-          if (k > 0 && __any_sync(0xffffffffu, m_new != m)) {
-#pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              float o[32];
-              tmem_ld32(to + c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= alpha;
-              tmem_st32(to + c, o);
+              for (int e = 0; e < 32; ++e) v[e] = c + e < left ? v[e] : -INFINITY;
+              tmem_st32(ts + c, v);
             }
+            tmem_wait_st();
           }
-          m = m_new;
-          const float ref = m == -INFINITY ? 0.f : m;
-          const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-ref, -ref);
-          const float2 one2 = make_float2(1.f, 1.f);
-          float2 sum[4];
+          uint32_t pk[kBN / 2];
+          float add, alpha = 1.f;
+#pragma unroll 1
+          for (bool fresh = k == 0;; fresh = true) {
+            if (fresh) {
+              float mx = -INFINITY;
+#pragma unroll 1
+              for (int c = 0; c < kBN; c += 32) {
+                float v[32];
+                tmem_ld32(ts + c, v);
+                wait_ld32(v);
 #pragma unroll
-          for (int a = 0; a < 4; ++a) sum[a] = make_float2(0.f, 0.f);
+                for (int e = 0; e < 32; e += 2) mx = max3(mx, v[e], v[e + 1]);
+              }
+              mx *= scale;
+              // O follows the reference (P V of the tile before has ended).
+              float m_new = m;
+              if (mx > m + 8.f) {
+                m_new = mx;
+                alpha = m == -INFINITY ? 0.f : ex2(m - mx);
+              }
+              if (k > 0 && __any_sync(0xffffffffu, m_new != m)) {
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 32) {
+                  float o[32];
+                  tmem_ld32(to + c, o);
+                  wait_ld32(o);
 #pragma unroll
-          for (int c = 0; c < kBN; c += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 x = ffma2(make_float2(v[c + e], v[c + e + 1]), sc2, nm2);
-              const float2 q = make_float2(ex2(x.x), ex2(x.y));
-              sum[(e >> 1) & 3] = ffma2(q, one2, sum[(e >> 1) & 3]);
-              // bf16 for the product alone; the sum keeps the weights whole.
-              pk[e >> 1] = pack_bf16(q.x, q.y);
+                  for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                  tmem_st32(to + c, o);
+                }
+              }
+              m = m_new;
             }
-            tmem_st16(ts + (c >> 1), pk);
+            const float ref = m == -INFINITY ? 0.f : m;
+            float v[2][32];
+            add = 0.f;
+            tmem_ld32(ts, v[0]);
+#pragma unroll
+            for (int c = 0; c < kBN; c += 32) {
+              wait_ld32(v[(c >> 5) & 1]);
+              if (c + 32 < kBN) tmem_ld32(ts + c + 32, v[(c >> 5 & 1) ^ 1]);
+              add += weights32(v[(c >> 5) & 1], scale, ref, pk + (c >> 1));
+            }
+            if (fresh || !__any_sync(0xffffffffu, !(add < 65536.f))) break;
           }
-          const float add = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) +
-                            ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+          pass_turn();
+#pragma unroll
+          for (int c = 0; c < kBN / 2; c += 16) tmem_st16(ts + c, pk + c);
           l = l * alpha + add;
           tmem_wait_st();
+        } else {
+          pass_turn();
         }
         if (left < kBN && (one || w == 0)) {
           const uint32_t e = first + 2 * jj + 1;
@@ -537,7 +566,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_shared();
         }
         tc_fence_before();
-        mbar_arrive(&p_full[w]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+      }
+      // A group with fewer tiles lets its turns pass.
+      for (int k = cnt; ok && k < (one ? (n + 1) / 2 : n); ++k) {
+        ok = take_turn() && *abort_flag == 0;
+        pass_turn();
       }
       if (ok && cnt > 0) {
         ok = mbar_wait(&o_full[w], oseg & 1u) && *abort_flag == 0;
