@@ -35,11 +35,11 @@ template <int R>
 struct ElemTile;
 template <>
 struct ElemTile<64> {
-  static constexpr int RT = 4, TR = 16, TC = 8;
+  static constexpr int RT = 4, TC = 8;  // 16 x 8 threads
 };
 template <>
 struct ElemTile<8> {
-  static constexpr int RT = 1, TR = 8, TC = 16;
+  static constexpr int RT = 1, TC = 16;  // 8 x 16 threads
 };
 
 template <int R, int DP>
@@ -469,7 +469,7 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
              : launch_prefix_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
     if (rc != B200_OK) return rc;
   }
-  if (pl.mma) return launch_shared_own_mma(p, a.pool, stream);
+  if (pl.mma) return launch_shared_own_mma(p, a.pool, pl.tc, stream);
   return f32 ? launch_own_elem_d<float>(p, dev.device, stream)
              : launch_own_elem_d<__nv_bfloat16>(p, dev.device, stream);
 }

@@ -46,14 +46,16 @@ struct SharedParams {
   float qscale;  // log2(e) / sqrt(D)
 };
 
-// Own keys and join, bf16 pool and queries; the rows of a key head one CTA takes.
-int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, cudaStream_t stream);
+// Own keys and join, bf16 pool and queries; the rows of a key head one CTA
+// takes.  `overlap`: the kernel ahead on the stream is the prefix's.
+int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
+                          cudaStream_t stream);
 int shared_own_rows(int64_t rep);
 
 // The prefix on tensor cores: how its key tiles are cut.
 struct TcSplit {
-  int64_t total;   // key tiles of all units
-  int unit_tiles;  // of one unit (up to 256 rows of a key head)
+  int64_t units;   // up to 256 rows of a key head each
+  int unit_tiles;  // key tiles of one unit
   int unit_pairs;  // units per key head
   int ctas;
   int np;          // most CTAs that share a unit
@@ -73,6 +75,12 @@ __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int s
   *k1 = min(*k0 + per, n);
   return parts;
 }
+
+// The own-key kernel may begin while the prefix's is still running:
+// `let_next_start` allows it, `wait_for_previous` waits until the kernel ahead
+// on the stream has ended and its writes can be read.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The joined row (g, R): element d of sum_s 2^(m_s - M) acc_s / sum_s
 // 2^(m_s - M) l_s over the prefix's slots and the first `parts` own ones,

@@ -78,7 +78,7 @@ struct OwnSmem {
   static constexpr int HALF = kStep * 128;        // 16 keys x 64 d
   static constexpr int TILE = HALVES * HALF;      // K or V of a step
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int STAGES = DP == 128 ? 3 : 6;
+  static constexpr int STAGES = DP == 128 ? 2 : 4;
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int R = 8 * NQ;
   static constexpr int LD = DP + 4;               // 2 LD = 8 mod 32: no bank is hit twice
@@ -339,6 +339,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
   __syncthreads();
 
+  // So far nothing came from the prefix's kernel, whose end this kernel
+  // overlaps; its parts, and the counters that it cleared, do.
+  wait_for_previous();
   const int64_t slot_row = (static_cast<int64_t>(g) * p.rows + row0) * p.ns;
   int warps = kWarps, slots = p.np;  // what is joined: the warps' states, slots of the workspace
   if (parts > 1) {
@@ -437,7 +440,8 @@ __global__ void __launch_bounds__(kWarps * 32)
 }
 
 template <int DP, int NQ>
-int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, cudaStream_t stream) {
+int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
+           cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(p.B) * p.own_splits * p.row_chunks * p.Hkv;
   if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
@@ -463,8 +467,17 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
     if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
   }
-  kern<<<static_cast<unsigned>(grid), kWarps * 32, smem, stream>>>(tk, tv, op);
-  cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tk, tv, op);
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
 }
 
@@ -477,7 +490,8 @@ bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
 
 int shared_own_rows(int64_t rep) { return rep <= 8 ? 8 : 16; }
 
-int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, cudaStream_t stream) {
+int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
+                          cudaStream_t stream) {
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc != B200_OK) return rc;
@@ -488,8 +502,9 @@ int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, cud
   op.q_vec = aligned(p.q, p.qs0, p.qs1, p.qs2, 4);
   op.out_vec = p.out_dtype == B200_DTYPE_BF16 && aligned(p.out, p.os0, p.os1, p.os2, 8);
   const bool wide = shared_own_rows(p.rep) == 16;
-  if (p.D <= 64) return wide ? launch<64, 2>(op, pool, dev, stream) : launch<64, 1>(op, pool, dev, stream);
-  return wide ? launch<128, 2>(op, pool, dev, stream) : launch<128, 1>(op, pool, dev, stream);
+  if (p.D <= 64)
+    return wide ? launch<64, 2>(op, pool, dev, overlap, stream) : launch<64, 1>(op, pool, dev, overlap, stream);
+  return wide ? launch<128, 2>(op, pool, dev, overlap, stream) : launch<128, 1>(op, pool, dev, overlap, stream);
 }
 
 }  // namespace b200

@@ -47,7 +47,7 @@ constexpr int kThreads = 384;
 
 struct TcParams {
   SharedParams s;
-  int64_t total;    // key tiles of all units
+  int64_t units;
   int32_t unit_tiles;  // key tiles per unit
   int32_t unit_pairs;  // units per key head
   int32_t one_tile;    // at most 128 rows per key head
@@ -115,14 +115,32 @@ __device__ __forceinline__ uint32_t sw128(int r, int ch) {
   return static_cast<uint32_t>(r) * 128u + (static_cast<uint32_t>(ch ^ (r & 7)) << 4);
 }
 
+// What a segment costs besides its tiles (queries in, rows out, the first
+// scores), in tiles: 9 us against 2.2 us a tile.
+constexpr int kSegment = 4;
+
+// Runs of equal cost: a unit's tiles, then the segment's cost, is a stretch of
+// unit_tiles + kSegment; the stretches, end to end, are cut evenly.
+__host__ __device__ inline int64_t run_begin(int64_t units, int unit_tiles, int64_t cta, int64_t ctas) {
+  const int64_t stretch = unit_tiles + kSegment;
+  const int64_t x = units * stretch * cta / ctas;
+  const int64_t unit = x / stretch, off = x - unit * stretch;
+  return unit * unit_tiles + (off < unit_tiles ? off : unit_tiles);
+}
+// The CTA that has tile `tile` of unit `unit`: the last that begins at or before it.
+__host__ __device__ inline int64_t cta_of(int64_t units, int unit_tiles, int64_t ctas, int64_t unit, int tile) {
+  const int64_t stretch = unit_tiles + kSegment;
+  return ((unit * stretch + tile + 1) * ctas - 1) / (units * stretch);
+}
+
 // A CTA's run of key tiles, segment by segment.
 struct Segments {
   int64_t pos, end;
   int tiles_per_unit;
   int unit, j0, n;  // this segment: key tiles [j0, j0 + n) of a unit
   __device__ Segments(const TcParams& p) {
-    pos = p.total * blockIdx.x / gridDim.x;
-    end = p.total * (blockIdx.x + 1) / gridDim.x;
+    pos = run_begin(p.units, p.unit_tiles, blockIdx.x, gridDim.x);
+    end = run_begin(p.units, p.unit_tiles, blockIdx.x + 1, gridDim.x);
     tiles_per_unit = p.unit_tiles;
   }
   __device__ bool next() {
@@ -238,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   static_assert((2 * NS + 23) * 8 <= 512, "barrier area too small");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  let_next_start();
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
@@ -581,8 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // Slot of this CTA among those that share the unit.
-      const int64_t a = static_cast<int64_t>(sg.unit) * p.unit_tiles;
-      const int slot = static_cast<int>(blockIdx.x - ((a + 1) * gridDim.x - 1) / p.total);
+      const int slot =
+          static_cast<int>(blockIdx.x - cta_of(p.units, p.unit_tiles, gridDim.x, sg.unit, 0));
       // The groups' columns and factors: group w writes its own tile, or in the
       // one-tile form half of the columns of f0 O_0 + f1 O_1.
       const bool both = one && n >= 2;
@@ -710,24 +729,22 @@ TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) 
   TcSplit t{};
   t.unit_pairs = static_cast<int>(ceil_div(rows, 2 * kBM));
   t.unit_tiles = static_cast<int>(ceil_div(prefix, kBN));
-  const int64_t units = Hkv * t.unit_pairs;
-  t.total = units * t.unit_tiles;
-  const int64_t ctas = std::min<int64_t>({static_cast<int64_t>(num_sms), ceil_div(t.total, kMinTiles),
-                                          units * kMaxParts});
+  t.units = Hkv * t.unit_pairs;
+  const int64_t total = t.units * t.unit_tiles;
+  const int64_t ctas = std::min<int64_t>({static_cast<int64_t>(num_sms), ceil_div(total, kMinTiles),
+                                          t.units * kMaxParts});
   t.ctas = static_cast<int>(std::max<int64_t>(ctas, 1));
-  // Parts of a unit: each of its CTAs but the first and last has at least
-  // total / ctas of its tiles.
-  const int64_t least = t.total / t.ctas;
-  t.np = static_cast<int>(std::min<int64_t>(ceil_div(t.unit_tiles - 1, least) + 1, t.ctas));
-  if (units <= 1024) {
-    int64_t most = 1;
-    for (int64_t u = 0; u < units; ++u) {
-      const int64_t c0 = ((u * t.unit_tiles + 1) * t.ctas - 1) / t.total;
-      const int64_t c1 = ((u + 1) * t.unit_tiles * t.ctas - 1) / t.total;
-      most = std::max(most, c1 - c0 + 1);
-    }
-    t.np = static_cast<int>(most);
+  // The most CTAs that share a unit (an upper bound where the units are many).
+  int64_t most = 1;
+  if (t.units <= 1024) {
+    for (int64_t u = 0; u < t.units; ++u)
+      most = std::max(most, cta_of(t.units, t.unit_tiles, t.ctas, u, t.unit_tiles - 1) -
+                                cta_of(t.units, t.unit_tiles, t.ctas, u, 0) + 1);
+  } else {
+    const int64_t least = t.units * (t.unit_tiles + kSegment) / t.ctas;
+    most = std::min<int64_t>(ceil_div(t.unit_tiles - 1, least) + 1, t.ctas);
   }
+  t.np = static_cast<int>(most);
   return t;
 }
 
@@ -738,7 +755,7 @@ int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, c
   if (rc != B200_OK) return rc;
   TcParams p{};
   p.s = s;
-  p.total = t.total;
+  p.units = t.units;
   p.unit_tiles = t.unit_tiles;
   p.unit_pairs = t.unit_pairs;
   p.one_tile = s.rows <= kBM;
