@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -120,6 +121,24 @@ class PrefillBatchArgs(ctypes.Structure):
     _fields_ = [("num_seqs", _i64), ("seqs", ctypes.POINTER(PrefillArgs))]
 
 
+_CODES = {ctypes.c_int64: "q", ctypes.c_void_p: "P", ctypes.c_size_t: "N", ctypes.c_int: "i",
+          ctypes.c_int32: "i", ctypes.c_float: "f"}
+
+
+def packer(cls) -> struct.Struct:
+    """The struct module's form of an argument structure, nested ones written
+    out field by field (native alignment is the C layout; a nested structure
+    must end on 8 bytes).  Packing the fields costs a third of what filling a
+    ctypes structure does, which is most of the host time of a small call;
+    a C entry reads its arguments only while it runs, so the bytes serve."""
+    def codes(c):
+        return "".join(codes(t) if issubclass(t, ctypes.Structure) else _CODES[t]
+                       for _, t in c._fields_)
+    form = struct.Struct("@" + codes(cls) + "0q")
+    assert form.size == ctypes.sizeof(cls)
+    return form
+
+
 # Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "b200_kv_scatter": (ctypes.c_int, [ctypes.POINTER(ScatterArgs), _p]),
@@ -131,9 +150,9 @@ SIGNATURES = {
     "b200_qkv_kv_write_plan": (ctypes.c_int, [_i64, _i64, ctypes.POINTER(ctypes.c_int32),
                                               ctypes.POINTER(ctypes.c_int32),
                                               ctypes.POINTER(ctypes.c_int32)]),
-    "b200_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), _p]),
-    "b200_rope_kv_append": (ctypes.c_int, [ctypes.POINTER(RopeKvAppendArgs), _p]),
-    "b200_shared_prefix_decode": (ctypes.c_int, [ctypes.POINTER(SharedPrefixArgs), _p]),
+    "b200_qk_norm_rope": (ctypes.c_int, [_p, _p]),
+    "b200_rope_kv_append": (ctypes.c_int, [_p, _p]),
+    "b200_shared_prefix_decode": (ctypes.c_int, [_p, _p]),
     "b200_shared_prefix_decode_workspace_size": (
         ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "b200_paged_decode_workspace_size": (

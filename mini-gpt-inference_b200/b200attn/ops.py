@@ -52,8 +52,10 @@ def _inference_only(*tensors) -> None:
     """The ops have no backward: like the reference's triton_v0 branch
     (minivllm/attention.py:404-405) they refuse inputs that require grad
     while grad mode is on."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the b200 backend is inference-only; run under torch.inference_mode()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the b200 backend is inference-only; run under torch.inference_mode()")
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -121,25 +123,58 @@ class PreparedCall:
         return self._result
 
 
-def _launch(fn, args, device: torch.device, what: str) -> None:
-    """Calls a C entry on the current stream of ``device``, whichever device
-    is the current one."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+def _launch(fn, args, index: int, what: str) -> None:
+    """Calls a C entry on the current stream of device ``index``, whichever
+    device is the current one.  args: a packed argument structure."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
 
 
 class _DeviceCall(PreparedCall):
-    """A prepared call that may be made while another device is current."""
+    """A prepared call (of packed arguments) that may be made while another
+    device is current."""
+
+    def __init__(self, fn, args: bytes, index: int, result, what: str, keep=()):
+        self._fn, self._args, self._index = fn, args, index
+        self._result, self._what, self._keep = result, what, keep
 
     def __call__(self):
-        _launch(self._fn, self._args, self._device, self._what)
+        _launch(self._fn, self._args, self._index, self._what)
         return self._result
+
+
+def _status_ptr(status, index: int):
+    if status is None:
+        return 0
+    if status.dtype != torch.int32 or status.get_device() != index or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor on the q device")
+    return status.data_ptr()
+
+
+def _pool_fields(pool, index: int, layer_idx: int):
+    """The checked fields of _lib.KVPool, and the block size, heads and head
+    dimension."""
+    k, v = pool.k, pool.v
+    shape = k.shape
+    if len(shape) != 5 or v.shape != shape:
+        raise ValueError("KV tensors must have matching [L,P,S,H,D] shape")
+    dtype = k.dtype
+    if dtype not in _POOL_DTYPES or v.dtype != dtype:
+        raise ValueError("KV pool dtype must be float32 or bfloat16")
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("KV pool tensors must be contiguous [L,P,S,H,D]")
+    if shape[2] != pool.block_size:
+        raise ValueError("pool.block_size does not match the KV tensor shape")
+    if not (0 <= layer_idx < shape[0]):
+        raise ValueError("layer_idx outside KV pool")
+    if k.get_device() != index or v.get_device() != index:
+        raise ValueError("all inputs must reside on same CUDA device")
+    return (k.data_ptr(), v.data_ptr(), *shape, _POOL_DTYPES[dtype])
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int, private: bool):

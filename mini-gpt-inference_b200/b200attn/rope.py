@@ -17,7 +17,11 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch, _pool_struct
+from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch,
+                  _pool_fields, _status_ptr)
+
+_PACK_ROPE = _lib.packer(_lib.QkNormRopeArgs).pack
+_PACK_APPEND = _lib.packer(_lib.RopeKvAppendArgs).pack
 
 
 def rope_table(max_positions: int, rotary_dim: int, *, base: float = 10000.0,
@@ -74,23 +78,24 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None
             raise ValueError(f"{name} must be its input itself or not overlap the inputs")
 
 
-def _rope_args(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out,
-               want_k, status):
-    """Checks the arguments both ops share; (struct, q_out, k_out)."""
+def _rope_fields(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out,
+                 status):
+    """Checks the arguments both ops share (v is None: no append); returns the
+    fields of _lib.QkNormRopeArgs, the outputs and the device."""
     if not q.is_cuda:
         raise ValueError("CUDA q required for the b200 backend")
     if q.ndim != 3 or k.ndim != 3:
         raise ValueError("q must have shape [T,Hq,D] and k [T,Hkv,D]")
     t, hq, d = q.shape
-    hkv = k.shape[1]
-    if k.shape[0] != t or k.shape[2] != d:
+    kt, hkv, kd = k.shape
+    if kt != t or kd != d:
         raise ValueError("q and k must agree in tokens and head dimension")
     if hq == 0 or hkv == 0 or d == 0:
         raise ValueError("q and k dimensions must be nonzero")
     dtype = q.dtype
     if dtype not in _DTYPES or k.dtype != dtype:
         raise ValueError("q and k must share a dtype: float32, bfloat16 or float16")
-    dev = q.device
+    index = q.get_device()
     if positions.dtype not in _INDEX or positions.shape != (t,):
         raise ValueError("positions must be a [T] integer tensor")
     if cos_sin.dtype != torch.float32 or cos_sin.ndim != 2 or not cos_sin.is_contiguous():
@@ -100,43 +105,45 @@ def _rope_args(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved
         raise ValueError("rotary_dim must be even and in [2, D]")
     if rows == 0:
         raise ValueError("cos_sin must have at least one row")
-    if k.device != dev or positions.device != dev or cos_sin.device != dev:
+    if (k.get_device() != index or positions.get_device() != index
+            or cos_sin.get_device() != index):
         raise ValueError("all inputs must reside on same CUDA device")
-    weight = q_weight if q_weight is not None else k_weight
-    wdtype = 0
+    wdtype = qw = kw = 0
+    weight = k_weight if q_weight is None else q_weight
     if weight is not None:
         for w in (q_weight, k_weight):
             if w is not None and (w.shape != (d,) or w.dtype not in _DTYPES
                                   or w.dtype != weight.dtype or not w.is_contiguous()
-                                  or w.device != dev):
+                                  or w.get_device() != index):
                 raise ValueError("norm weights must be contiguous [D] tensors of one float dtype "
                                  "on the q device")
         wdtype = _DTYPES[weight.dtype]
+        qw = 0 if q_weight is None else q_weight.data_ptr()
+        kw = 0 if k_weight is None else k_weight.data_ptr()
     if not eps > 0:
         raise ValueError("eps must be positive")
-    if status is not None and (status.dtype != torch.int32 or status.device != dev
-                               or status.numel() < 1):
-        raise ValueError("status must be an int32 tensor on the q device")
-    ins = (q, k) if v is None else (q, k, v)
-    if q_out is None:
-        q_out = torch.empty((t, hq, d), dtype=dtype, device=dev)
+    sp = 0 if status is None else _status_ptr(status, index)
+    if q_out is not None:
+        _check_out(q_out, q, "q_out", (q, k) if v is None else (q, k, v))
+        qs = q_out.stride()
     else:
-        _check_out(q_out, q, "q_out", ins)
-    kp = None
+        q_out = q.new_empty((t, hq, d))
+        qs = (hq * d, d, 1)
+    kp = 0
     ks = (0, 0, 0)
-    if want_k:
-        if k_out is None:
-            k_out = torch.empty((t, hkv, d), dtype=dtype, device=dev)
+    if v is None:
+        if k_out is not None:
+            _check_out(k_out, k, "k_out", (q, k, q_out))
+            ks = k_out.stride()
         else:
-            _check_out(k_out, k, "k_out", ins + (q_out,))
-        kp, ks = k_out.data_ptr(), k_out.stride()
-    args = _lib.QkNormRopeArgs(
-        t, hq, hkv, d, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), q_out.data_ptr(),
-        *q_out.stride(), kp, *ks, None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), cos_sin.data_ptr(), rows, rot,
-        positions.data_ptr(), positions.stride(0), None if status is None else status.data_ptr(),
-        _DTYPES[dtype], wdtype, _INDEX[positions.dtype], 1 if interleaved else 0, eps, 0)
-    return args, q_out, k_out
+            k_out = k.new_empty((t, hkv, d))
+            ks = (hkv * d, d, 1)
+        kp = k_out.data_ptr()
+    fields = (t, hq, hkv, d, q.data_ptr(), *q.stride(), k.data_ptr(), *k.stride(), q_out.data_ptr(),
+              *qs, kp, *ks, qw, kw, cos_sin.data_ptr(), rows, rot, positions.data_ptr(),
+              *positions.stride(), sp, _DTYPES[dtype], wdtype, _INDEX[positions.dtype],
+              1 if interleaved else 0, eps, 0)
+    return fields, q_out, k_out, index
 
 
 def qk_norm_rope_b200(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -161,13 +168,14 @@ def qk_norm_rope_b200(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     """
     _inference_only(q, k, q_weight, k_weight)
     lib = _lib.load()
-    args, q_out, k_out = _rope_args(q, k, None, positions, cos_sin, q_weight, k_weight, eps,
-                                    interleaved, q_out, k_out, True, status)
+    fields, q_out, k_out, index = _rope_fields(q, k, None, positions, cos_sin, q_weight, k_weight,
+                                               eps, interleaved, q_out, k_out, status)
+    args = _PACK_ROPE(*fields)
     if prepare:
-        return _DeviceCall(lib.b200_qk_norm_rope, args, q.device, (q_out, k_out),
+        return _DeviceCall(lib.b200_qk_norm_rope, args, index, (q_out, k_out),
                            "head norm and rotation",
                            (q, k, positions, cos_sin, q_weight, k_weight, status))
-    _launch(lib.b200_qk_norm_rope, args, q.device, "head norm and rotation")
+    _launch(lib.b200_qk_norm_rope, args, index, "head norm and rotation")
     return q_out, k_out
 
 
@@ -191,26 +199,23 @@ def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool,
     """
     _inference_only(q, k, v, q_weight, k_weight)
     lib = _lib.load()
-    if v.shape != k.shape or v.dtype != k.dtype or v.device != q.device:
+    if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != k.get_device():
         raise ValueError("k and v must have matching shape [T,Hkv,D], dtype and device")
-    rope, q_out, _ = _rope_args(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved,
-                                q_out, None, False, status)
-    pstruct = _pool_struct(pool)
-    if pool.k.shape[3:] != k.shape[1:]:
+    fields, q_out, _, index = _rope_fields(q, k, v, positions, cos_sin, q_weight, k_weight, eps,
+                                           interleaved, q_out, None, status)
+    pool_fields = _pool_fields(pool, index, layer_idx)
+    if pool_fields[5] != fields[2] or pool_fields[6] != fields[3]:
         raise ValueError("k/v head dimensions do not match the KV pool")
-    if not (0 <= layer_idx < pool.k.shape[0]):
-        raise ValueError("layer_idx outside KV pool")
-    dev = q.device
-    if pool.k.device != dev or pool.v.device != dev:
-        raise ValueError("all inputs must reside on same CUDA device")
-    slots = _index_tensor(slot_mapping, dev, "slot_mapping")
-    if slots.shape != (q.shape[0],):
+    slots = slot_mapping
+    if not (isinstance(slots, torch.Tensor) and slots.dtype in _INDEX and slots.get_device() == index):
+        slots = _index_tensor(slots, q.device, "slot_mapping")
+    if slots.shape != (fields[0],):
         raise ValueError("slot_mapping must have shape [T]")
-    args = _lib.RopeKvAppendArgs(rope, pstruct, layer_idx, v.data_ptr(), *v.stride(),
-                                 slots.data_ptr(), slots.stride(0), _INDEX[slots.dtype], 0)
+    args = _PACK_APPEND(*fields, *pool_fields, layer_idx, v.data_ptr(), *v.stride(),
+                        slots.data_ptr(), *slots.stride(), _INDEX[slots.dtype], 0)
     if prepare:
-        return _DeviceCall(lib.b200_rope_kv_append, args, dev, q_out, "rotary KV append",
+        return _DeviceCall(lib.b200_rope_kv_append, args, index, q_out, "rotary KV append",
                            (q, k, v, pool.k, pool.v, slots, positions, cos_sin, q_weight, k_weight,
                             status))
-    _launch(lib.b200_rope_kv_append, args, dev, "rotary KV append")
+    _launch(lib.b200_rope_kv_append, args, index, "rotary KV append")
     return q_out

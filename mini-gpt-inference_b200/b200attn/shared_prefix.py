@@ -11,7 +11,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch, _pool_struct
+from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch,
+                  _pool_fields, _status_ptr)
+
+_PACK = _lib.packer(_lib.SharedPrefixArgs).pack
 
 
 def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: int,
@@ -46,53 +49,52 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
         raise ValueError("q dimensions must be nonzero")
     if q.dtype not in _DTYPES:
         raise ValueError("q must be float32, bfloat16 or float16")
-    pstruct = _pool_struct(pool)
-    layers, _, block, h, pd = pool.k.shape
+    index = q.get_device()
+    pool_fields = _pool_fields(pool, index, layer_idx)
+    _, _, _, _, block, h, pd, kv_dtype = pool_fields
     if pd != d or hq % h:
         raise ValueError("the KV pool needs q's head dimension and a divisor of its heads")
-    if block_tables.ndim != 2 or block_tables.shape[0] != b or block_tables.shape[1] < 1:
+    if block_tables.ndim != 2:
+        raise ValueError("block_tables must have shape [B,M]")
+    rows, width = block_tables.shape
+    if rows != b or width < 1:
         raise ValueError("block_tables must have shape [B,M] with at least one block column")
     if context_lengths.shape != (b,):
         raise ValueError("context_lengths must have shape [B]")
     if block_tables.dtype not in _INDEX or context_lengths.dtype not in _INDEX:
         raise ValueError("block_tables and context_lengths must contain integers")
-    if not (0 <= layer_idx < layers):
-        raise ValueError("layer_idx outside KV pool")
     if prefix_len < 0:
         raise ValueError("prefix_len must be >= 0")
-    dev = q.device
-    if (pool.k.device != dev or pool.v.device != dev or block_tables.device != dev
-            or context_lengths.device != dev):
+    if block_tables.get_device() != index or context_lengths.get_device() != index:
         raise ValueError("all inputs must reside on same CUDA device")
-    table = _index_tensor(prefix_table, dev, "prefix_table")
+    table = prefix_table
+    if not (isinstance(table, torch.Tensor) and table.dtype in _INDEX and table.get_device() == index):
+        table = _index_tensor(table, q.device, "prefix_table")
     if table.ndim != 1:
         raise ValueError("prefix_table must be 1-D")
-    if table.shape[0] * block < prefix_len:
+    entries = table.shape[0]
+    if entries * block < prefix_len:
         raise ValueError("incomplete KV block table for prefix")
-    if status is not None and (status.dtype != torch.int32 or status.device != dev
-                               or status.numel() < 1):
-        raise ValueError("status must be an int32 tensor on the q device")
+    sp = 0 if status is None else _status_ptr(status, index)
     if out is None:
-        out = torch.empty((b, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != (b, hq, d) or out.dtype not in _DTYPES or out.device != dev:
+        out = q.new_empty((b, hq, d))
+    elif out.shape != (b, hq, d) or out.dtype not in _DTYPES or out.get_device() != index:
         raise ValueError("out must be a [B,Hq,D] tensor on the q device")
     qd = _DTYPES[q.dtype]
-    width = block_tables.shape[1]
     # A workspace of the call's own, from the allocator of the current stream
     # (or of the graph being captured): calls on other streams, and other
     # graphs' replays, have others.
     nbytes = lib.b200_shared_prefix_decode_workspace_size(b, hq, h, d, prefix_len, width, block,
-                                                          pstruct.dtype, qd)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args = _lib.SharedPrefixArgs(
-        pstruct, layer_idx, b, hq, prefix_len, width, q.data_ptr(), *q.stride(), out.data_ptr(),
-        *out.stride(), table.data_ptr(), table.shape[0], table.stride(0), block_tables.data_ptr(),
-        *block_tables.stride(), context_lengths.data_ptr(), context_lengths.stride(0),
-        ws.data_ptr(), nbytes, None if status is None else status.data_ptr(), qd,
-        _DTYPES[out.dtype], _INDEX[table.dtype], _INDEX[block_tables.dtype],
-        _INDEX[context_lengths.dtype], 0)
+                                                          kv_dtype, qd)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _PACK(
+        *pool_fields, layer_idx, b, hq, prefix_len, width, q.data_ptr(), *q.stride(), out.data_ptr(),
+        *out.stride(), table.data_ptr(), entries, *table.stride(), block_tables.data_ptr(),
+        *block_tables.stride(), context_lengths.data_ptr(), *context_lengths.stride(),
+        ws.data_ptr(), nbytes, sp, qd, _DTYPES[out.dtype], _INDEX[table.dtype],
+        _INDEX[block_tables.dtype], _INDEX[context_lengths.dtype], 0)
     if prepare:
-        return _DeviceCall(lib.b200_shared_prefix_decode, args, dev, out, "shared prefix decode",
+        return _DeviceCall(lib.b200_shared_prefix_decode, args, index, out, "shared prefix decode",
                            (q, pool.k, pool.v, table, block_tables, context_lengths, status, ws))
-    _launch(lib.b200_shared_prefix_decode, args, dev, "shared prefix decode")
+    _launch(lib.b200_shared_prefix_decode, args, index, "shared prefix decode")
     return out
