@@ -10,6 +10,7 @@
 // bytes; what a small call costs is the launch and the chain position ->
 // table row -> store.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -46,210 +47,250 @@ struct RopeParams {
   float eps, inv_d;
 };
 
-// Elem, Pack: one 16-byte chunk of the input type as floats and back.
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// One 16-byte chunk of the input type: N elements, as N / 2 pairs of floats.
 template <typename T>
-struct Chunk;
-template <>
-struct Chunk<float> {
-  static constexpr int N = 4;
-  __device__ __forceinline__ static void unpack(const uint4& c, float* f) { Elem<float>::unpack(c, f); }
-};
-template <>
-struct Chunk<__nv_bfloat16> {
-  static constexpr int N = 8;
-  __device__ __forceinline__ static void unpack(const uint4& c, float* f) {
-    Elem<__nv_bfloat16>::unpack(c, f);
-  }
-};
-template <>
-struct Chunk<__half> {
-  static constexpr int N = 8;
-  __device__ __forceinline__ static void unpack(const uint4& c, float* f) {
+struct Chunk {
+  static constexpr int N = 16 / sizeof(T);
+  __device__ __forceinline__ static void unpack(const uint4& c, float2* f) {
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    if constexpr (sizeof(T) == 4) {
+      f[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      f[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value)
+          f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        else
+          f[i] = bf16x2_to_float2(w[i]);
+      }
     }
   }
 };
 
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t pack2(float2 f) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
 
-// Stores N (4 or 8) consecutive floats as T, in 8- or 16-byte stores.
-template <typename T, int N>
-__device__ __forceinline__ void store_chunk(T* dst, const float* f) {
+// Stores P (2 or 4) pairs as T.
+template <typename T, int P>
+__device__ __forceinline__ void store_chunk(T* dst, const float2* f) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<float4*>(dst + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-  } else if constexpr (N == 8) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]),
-                                                pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+    for (int i = 0; i < P; i += 2)
+      *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(f[i].x, f[i].y, f[i + 1].x, f[i + 1].y);
+  } else if constexpr (P == 4) {
+    *reinterpret_cast<uint4*>(dst) =
+        make_uint4(pack2<T>(f[0]), pack2<T>(f[1]), pack2<T>(f[2]), pack2<T>(f[3]));
   } else {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(f[0]), pack2<T>(f[1]));
   }
 }
 
-// The weights of one chunk (input type or f32) as floats.
+// The weights of one chunk (input type or f32).
 template <typename In>
-__device__ __forceinline__ void load_weight(const void* w, int weight_dtype, int e0, float* f) {
-  constexpr int N = Chunk<In>::N;
+__device__ __forceinline__ void load_weight(const void* w, int weight_dtype, int e0, float2* f) {
+  constexpr int P = Chunk<In>::N / 2;
   if (weight_dtype == B200_DTYPE_F32) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      Elem<float>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e0 + i)),
-                          f + i);
+    for (int i = 0; i < P; i += 2)
+      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e0 + 2 * i)),
+                           f + i);
   } else {
     Chunk<In>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const In*>(w) + e0)), f);
   }
 }
 
-// Where a head row of a token lies: which tensor, which head.
 enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
 
-// Vector path.  One CTA per token; LPH lanes (a power of two) share a head
-// row, lane j owning two 16-byte chunks: (j, j + R/2) of the rotated part in
-// the split form, (2j, 2j + 1) otherwise, so that both elements of every pair
-// are in one lane, the pairs of lane j are i = j*N .. j*N + N - 1 in either
-// form, and the table's values stay in registers over the token's rows.  Each
-// lane writes exactly the elements it read, so q_out may be q.
-// A thread loads the chunks of up to U rows before it stores the first.
-template <typename In, typename PoolT, int U>
-__global__ void __launch_bounds__(256) rope_vec_kernel(const RopeParams p, const int lph_shift) {
-  constexpr int N = Chunk<In>::N;
-  const int64_t t = blockIdx.x;
-  const int lph = 1 << lph_shift;
-  const int j = threadIdx.x & (lph - 1);
-  const int group = threadIdx.x >> lph_shift;
-  const int groups = blockDim.x >> lph_shift;
-  const int pairs = p.D / (2 * N);   // lanes that own chunks
-  const int turned = p.R / (2 * N);  // of which these are rotated
+// Head rows a warp takes together (rounds), and the jobs of a token: up to kU
+// rounds of one kind each.
+constexpr int kU = 2;
+constexpr int kJobWarps = 4;  // per CTA
+
+// Vector path: a warp per job, tokens' jobs end to end.  LPH lanes (a power of two)
+// share a head row, lane j owning two 16-byte chunks: (j, j + R/2) of the
+// rotated part in the split form, (2j, 2j + 1) otherwise, so that both elements
+// of every pair are in one lane, and the pairs of lane j are i = j N .. j N + N
+// - 1 in either form.  Norm weight and rotation are combined once per job into
+//   a' = a A + o B,   b' = b C + o' D     (o, o' the chunks' partners)
+// so that a row costs two packed products an element pair; all loads of a job
+// are on their way before the first sum.  Each lane writes exactly the
+// elements that it read, so q_out may be q.
+// 8192 tokens of 32 + 8 heads of 128, bf16: <t> us, <r> TB/s (27 us at the copy
+// rate); with a row's kind, weights and addresses worked out row by row it was
+// 57 us and bound by its instructions.
+template <typename In, typename PoolT, bool INTER>
+__global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_constant__ RopeParams p,
+                                                                 const int lph_shift, const int jobs_q,
+                                                                 const int jobs_k, const int64_t all_jobs) {
+  constexpr int N = Chunk<In>::N, P = N / 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t index = static_cast<int64_t>(blockIdx.x) * kJobWarps + (threadIdx.x >> 5);
+  if (index >= all_jobs) return;
+  const int jobs = jobs_q + jobs_k * (p.append ? 2 : 1);  // of a token
+  const int64_t t = index / jobs;
+  const int job = static_cast<int>(index - t * jobs);
+  const int j = lane & ((1 << lph_shift) - 1);
+  const int sub = lane >> lph_shift;     // row of a round
+  const int rpw = 32 >> lph_shift;       // rows of a round
+  const int pairs = p.D / (2 * N);       // lanes that own chunks
+  const int turned = p.R / (2 * N);      // of which these are rotated
   const bool mine = j < pairs;
   const bool rot = j < turned;
-  const bool split = rot && !p.interleaved;
-  const int ea = (split ? j : 2 * j) * N;                   // first element of chunk a
-  const int eb = (split ? j + turned : 2 * j + 1) * N;      // and of chunk b
+  const bool split = rot && !INTER;
+  const int ea = (split ? j : 2 * j) * N;               // first element of chunk a
+  const int eb = (split ? j + turned : 2 * j + 1) * N;  // and of chunk b
 
   const int64_t pos = load_index(p.positions, t * p.pos_stride, p.pos_i64);
   const int64_t slot = p.append ? load_index(p.slots, t * p.slot_stride, p.slots_i64) : 0;
+  const int kind = job < jobs_q ? kRowQ : job < jobs_q + jobs_k ? kRowK : kRowV;
+  const int row0 = (kind == kRowQ ? job : kind == kRowK ? job - jobs_q : job - jobs_q - jobs_k) * (kU * rpw) + sub;
+  const int rows = kind == kRowQ ? p.Hq : p.Hkv;
+  const In* src = kind == kRowQ   ? static_cast<const In*>(p.q) + t * p.qs0
+                  : kind == kRowK ? static_cast<const In*>(p.k) + t * p.ks0
+                                  : static_cast<const In*>(p.v) + t * p.vs0;
+  const int64_t step = kind == kRowQ ? p.qs1 : kind == kRowK ? p.ks1 : p.vs1;
+  src += row0 * step;
+  uint4 ca[kU], cb[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    ca[u] = cb[u] = make_uint4(0, 0, 0, 0);
+    if (mine && row0 + u * rpw < rows) {
+      ca[u] = *reinterpret_cast<const uint4*>(src + u * rpw * step + ea);
+      cb[u] = *reinterpret_cast<const uint4*>(src + u * rpw * step + eb);
+    }
+  }
   const bool pos_ok = pos >= 0 && pos < p.table_rows;
   const bool slot_ok = !p.append || (slot >= 0 && slot < p.pool_slots);
-  if (threadIdx.x == 0 && !(pos_ok && slot_ok))
+  if (job == 0 && lane == 0 && !(pos_ok && slot_ok))
     report(p.status, (pos_ok ? 0 : B200_DEV_BAD_POSITION) | (slot_ok ? 0 : B200_DEV_BAD_SLOT));
+  const bool to_pool = p.append && kind != kRowQ;
+  if (to_pool && !(pos_ok && slot_ok)) return;
+  PoolT* pool = nullptr;
+  if (to_pool)
+    pool = static_cast<PoolT*>(kind == kRowK ? p.k_pool : p.v_pool) +
+           ((p.layer_row0 + slot) * p.Hkv + row0) * p.D;
 
-  float c[N], s[N];
+  if (kind == kRowV) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    c[i] = 1.f;
-    s[i] = 0.f;
+    for (int u = 0; u < kU; ++u) {
+      if (!mine || row0 + u * rpw >= rows) continue;
+      PoolT* dst = pool + static_cast<int64_t>(u * rpw) * p.D;
+      if constexpr (std::is_same<In, PoolT>::value) {  // values as they are
+        *reinterpret_cast<uint4*>(dst + ea) = ca[u];
+        *reinterpret_cast<uint4*>(dst + eb) = cb[u];
+      } else {
+        float2 f[P];
+        Chunk<In>::unpack(ca[u], f);
+        store_chunk<PoolT, P>(dst + ea, f);
+        Chunk<In>::unpack(cb[u], f);
+        store_chunk<PoolT, P>(dst + eb, f);
+      }
+    }
+    return;
+  }
+
+  // A, C: the weights (times the cosines); B, D: the partners' sines.
+  const void* weight = kind == kRowQ ? p.q_weight : p.k_weight;
+  float2 A[P], B[P], C[P], D[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) A[i] = C[i] = make_float2(1.f, 1.f);
+  if (weight != nullptr && mine) {
+    load_weight<In>(weight, p.weight_dtype, ea, A);
+    load_weight<In>(weight, p.weight_dtype, eb, C);
   }
   if (rot && pos_ok) {
+    float2 c[P], s[P];
     const float* row = p.cos_sin + pos * p.R + j * N;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      Elem<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + i)), c + i);
-      Elem<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + p.R / 2 + i)), s + i);
+    for (int i = 0; i < P; i += 2) {
+      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + 2 * i)), c + i);
+      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + p.R / 2 + 2 * i)), s + i);
     }
+    if constexpr (!INTER) {  // a' = a wa c - b wb s,  b' = b wb c + a wa s
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        B[i] = fmul2(C[i], make_float2(-s[i].x, -s[i].y));
+        D[i] = fmul2(A[i], s[i]);
+        A[i] = fmul2(A[i], c[i]);
+        C[i] = fmul2(C[i], c[i]);
+      }
+    } else {  // (x, y)' = (x wx, y wy) c + (-y wy, x wx) s, a word of the chunk a pair
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        // Pair i of chunk a and pair P + i of the lane (chunk b).
+        const float ca_ = i & 1 ? c[i / 2].y : c[i / 2].x, sa_ = i & 1 ? s[i / 2].y : s[i / 2].x;
+        const float cb_ = i & 1 ? c[(P + i) / 2].y : c[(P + i) / 2].x;
+        const float sb_ = i & 1 ? s[(P + i) / 2].y : s[(P + i) / 2].x;
+        B[i] = make_float2(-A[i].y * sa_, A[i].x * sa_);
+        D[i] = make_float2(-C[i].y * sb_, C[i].x * sb_);
+        A[i] = make_float2(A[i].x * ca_, A[i].y * ca_);
+        C[i] = make_float2(C[i].x * cb_, C[i].y * cb_);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) B[i] = D[i] = make_float2(0.f, 0.f);
   }
 
-  for (int r0 = group; r0 - group < p.rows; r0 += U * groups) {
-    uint4 ca[U], cb[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * groups;
-      ca[u] = cb[u] = make_uint4(0, 0, 0, 0);
-      if (r < p.rows && mine) {
-        const In* src;
-        if (r < p.Hq)
-          src = static_cast<const In*>(p.q) + t * p.qs0 + r * p.qs1;
-        else if (r < p.Hq + p.Hkv)
-          src = static_cast<const In*>(p.k) + t * p.ks0 + (r - p.Hq) * p.ks1;
-        else
-          src = static_cast<const In*>(p.v) + t * p.vs0 + (r - p.Hq - p.Hkv) * p.vs1;
-        ca[u] = *reinterpret_cast<const uint4*>(src + ea);
-        cb[u] = *reinterpret_cast<const uint4*>(src + eb);
+  for (int u = 0; u < kU; ++u) {
+    float2 a[P], b[P];
+    Chunk<In>::unpack(ca[u], a);
+    Chunk<In>::unpack(cb[u], b);
+    if (weight != nullptr) {  // the same for the whole warp
+      float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < P; ++i) ss = ffma2(a[i], a[i], ffma2(b[i], b[i], ss));
+      float sum = ss.x + ss.y;
+      for (int o = 1; o < 1 << lph_shift; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const float inv = rsqrtf(fmaf(sum, p.inv_d, p.eps));
+      const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        a[i] = fmul2(a[i], inv2);
+        b[i] = fmul2(b[i], inv2);
       }
     }
+    if (!mine || row0 + u * rpw >= rows) continue;
+    float2 x[P], y[P];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // Uniform over the row's lanes, not over the warp: every lane takes
-      // part in the shuffles below.
-      const int r = r0 + u * groups;
-      const int kind = r < p.Hq ? kRowQ : r < p.Hq + p.Hkv ? kRowK : kRowV;
-      float a[N], b[N];
-      Chunk<In>::unpack(ca[u], a);
-      Chunk<In>::unpack(cb[u], b);
-      const void* w = kind == kRowQ ? p.q_weight : kind == kRowK ? p.k_weight : nullptr;
-      if (p.q_weight != nullptr || p.k_weight != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        for (int o = lph >> 1; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w != nullptr && mine) {
-          const float inv = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-          float wa[N], wb[N];
-          load_weight<In>(w, p.weight_dtype, ea, wa);
-          load_weight<In>(w, p.weight_dtype, eb, wb);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            a[i] *= inv * wa[i];
-            b[i] *= inv * wb[i];
-          }
-        }
+    for (int i = 0; i < P; ++i) {
+      x[i] = fmul2(a[i], A[i]);
+      y[i] = fmul2(b[i], C[i]);
+      if (rot) {  // unrotated elements take nothing of a partner (0 * inf is NaN)
+        x[i] = ffma2(INTER ? make_float2(a[i].y, a[i].x) : b[i], B[i], x[i]);
+        y[i] = ffma2(INTER ? make_float2(b[i].y, b[i].x) : a[i], D[i], y[i]);
       }
-      if (r >= p.rows || !mine) continue;
-      if (kind != kRowV && rot) {
-        if (!p.interleaved) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = x * c[i] - y * s[i];
-            b[i] = x * s[i] + y * c[i];
-          }
-        } else {
-          // Pair i of the lane: elements 2i, 2i + 1 of its 2N consecutive ones.
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            float& x0 = 2 * i < N ? a[(2 * i) % N] : b[(2 * i) % N];
-            float& y0 = 2 * i < N ? a[(2 * i + 1) % N] : b[(2 * i + 1) % N];
-            const float x = x0, y = y0;
-            x0 = x * c[i] - y * s[i];
-            y0 = x * s[i] + y * c[i];
-          }
-        }
-      }
-      if (!pos_ok) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) a[i] = b[i] = 0.f;
-      }
-      if (kind == kRowQ || !p.append) {
-        In* dst = kind == kRowQ ? static_cast<In*>(p.q_out) + t * p.qo0 + r * p.qo1
-                                : static_cast<In*>(p.k_out) + t * p.ko0 + (r - p.Hq) * p.ko1;
-        store_chunk<In, N>(dst + ea, a);
-        store_chunk<In, N>(dst + eb, b);
-      } else if (pos_ok && slot_ok) {
-        const int head = kind == kRowK ? r - p.Hq : r - p.Hq - p.Hkv;
-        PoolT* dst = static_cast<PoolT*>(kind == kRowK ? p.k_pool : p.v_pool) +
-                     ((p.layer_row0 + slot) * p.Hkv + head) * p.D;
-        if (std::is_same<In, PoolT>::value && kind == kRowV) {  // values as they are
-          *reinterpret_cast<uint4*>(dst + ea) = ca[u];
-          *reinterpret_cast<uint4*>(dst + eb) = cb[u];
-        } else {
-          store_chunk<PoolT, N>(dst + ea, a);
-          store_chunk<PoolT, N>(dst + eb, b);
-        }
-      }
+      if (!pos_ok) x[i] = y[i] = make_float2(0.f, 0.f);
+    }
+    if (to_pool) {
+      PoolT* dst = pool + static_cast<int64_t>(u * rpw) * p.D;
+      store_chunk<PoolT, P>(dst + ea, x);
+      store_chunk<PoolT, P>(dst + eb, y);
+    } else {
+      In* dst = kind == kRowQ
+                    ? static_cast<In*>(p.q_out) + t * p.qo0 + static_cast<int64_t>(row0 + u * rpw) * p.qo1
+                    : static_cast<In*>(p.k_out) + t * p.ko0 + static_cast<int64_t>(row0 + u * rpw) * p.ko1;
+      store_chunk<In, P>(dst + ea, x);
+      store_chunk<In, P>(dst + eb, y);
     }
   }
 }
@@ -343,32 +384,27 @@ bool rows_vec(const void* p, const int64_t* st, size_t es) {
 }
 
 template <typename In, typename PoolT>
-void launch_vec(const RopeParams& p, int64_t tokens, int num_sms, cudaStream_t stream) {
+int launch_vec(const RopeParams& p, int64_t tokens, cudaStream_t stream) {
   constexpr int N = Chunk<In>::N;
-  const int pairs = p.D / (2 * N);
-  const int shift = log2i(pairs);
-  const int lph = 1 << shift;
-  // Up to 256 threads per token, the token's rows dealt out evenly.
-  const int groups_max = 256 / lph;
-  const int iters = static_cast<int>(ceil_div(p.rows, groups_max));
-  const int groups = static_cast<int>(ceil_div(p.rows, iters));
-  const unsigned threads = static_cast<unsigned>((groups * lph + 31) / 32 * 32);
-  const unsigned grid = static_cast<unsigned>(tokens);
-  if (iters == 1)
-    rope_vec_kernel<In, PoolT, 1><<<grid, threads, 0, stream>>>(p, shift);
-  else if (iters == 2)
-    rope_vec_kernel<In, PoolT, 2><<<grid, threads, 0, stream>>>(p, shift);
+  const int shift = log2i(p.D / (2 * N));
+  const int per_job = kU * (32 >> shift);
+  const int jobs_q = static_cast<int>(ceil_div(p.Hq, per_job)), jobs_k = static_cast<int>(ceil_div(p.Hkv, per_job));
+  const int64_t jobs = tokens * (jobs_q + jobs_k * (p.append ? 2 : 1));
+  const int64_t grid = ceil_div(jobs, kJobWarps);
+  if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "rotation: too many head rows");
+  if (p.interleaved)
+    rope_vec_kernel<In, PoolT, true>
+        <<<static_cast<unsigned>(grid), kJobWarps * 32, 0, stream>>>(p, shift, jobs_q, jobs_k, jobs);
   else
-    rope_vec_kernel<In, PoolT, 3><<<grid, threads, 0, stream>>>(p, shift);
+    rope_vec_kernel<In, PoolT, false>
+        <<<static_cast<unsigned>(grid), kJobWarps * 32, 0, stream>>>(p, shift, jobs_q, jobs_k, jobs);
+  return B200_OK;
 }
 
 }  // namespace
 
 int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_append_args_t* append,
                         cudaStream_t stream) {
-  DeviceInfo dev;
-  int rc = current_device_info(&dev);
-  if (rc != B200_OK) return rc;
   RopeParams p{};
   p.q = a.q;
   p.k = a.k;
@@ -425,23 +461,25 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
           (a.q_weight == nullptr || aligned16(a.q_weight)) &&
           (a.k_weight == nullptr || aligned16(a.k_weight));
   if (vec) {
+    int rc = B200_OK;
     const bool pool_f32 = p.pool_dtype == B200_DTYPE_F32;
     if (a.dtype == B200_DTYPE_F32) {
       if (pool_f32)
-        launch_vec<float, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<float, float>(p, a.num_tokens, stream);
       else
-        launch_vec<float, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<float, __nv_bfloat16>(p, a.num_tokens, stream);
     } else if (a.dtype == B200_DTYPE_BF16) {
       if (pool_f32)
-        launch_vec<__nv_bfloat16, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__nv_bfloat16, float>(p, a.num_tokens, stream);
       else
-        launch_vec<__nv_bfloat16, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__nv_bfloat16, __nv_bfloat16>(p, a.num_tokens, stream);
     } else {
       if (pool_f32)
-        launch_vec<__half, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__half, float>(p, a.num_tokens, stream);
       else
-        launch_vec<__half, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__half, __nv_bfloat16>(p, a.num_tokens, stream);
     }
+    if (rc != B200_OK) return rc;
   } else {
     const unsigned threads = static_cast<unsigned>(std::min(256, p.rows * 32));
     rope_any_kernel<<<static_cast<unsigned>(a.num_tokens), threads, 0, stream>>>(p);
