@@ -119,12 +119,12 @@ __device__ __forceinline__ void load_weight(const void* w, int weight_dtype, int
 
 enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
 
-// Head rows a warp takes together (rounds), and the jobs of a token: up to kU
-// rounds of one kind each.
-constexpr int kU = 2;
-constexpr int kJobWarps = 4;  // per CTA
+constexpr int kJobWarps = 4;  // warps per CTA
 
-// Vector path: a warp per job, tokens' jobs end to end.  LPH lanes (a power of two)
+
+// Vector path.  A round is the head rows a warp takes side by side, a job up to
+// U rounds of one kind (queries, keys, values) of a token; a warp per job,
+// tokens' jobs end to end.  LPH lanes (a power of two)
 // share a head row, lane j owning two 16-byte chunks: (j, j + R/2) of the
 // rotated part in the split form, (2j, 2j + 1) otherwise, so that both elements
 // of every pair are in one lane, and the pairs of lane j are i = j N .. j N + N
@@ -133,20 +133,24 @@ constexpr int kJobWarps = 4;  // per CTA
 // so that a row costs two packed products an element pair; all loads of a job
 // are on their way before the first sum.  Each lane writes exactly the
 // elements that it read, so q_out may be q.
-// 8192 tokens of 32 + 8 heads of 128, bf16: <t> us, <r> TB/s (27 us at the copy
-// rate); with a row's kind, weights and addresses worked out row by row it was
-// 57 us and bound by its instructions.
-template <typename In, typename PoolT, bool INTER>
-__global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_constant__ RopeParams p,
-                                                                 const int lph_shift, const int jobs_q,
-                                                                 const int jobs_k, const int64_t all_jobs) {
+// 8192 tokens of 32 + 8 heads of 128, bf16: 35 us, 4.9 TB/s (27 us at the copy
+// rate), 32 + 32 heads with the append 67 us, 6.1 TB/s (64); with a row's kind,
+// weights and addresses worked out row by row 57 and 108 us, bound by
+// instructions.  U: 4 where the warps fill the GPU all the same (with 2: 38 and
+// 78 us), else 2 (64 tokens: 2.8 us, with 4: 3.3 us).
+// SHIFT: log2(LPH) where it is known (heads of 128), else -1.
+template <typename In, typename PoolT, bool INTER, int SHIFT, int U>
+__global__ void __launch_bounds__(kJobWarps * 32)
+    rope_vec_kernel(const __grid_constant__ RopeParams p, const int shift_arg, const uint32_t jobs_q,
+                    const uint32_t jobs_k, const uint32_t jobs, const uint32_t all_jobs, const int64_t t0) {
   constexpr int N = Chunk<In>::N, P = N / 2;
+  const int lph_shift = SHIFT >= 0 ? SHIFT : shift_arg;
   const int lane = threadIdx.x & 31;
-  const int64_t index = static_cast<int64_t>(blockIdx.x) * kJobWarps + (threadIdx.x >> 5);
+  const uint32_t index = blockIdx.x * kJobWarps + (threadIdx.x >> 5);
   if (index >= all_jobs) return;
-  const int jobs = jobs_q + jobs_k * (p.append ? 2 : 1);  // of a token
-  const int64_t t = index / jobs;
-  const int job = static_cast<int>(index - t * jobs);
+  const uint32_t token = index / jobs;  // of this launch
+  const uint32_t job = index - token * jobs;
+  const int64_t t = t0 + token;
   const int j = lane & ((1 << lph_shift) - 1);
   const int sub = lane >> lph_shift;     // row of a round
   const int rpw = 32 >> lph_shift;       // rows of a round
@@ -161,16 +165,18 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
   const int64_t pos = load_index(p.positions, t * p.pos_stride, p.pos_i64);
   const int64_t slot = p.append ? load_index(p.slots, t * p.slot_stride, p.slots_i64) : 0;
   const int kind = job < jobs_q ? kRowQ : job < jobs_q + jobs_k ? kRowK : kRowV;
-  const int row0 = (kind == kRowQ ? job : kind == kRowK ? job - jobs_q : job - jobs_q - jobs_k) * (kU * rpw) + sub;
+  const int row0 = static_cast<int>(kind == kRowQ   ? job
+                                    : kind == kRowK ? job - jobs_q
+                                                    : job - jobs_q - jobs_k) * (U * rpw) + sub;
   const int rows = kind == kRowQ ? p.Hq : p.Hkv;
   const In* src = kind == kRowQ   ? static_cast<const In*>(p.q) + t * p.qs0
                   : kind == kRowK ? static_cast<const In*>(p.k) + t * p.ks0
                                   : static_cast<const In*>(p.v) + t * p.vs0;
   const int64_t step = kind == kRowQ ? p.qs1 : kind == kRowK ? p.ks1 : p.vs1;
   src += row0 * step;
-  uint4 ca[kU], cb[kU];
+  uint4 ca[U], cb[U];
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
+  for (int u = 0; u < U; ++u) {
     ca[u] = cb[u] = make_uint4(0, 0, 0, 0);
     if (mine && row0 + u * rpw < rows) {
       ca[u] = *reinterpret_cast<const uint4*>(src + u * rpw * step + ea);
@@ -182,7 +188,24 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
   if (job == 0 && lane == 0 && !(pos_ok && slot_ok))
     report(p.status, (pos_ok ? 0 : B200_DEV_BAD_POSITION) | (slot_ok ? 0 : B200_DEV_BAD_SLOT));
   const bool to_pool = p.append && kind != kRowQ;
-  if (to_pool && !(pos_ok && slot_ok)) return;
+  In* out = nullptr;
+  int64_t out_step = 0;
+  if (!to_pool) {
+    out = kind == kRowQ ? static_cast<In*>(p.q_out) + t * p.qo0 : static_cast<In*>(p.k_out) + t * p.ko0;
+    out_step = kind == kRowQ ? p.qo1 : p.ko1;
+    out += row0 * out_step;
+  }
+  if (!(pos_ok && (slot_ok || !to_pool))) {  // nothing for the pool, zeros for the rest
+    float2 z[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) z[i] = make_float2(0.f, 0.f);
+    for (int u = 0; u < U; ++u)
+      if (!to_pool && mine && row0 + u * rpw < rows) {
+        store_chunk<In, P>(out + u * rpw * out_step + ea, z);
+        store_chunk<In, P>(out + u * rpw * out_step + eb, z);
+      }
+    return;
+  }
   PoolT* pool = nullptr;
   if (to_pool)
     pool = static_cast<PoolT*>(kind == kRowK ? p.k_pool : p.v_pool) +
@@ -190,7 +213,7 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
 
   if (kind == kRowV) {
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (!mine || row0 + u * rpw >= rows) continue;
       PoolT* dst = pool + static_cast<int64_t>(u * rpw) * p.D;
       if constexpr (std::is_same<In, PoolT>::value) {  // values as they are
@@ -216,7 +239,7 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
     load_weight<In>(weight, p.weight_dtype, ea, A);
     load_weight<In>(weight, p.weight_dtype, eb, C);
   }
-  if (rot && pos_ok) {
+  if (rot) {
     float2 c[P], s[P];
     const float* row = p.cos_sin + pos * p.R + j * N;
 #pragma unroll
@@ -251,7 +274,7 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
   }
 
 #pragma unroll
-  for (int u = 0; u < kU; ++u) {
+  for (int u = 0; u < U; ++u) {
     float2 a[P], b[P];
     Chunk<In>::unpack(ca[u], a);
     Chunk<In>::unpack(cb[u], b);
@@ -260,7 +283,9 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < P; ++i) ss = ffma2(a[i], a[i], ffma2(b[i], b[i], ss));
       float sum = ss.x + ss.y;
-      for (int o = 1; o < 1 << lph_shift; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+      for (int o = 0; o < (SHIFT >= 0 ? SHIFT : 5); ++o)
+        if (SHIFT >= 0 || o < lph_shift) sum += __shfl_xor_sync(0xffffffffu, sum, 1 << o);
       const float inv = rsqrtf(fmaf(sum, p.inv_d, p.eps));
       const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
@@ -279,16 +304,13 @@ __global__ void __launch_bounds__(kJobWarps * 32) rope_vec_kernel(const __grid_c
         x[i] = ffma2(INTER ? make_float2(a[i].y, a[i].x) : b[i], B[i], x[i]);
         y[i] = ffma2(INTER ? make_float2(b[i].y, b[i].x) : a[i], D[i], y[i]);
       }
-      if (!pos_ok) x[i] = y[i] = make_float2(0.f, 0.f);
     }
     if (to_pool) {
       PoolT* dst = pool + static_cast<int64_t>(u * rpw) * p.D;
       store_chunk<PoolT, P>(dst + ea, x);
       store_chunk<PoolT, P>(dst + eb, y);
     } else {
-      In* dst = kind == kRowQ
-                    ? static_cast<In*>(p.q_out) + t * p.qo0 + static_cast<int64_t>(row0 + u * rpw) * p.qo1
-                    : static_cast<In*>(p.k_out) + t * p.ko0 + static_cast<int64_t>(row0 + u * rpw) * p.ko1;
+      In* dst = out + u * rpw * out_step;
       store_chunk<In, P>(dst + ea, x);
       store_chunk<In, P>(dst + eb, y);
     }
@@ -383,28 +405,45 @@ bool rows_vec(const void* p, const int64_t* st, size_t es) {
          (st[1] * static_cast<int64_t>(es)) % 16 == 0;
 }
 
-template <typename In, typename PoolT>
-int launch_vec(const RopeParams& p, int64_t tokens, cudaStream_t stream) {
+template <typename In, typename PoolT, int U>
+int launch_jobs(const RopeParams& p, int64_t tokens, cudaStream_t stream) {
   constexpr int N = Chunk<In>::N;
+  constexpr int kShift128 = N == 8 ? 3 : 4;
   const int shift = log2i(p.D / (2 * N));
-  const int per_job = kU * (32 >> shift);
-  const int jobs_q = static_cast<int>(ceil_div(p.Hq, per_job)), jobs_k = static_cast<int>(ceil_div(p.Hkv, per_job));
-  const int64_t jobs = tokens * (jobs_q + jobs_k * (p.append ? 2 : 1));
-  const int64_t grid = ceil_div(jobs, kJobWarps);
-  if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "rotation: too many head rows");
-  if (p.interleaved)
-    rope_vec_kernel<In, PoolT, true>
-        <<<static_cast<unsigned>(grid), kJobWarps * 32, 0, stream>>>(p, shift, jobs_q, jobs_k, jobs);
-  else
-    rope_vec_kernel<In, PoolT, false>
-        <<<static_cast<unsigned>(grid), kJobWarps * 32, 0, stream>>>(p, shift, jobs_q, jobs_k, jobs);
-  return B200_OK;
+  const int per_job = U * (32 >> shift);
+  const uint32_t jobs_q = static_cast<uint32_t>(ceil_div(p.Hq, per_job));
+  const uint32_t jobs_k = static_cast<uint32_t>(ceil_div(p.Hkv, per_job));
+  const uint32_t jobs = jobs_q + jobs_k * (p.append ? 2 : 1);
+  auto kern = shift == kShift128 ? (p.interleaved ? rope_vec_kernel<In, PoolT, true, kShift128, U>
+                                                  : rope_vec_kernel<In, PoolT, false, kShift128, U>)
+                                 : (p.interleaved ? rope_vec_kernel<In, PoolT, true, -1, U>
+                                                  : rope_vec_kernel<In, PoolT, false, -1, U>);
+  // Job numbers are 32-bit: very many tokens take several launches.
+  const int64_t most = (int64_t(1) << 31) / jobs;
+  for (int64_t t0 = 0; t0 < tokens; t0 += most) {
+    const uint32_t all = static_cast<uint32_t>(std::min(most, tokens - t0) * jobs);
+    kern<<<(all + kJobWarps - 1) / kJobWarps, kJobWarps * 32, 0, stream>>>(p, shift, jobs_q, jobs_k, jobs, all, t0);
+  }
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "rotation launch");
+}
+
+template <typename In, typename PoolT>
+int launch_vec(const RopeParams& p, int64_t tokens, int num_sms, cudaStream_t stream) {
+  const int shift = log2i(p.D / (2 * Chunk<In>::N));
+  const int64_t rounds = tokens * (ceil_div(p.rows, 32 >> shift));
+  // About 20 warps of four rounds to an SM.
+  if (rounds >= int64_t(4) * 20 * num_sms) return launch_jobs<In, PoolT, 4>(p, tokens, stream);
+  return launch_jobs<In, PoolT, 2>(p, tokens, stream);
 }
 
 }  // namespace
 
 int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_append_args_t* append,
                         cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc != B200_OK) return rc;
   RopeParams p{};
   p.q = a.q;
   p.k = a.k;
@@ -461,25 +500,24 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
           (a.q_weight == nullptr || aligned16(a.q_weight)) &&
           (a.k_weight == nullptr || aligned16(a.k_weight));
   if (vec) {
-    int rc = B200_OK;
     const bool pool_f32 = p.pool_dtype == B200_DTYPE_F32;
     if (a.dtype == B200_DTYPE_F32) {
       if (pool_f32)
-        rc = launch_vec<float, float>(p, a.num_tokens, stream);
+        rc = launch_vec<float, float>(p, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<float, __nv_bfloat16>(p, a.num_tokens, stream);
+        rc = launch_vec<float, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
     } else if (a.dtype == B200_DTYPE_BF16) {
       if (pool_f32)
-        rc = launch_vec<__nv_bfloat16, float>(p, a.num_tokens, stream);
+        rc = launch_vec<__nv_bfloat16, float>(p, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<__nv_bfloat16, __nv_bfloat16>(p, a.num_tokens, stream);
+        rc = launch_vec<__nv_bfloat16, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
     } else {
       if (pool_f32)
-        rc = launch_vec<__half, float>(p, a.num_tokens, stream);
+        rc = launch_vec<__half, float>(p, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<__half, __nv_bfloat16>(p, a.num_tokens, stream);
+        rc = launch_vec<__half, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
     }
-    if (rc != B200_OK) return rc;
+    return rc;
   } else {
     const unsigned threads = static_cast<unsigned>(std::min(256, p.rows * 32));
     rope_any_kernel<<<static_cast<unsigned>(a.num_tokens), threads, 0, stream>>>(p);

@@ -103,6 +103,32 @@ def test_norm_rope_in_place_gives_the_same(size):
     assert torch.equal(v, v0)  # the third view of the same rows
 
 
+@pytest.mark.parametrize("size,dtype,interleaved", [((1301, 32, 8, 128, 128), BF16, False),
+                                                    ((3001, 20, 4, 80, 32), F32, True),
+                                                    ((2999, 9, 3, 64, 64), F16, False)], ids=str)
+def test_many_tokens_equal_few(size, dtype, interleaved):
+    """Large calls give a warp more rows; every row comes out the same."""
+    from b200attn import qk_norm_rope_b200, rope_kv_append_b200
+
+    t, hq, hkv, d, rot = size
+    q, k, v, qw, kw, pos, table = _inputs(*size, dtype, 31)
+    qo, ko = qk_norm_rope_b200(q, k, pos, table, q_weight=qw, k_weight=kw, interleaved=interleaved)
+    assert_close(qo, norm_rope(q, pos, table, qw, EPS, interleaved), dtype, rot, interleaved, "q")
+    assert_close(ko, norm_rope(k, pos, table, kw, EPS, interleaved), dtype, rot, interleaved, "k")
+    pool = _pool(1, -(-t // 16), 16, hkv, d, F32, 95)
+    slots = torch.randperm(t, generator=torch.Generator().manual_seed(6)).to(DEV)
+    qa = rope_kv_append_b200(q, k, v, pool, slots, pos, table, 0, q_weight=qw, k_weight=kw,
+                             interleaved=interleaved)
+    assert torch.equal(qa, qo)
+    at = (0, slots // 16, slots % 16)
+    assert torch.equal(pool.k[at].to(dtype), ko) and torch.equal(pool.v[at], v.float())
+    for lo in (0, 500, t - 7):
+        one = slice(lo, lo + 7)
+        q7, k7 = qk_norm_rope_b200(q[one], k[one], pos[one], table, q_weight=qw, k_weight=kw,
+                                   interleaved=interleaved)
+        assert torch.equal(q7, qo[one]) and torch.equal(k7, ko[one])
+
+
 def test_zero_rows_infinities_and_far_positions():
     from b200attn import qk_norm_rope_b200, rope_table
 
