@@ -47,8 +47,8 @@ struct ElemSmem {
   static constexpr int LD = DP + 4;  // row pitch: float4 reads of 8 rows spread over the banks
   static constexpr int Q = 0, K = Q + R * LD, V = K + kKeys * LD, P = V + kKeys * LD;
   static constexpr int LP = kKeys + 1;
-  static constexpr int FLOATS = P + R * LP;
-  static constexpr int BYTES = FLOATS * 4;
+  static constexpr int ROWS = P + R * LP;  // int [2][kKeys]: pool rows of the next tiles' keys
+  static constexpr int BYTES = (ROWS + 2 * kKeys) * 4;
 };
 
 // One part: R rows (row i of the tile is query row row0 + i of key head g,
@@ -89,29 +89,55 @@ struct ElemAttend {
     }
     const KV* kp = static_cast<const KV*>(p.k_pool);
     const KV* vp = static_cast<const KV*>(p.v_pool);
-    constexpr int E = 16 / sizeof(KV);  // elements per 16-byte chunk
-    constexpr int CH = DP / E;          // chunks per row
-
-    for (int64_t key0 = k0; key0 < k1; key0 += kKeys) {
-      __syncthreads();  // the tile before is done with K and V (and Q is there)
-      for (int i = tid; i < kKeys * CH; i += 128) {
-        const int r = i / CH, d0 = (i % CH) * E;
-        const int64_t key = key0 + r;
-        float fk[E], fv[E];
+    constexpr int E = 16 / sizeof(KV);     // elements per 16-byte chunk
+    constexpr int CH = DP / E;             // chunks per row
+    constexpr int IT = kKeys * CH / 128;   // chunks of K (and of V) per thread and tile
+    static_assert(kKeys * CH % 128 == 0, "whole chunks per thread");
+    int* rows = reinterpret_cast<int*>(sm + L::ROWS);
+    // Loads run ahead of the arithmetic: a tile's chunks wait in registers
+    // while the tile before it is worked on, and the first warp looks its
+    // keys' pool rows up one tile earlier still (-1: past the end).
+    auto lookup = [&](int64_t key0) -> int {
+      const int64_t key = key0 + tid;
+      if (key >= k1) return -1;
+      const int64_t page = key >> p.s_shift;
+      int64_t phys = page < tlen ? load_index(table, page * tstride, ti64) : -1;
+      if (phys < 0 || phys >= p.P) {
+        report(p.status, B200_DEV_BAD_BLOCK);
+        phys = 0;  // an in-bounds page; the status word tells
+      }
+      return static_cast<int>(p.layer_row0 + phys * p.S + (key & (p.S - 1)));
+    };
+    uint4 ck[IT], cv[IT];
+    auto fetch = [&](const int* tile_rows) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) fk[e] = fv[e] = 0.f;  // keys past the end, columns past D
-        if (key < k1 && d0 < p.D) {
-          const int64_t page = key >> p.s_shift;
-          int64_t phys = page < tlen ? load_index(table, page * tstride, ti64) : -1;
-          if (phys < 0 || phys >= p.P) {
-            report(p.status, B200_DEV_BAD_BLOCK);
-            phys = 0;  // an in-bounds page; the status word tells
-          }
-          const int64_t at =
-              ((p.layer_row0 + phys * p.S + (key & (p.S - 1))) * p.Hkv + g) * p.D + d0;
-          Elem<KV>::unpack(*reinterpret_cast<const uint4*>(kp + at), fk);
-          Elem<KV>::unpack(*reinterpret_cast<const uint4*>(vp + at), fv);
+      for (int i = 0; i < IT; ++i) {
+        const int at = tid + 128 * i, r = at / CH, d0 = (at % CH) * E;
+        const int row = tile_rows[r];
+        ck[i] = cv[i] = make_uint4(0, 0, 0, 0);  // keys past the end, columns past D
+        if (row >= 0 && d0 < p.D) {
+          const int64_t off = (static_cast<int64_t>(row) * p.Hkv + g) * p.D + d0;
+          ck[i] = __ldg(reinterpret_cast<const uint4*>(kp + off));
+          cv[i] = __ldg(reinterpret_cast<const uint4*>(vp + off));
         }
+      }
+    };
+    if (tid < kKeys) {
+      rows[tid] = lookup(k0);
+      rows[kKeys + tid] = lookup(k0 + kKeys);
+    }
+    __syncthreads();
+    fetch(rows);
+
+    int buf = 0;
+    for (int64_t key0 = k0; key0 < k1; key0 += kKeys, buf ^= 1) {
+      __syncthreads();  // the tile before is done with K and V
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int at = tid + 128 * i, r = at / CH, d0 = (at % CH) * E;
+        float fk[E], fv[E];
+        Elem<KV>::unpack(ck[i], fk);
+        Elem<KV>::unpack(cv[i], fv);
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
           *reinterpret_cast<float4*>(K + r * L::LD + d0 + e) =
@@ -120,6 +146,8 @@ struct ElemAttend {
               make_float4(fv[e], fv[e + 1], fv[e + 2], fv[e + 3]);
         }
       }
+      if (key0 + kKeys < k1) fetch(rows + (buf ^ 1) * kKeys);
+      const int ahead = tid < kKeys ? lookup(key0 + 2 * kKeys) : -1;
       __syncthreads();
       // Scores: rows tr * RT + i, keys tc + TC * j.
       float2 s2[RT][KPT];
@@ -198,6 +226,7 @@ struct ElemAttend {
           }
         }
       }
+      if (tid < kKeys) rows[buf * kKeys + tid] = ahead;
     }
   }
 
@@ -224,9 +253,14 @@ struct ElemAttend {
 
 // Prefix: CTA (part, row tile, key head).
 template <typename KV, int R, int DP>
-__global__ void __launch_bounds__(128) shared_prefix_elem_kernel(const __grid_constant__ SharedParams p) {
+__global__ void __launch_bounds__(128) shared_prefix_elem_kernel(const __grid_constant__ SharedParams p,
+                                                                const int counters) {
+  let_next_start();
   extern __shared__ float4 sm4[];
   float* sm = reinterpret_cast<float*>(sm4);
+  const int64_t cta = blockIdx.x + static_cast<int64_t>(gridDim.x) * (blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z);
+  for (int64_t i = cta * 128 + threadIdx.x; i < counters; i += static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z * 128)
+    p.cnt[i] = 0;  // of the own-key kernel
   const int part = blockIdx.x, row0 = blockIdx.y * R, g = blockIdx.z;
   const int64_t k0 = static_cast<int64_t>(part) * p.prefix_per;
   const int64_t k1 = min(p.prefix, k0 + p.prefix_per);
@@ -273,6 +307,7 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
         static_cast<const char*>(p.tables) + b * p.ts0 * row_bytes, p.ts1, p.tables_i64,
         p.table_width);
   a.write(p, g, row0, nrows, p.np + split);
+  wait_for_previous();  // for the counters and the prefix's parts
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) last = atomicAdd(&p.cnt[unit], 1) == parts - 1;
@@ -280,7 +315,7 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
   if (!last) return;
   __threadfence();
   for (int r = threadIdx.x >> 5; r < nrows; r += 4)
-    join_row(p, g, row0 + r, parts, threadIdx.x & 31, 32);
+    join_row(p, g, row0 + r, parts);
 }
 
 // ------------------------------------------------------------------ host
@@ -345,7 +380,8 @@ int allow_smem(Kernel kern, int bytes, int device, std::atomic<int>* state) {
 }
 
 template <typename KV, int DP>
-int launch_prefix_elem(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
+int launch_prefix_elem(const SharedParams& p, const SharedPlan& pl, int counters, int device,
+                       cudaStream_t stream) {
   const int64_t tiles = ceil_div(p.rows, 64);
   if (tiles > 65535) return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
   auto kern = shared_prefix_elem_kernel<KV, 64, DP>;
@@ -354,36 +390,35 @@ int launch_prefix_elem(const SharedParams& p, const SharedPlan& pl, int device, 
   if (rc != B200_OK) return rc;
   const dim3 grid(static_cast<unsigned>(pl.np), static_cast<unsigned>(tiles),
                   static_cast<unsigned>(p.Hkv));
-  kern<<<grid, 128, ElemSmem<64, DP>::BYTES, stream>>>(p);
+  kern<<<grid, 128, ElemSmem<64, DP>::BYTES, stream>>>(p, counters);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix launch");
 }
 
 template <typename KV, int DP>
-int launch_own_elem(const SharedParams& p, int device, cudaStream_t stream) {
+int launch_own_elem(const SharedParams& p, bool overlap, int device, cudaStream_t stream) {
   const int64_t grid = static_cast<int64_t>(p.B) * p.Hkv * p.row_chunks * p.own_splits;
   if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
   auto kern = shared_own_elem_kernel<KV, DP>;
   static std::atomic<int> state[64];
   int rc = allow_smem(kern, ElemSmem<8, DP>::BYTES, device, state);
   if (rc != B200_OK) return rc;
-  kern<<<static_cast<unsigned>(grid), 128, ElemSmem<8, DP>::BYTES, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
+  return launch_own(kern, grid, 128, ElemSmem<8, DP>::BYTES, stream, overlap, p);
 }
 
 template <typename KV>
-int launch_prefix_elem_d(const SharedParams& p, const SharedPlan& pl, int device, cudaStream_t stream) {
-  if (p.D <= 32) return launch_prefix_elem<KV, 32>(p, pl, device, stream);
-  if (p.D <= 64) return launch_prefix_elem<KV, 64>(p, pl, device, stream);
-  return launch_prefix_elem<KV, 128>(p, pl, device, stream);
+int launch_prefix_elem_d(const SharedParams& p, const SharedPlan& pl, int counters, int device,
+                         cudaStream_t stream) {
+  if (p.D <= 32) return launch_prefix_elem<KV, 32>(p, pl, counters, device, stream);
+  if (p.D <= 64) return launch_prefix_elem<KV, 64>(p, pl, counters, device, stream);
+  return launch_prefix_elem<KV, 128>(p, pl, counters, device, stream);
 }
 
 template <typename KV>
-int launch_own_elem_d(const SharedParams& p, int device, cudaStream_t stream) {
-  if (p.D <= 32) return launch_own_elem<KV, 32>(p, device, stream);
-  if (p.D <= 64) return launch_own_elem<KV, 64>(p, device, stream);
-  return launch_own_elem<KV, 128>(p, device, stream);
+int launch_own_elem_d(const SharedParams& p, bool overlap, int device, cudaStream_t stream) {
+  if (p.D <= 32) return launch_own_elem<KV, 32>(p, overlap, device, stream);
+  if (p.D <= 64) return launch_own_elem<KV, 64>(p, overlap, device, stream);
+  return launch_own_elem<KV, 128>(p, overlap, device, stream);
 }
 
 }  // namespace
@@ -453,25 +488,24 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   p.q_dtype = a.q_dtype;
   p.out_dtype = a.out_dtype;
   p.qscale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(D)));
-  // The parts of a sequence's own keys count themselves; the tensor-core
-  // kernel clears the counters on its way.
+  // The parts of a sequence's own keys count themselves; the prefix's kernel,
+  // where there is one, clears the counters on its way.
   const int counters = pl.mma && pl.own_splits == 1 ? 0 : static_cast<int>(pl.cnt_bytes / sizeof(int32_t));
-  if (counters > 0 && !pl.tc) {
+  if (counters > 0 && pl.np == 0) {
     cudaError_t e = cudaMemsetAsync(p.cnt, 0, pl.cnt_bytes, stream);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(shared prefix counters)");
   }
   const bool f32 = a.pool.dtype == B200_DTYPE_F32;
-  if (pl.tc) {
+  if (pl.tc)
     rc = launch_shared_prefix_tc(p, a.pool, pl.split, counters, stream);
-    if (rc != B200_OK) return rc;
-  } else if (pl.np > 0) {
-    rc = f32 ? launch_prefix_elem_d<float>(p, pl, dev.device, stream)
-             : launch_prefix_elem_d<__nv_bfloat16>(p, pl, dev.device, stream);
-    if (rc != B200_OK) return rc;
-  }
-  if (pl.mma) return launch_shared_own_mma(p, a.pool, pl.tc, stream);
-  return f32 ? launch_own_elem_d<float>(p, dev.device, stream)
-             : launch_own_elem_d<__nv_bfloat16>(p, dev.device, stream);
+  else if (pl.np > 0)
+    rc = f32 ? launch_prefix_elem_d<float>(p, pl, counters, dev.device, stream)
+             : launch_prefix_elem_d<__nv_bfloat16>(p, pl, counters, dev.device, stream);
+  if (rc != B200_OK) return rc;
+  const bool overlap = pl.np > 0;
+  if (pl.mma) return launch_shared_own_mma(p, a.pool, overlap, stream);
+  return f32 ? launch_own_elem_d<float>(p, overlap, dev.device, stream)
+             : launch_own_elem_d<__nv_bfloat16>(p, overlap, dev.device, stream);
 }
 
 }  // namespace b200

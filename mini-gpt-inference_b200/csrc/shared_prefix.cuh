@@ -4,6 +4,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "host_util.h"
 #include "kernels.h"
 
 namespace b200 {
@@ -82,30 +83,81 @@ __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int s
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The joined row (g, R): element d of sum_s 2^(m_s - M) acc_s / sum_s
-// 2^(m_s - M) l_s over the prefix's slots and the first `parts` own ones,
-// for the elements of this thread (d = t, t + nt, ...).
-__device__ __forceinline__ void join_row(const SharedParams& p, int g, int R, int parts, int t,
-                                         int nt) {
+// Launches an own-key kernel, with leave to begin before the kernel ahead of it
+// has ended where that is the prefix's.
+template <typename... Params, typename... Args>
+int launch_own(void (*kern)(Params...), int64_t grid, int block, int smem, cudaStream_t stream, bool overlap,
+               const Args&... args) {
+  if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(block));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
+}
+
+// The joined row (g, R), by one warp: sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s -
+// M) l_s over the prefix's slots and the first `parts` own ones (at most 96 in
+// all).  A lane holds the factors of every 32nd part and four elements of the
+// row; eight parts' loads are on their way together.
+__device__ __forceinline__ void join_row(const SharedParams& p, int g, int R, int parts) {
+  constexpr int kHeld = 3;
+  const int lane = threadIdx.x & 31;
   const int64_t slot0 = (static_cast<int64_t>(g) * p.rows + R) * p.ns;
   const int n = p.np + parts;
-  float M = -INFINITY;
-  for (int s = 0; s < n; ++s) M = fmaxf(M, __ldcg(&p.ml[(slot0 + s) * 2]));
-  float L = 0.f;
-  for (int s = 0; s < n; ++s) {
-    const float m = __ldcg(&p.ml[(slot0 + s) * 2]);
-    if (m != -INFINITY) L = fmaf(exp2f(m - M), __ldcg(&p.ml[(slot0 + s) * 2 + 1]), L);
+  const float2* ml = reinterpret_cast<const float2*>(p.ml) + slot0;
+  float2 v[kHeld];
+  float M = -INFINITY, sum = 0.f, f[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    v[i] = lane + 32 * i < n ? __ldcg(ml + lane + 32 * i) : make_float2(-INFINITY, 0.f);
+    M = fmaxf(M, v[i].x);
   }
-  const float inv = 1.0f / L;
-  const int b = R / p.rep, h = g * p.rep + R % p.rep;
-  for (int d = t; d < p.D; d += nt) {
-    float o = 0.f;
-    for (int s = 0; s < n; ++s) {
-      const float m = __ldcg(&p.ml[(slot0 + s) * 2]);
-      if (m != -INFINITY) o = fmaf(exp2f(m - M), __ldcg(&p.acc[(slot0 + s) * p.D + d]), o);
+#pragma unroll
+  for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    // A part without a weight (no key, or a slot that stays unused) has no factor.
+    f[i] = v[i].x == -INFINITY ? (v[i].y == 0.f ? 0.f : 1.f) : exp2f(v[i].x - M);
+    sum = fmaf(f[i], v[i].y, sum);
+  }
+#pragma unroll
+  for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+  const float inv = 1.0f / sum;
+  const bool mine = lane * 4 < p.D;
+  const float* acc = p.acc + slot0 * p.D + lane * 4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j0 = 0; j0 < n; j0 += 8) {
+    float4 x[8];
+    float fj[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = j0 + k;
+      fj[k] = __shfl_sync(0xffffffffu, j < 32 ? f[0] : j < 64 ? f[1] : f[2], j & 31) * inv;
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (j < n && fj[k] != 0.f && mine)
+        x[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(j) * p.D));
     }
-    store_elem(p.out, b * p.os0 + h * p.os1 + d * p.os2, p.out_dtype, o * inv);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      a.x = fmaf(fj[k], x[k].x, a.x), a.y = fmaf(fj[k], x[k].y, a.y);
+      a.z = fmaf(fj[k], x[k].z, a.z), a.w = fmaf(fj[k], x[k].w, a.w);
+    }
   }
+  if (!mine) return;
+  const int b = R / p.rep, h = g * p.rep + R % p.rep;
+  const int64_t at = b * p.os0 + h * p.os1 + lane * 4 * p.os2;
+  store_elem(p.out, at, p.out_dtype, a.x);
+  store_elem(p.out, at + p.os2, p.out_dtype, a.y);
+  store_elem(p.out, at + 2 * p.os2, p.out_dtype, a.z);
+  store_elem(p.out, at + 3 * p.os2, p.out_dtype, a.w);
 }
 
 }  // namespace b200

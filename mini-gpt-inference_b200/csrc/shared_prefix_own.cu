@@ -444,7 +444,6 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
            cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(p.B) * p.own_splits * p.row_chunks * p.Hkv;
-  if (grid > 0x7fffffffLL) return fail(B200_ERR_UNSUPPORTED, "shared prefix: grid too large");
   if (p.np + p.own_splits + kWarps > kMaxSlots)
     return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
   const int smem = OwnSmem<DP, NQ>::BYTES + 1024;
@@ -467,18 +466,7 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
     if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = overlap ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tk, tv, op);
-  return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
+  return launch_own(kern, grid, kWarps * 32, smem, stream, overlap, tk, tv, op);
 }
 
 bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
