@@ -296,11 +296,15 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
         store_elem(p.out, b * p.os0 + (g * p.rep + chunk * R + i / p.D) * p.os1 + (i % p.D) * p.os2,
                    p.out_dtype, 0.f);
     }
+    end_after_previous();
     return;
   }
   int64_t k0, k1;
   const int parts = own_range(p, ctx - p.prefix, split, &k0, &k1);
-  if (split >= parts) return;
+  if (split >= parts) {
+    end_after_previous();
+    return;
+  }
   ElemAttend<KV, R, DP> a;
   const int64_t row_bytes = p.tables_i64 ? 8 : 4;
   a.run(p, sm, g, row0, nrows, p.prefix + k0, p.prefix + k1,

@@ -83,6 +83,13 @@ __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int s
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// For own-key CTAs with nothing to join: what comes after the own-key kernel on
+// the stream may take it that the prefix's kernel has ended too, so that the
+// last CTA, whatever it does, ends after it.
+__device__ __forceinline__ void end_after_previous() {
+  if (blockIdx.x == gridDim.x - 1) wait_for_previous();
+}
+
 // Launches an own-key kernel, with leave to begin before the kernel ahead of it
 // has ended where that is the prefix's.
 template <typename... Params, typename... Args>

@@ -116,8 +116,9 @@ __device__ __forceinline__ uint32_t sw128(int r, int ch) {
 }
 
 // What a segment costs besides its tiles (queries in, rows out, the first
-// scores), in tiles: 9 us against 2.2 us a tile.
-constexpr int kSegment = 4;
+// scores), in tiles: 11 us against 1.9 us a tile.  (64 sequences over 32k: 47.9
+// us at 4, 45.5 us at 6; 256 over 16k the same.)
+constexpr int kSegment = 6;
 
 // Runs of equal cost: a unit's tiles, then the segment's cost, is a stretch of
 // unit_tiles + kSegment; the stretches, end to end, are cut evenly.
@@ -249,11 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* merge_full = o_full + 2;
   uint64_t* merge_done = merge_full + 1;
   uint64_t* drained = merge_done + 1;                           // [2]
-  uint64_t* turn = drained + 2;                                 // [2 groups][4 warps]
-  uint64_t* idle = turn + 8;
+  uint64_t* idle = drained + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(idle + 2);
-  static_assert((2 * NS + 23) * 8 <= 512, "barrier area too small");
+  static_assert((2 * NS + 15) * 8 <= 512, "barrier area too small");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   let_next_start();
@@ -268,7 +268,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[w], 4);  // a lane of each warp
       mbar_init(&o_full[w], 1);
       mbar_init(&drained[w], 128);
-      for (int i = 0; i < 4; ++i) mbar_init(&turn[4 * w + i], 1);
     }
     mbar_init(merge_full, 256);
     mbar_init(merge_done, 256);
@@ -447,20 +446,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + w * 128 + lanes, to = tmem + 256 + w * 128 + lanes;
     const float scale = s.qscale;
-    // The groups take turns at the exponential unit, which their warps share
-    // pairwise: left to themselves they drift into using it side by side,
-    // each at half the speed, and then wait for the products side by side.
-    uint64_t* my_turn = &turn[4 * w + (warp & 3)];
-    uint64_t* their_turn = &turn[4 * (w ^ 1) + (warp & 3)];
-    uint32_t turns = 0;
-    auto take_turn = [&]() -> bool {  // group 0 begins
-      const uint32_t before = w == 0 ? turns++ : ++turns;  // turns of the other group to await
-      return before == 0 || mbar_wait(my_turn, (before - 1) & 1u);
-    };
-    auto pass_turn = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(their_turn);
-    };
     uint32_t tiles = 0, oseg = 0, mseg = 0, dseg = 0;
     uint32_t first = 0;
     bool ok = true;
@@ -489,10 +474,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        if (!take_turn()) {
-          ok = false;
-          break;
-        }
         const int left = static_cast<int>(  // keys from here on
             min(s.prefix - static_cast<int64_t>(sg.j0 + jj) * kBN, static_cast<int64_t>(kBN)));
         if (warp_live) {
@@ -560,13 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (fresh || !__any_sync(0xffffffffu, !(add < 65536.f))) break;
           }
-          pass_turn();
 #pragma unroll
           for (int c = 0; c < kBN / 2; c += 16) tmem_st16(ts + c, pk + c);
           l = l * alpha + add;
           tmem_wait_st();
-        } else {
-          pass_turn();
         }
         if (left < kBN && (one || w == 0)) {
           const uint32_t e = first + 2 * jj + 1;
@@ -587,11 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[w]);
-      }
-      // A group with fewer tiles lets its turns pass.
-      for (int k = cnt; ok && k < (one ? (n + 1) / 2 : n); ++k) {
-        ok = take_turn() && *abort_flag == 0;
-        pass_turn();
       }
       if (ok && cnt > 0) {
         ok = mbar_wait(&o_full[w], oseg & 1u) && *abort_flag == 0;

@@ -172,6 +172,45 @@ def test_graph_replays_and_streams_have_their_own_workspaces():
     assert torch.equal(call(), ra) and torch.equal(call(), ra)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_calls_back_to_back_in_one_stream(dtype):
+    """Kernels of a call overlap; calls must not: memory that one call has given
+    back serves the next, also where no row of a call is valid."""
+    a = to_device(case(33, 8, 2, 128, 16, 3000, [i for i in range(33)], dtype, seed=16))
+    b = to_device(case(3, 8, 2, 128, 16, 700, [9, 0, 10], dtype, seed=17))
+    none = to_device(case(33, 8, 2, 128, 16, 3000, [5] * 33, dtype, seed=18))
+    none.lens.fill_(1)
+    want_a, want_b = _run(a), _run(b)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        got.append((_run(a), _run(none), _run(b)))
+    torch.cuda.synchronize()
+    for x, z, y in got:
+        assert torch.equal(x, want_a) and torch.equal(y, want_b) and not z.any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_scores_that_keep_growing(dtype):
+    """Each key's score exceeds the last's: the reference moves again and again."""
+    cpu = case(5, 8, 2, 64, 16, 1500, [3, 0, 40, 100, 7], dtype, seed=19)
+    k = cpu.pool.k.float()
+    at = torch.arange(1500)
+    rows = cpu.table[at // 16]
+    step = (at / 1500 * 60)[:, None, None]
+    q = cpu.q.float()
+    k[0, rows, at % 16] = step * q[0, :2][None] / q[0, :2].square().sum(-1, keepdim=True) * 8
+    cpu.pool.k = k.to(cpu.pool.k.dtype)
+    _check(cpu)
+
+
+def test_a_long_prefix_in_several_runs_to_a_cta():
+    """Two row tiles, units that end inside a CTA's run, a prefix that ends
+    inside a key tile."""
+    _check(case(45, 14, 2, 128, 16, 9001, [i % 20 for i in range(45)], BF16, seed=20))
+    _check(case(9, 8, 8, 64, 32, 20011, [i for i in range(9)], BF16, seed=21))
+
+
 def test_torch_op_matches_direct_call():
     c = to_device(case(3, 4, 2, 64, 16, 70, [10, 20, 1], BF16, seed=13))
     got = torch.ops.b200attn.shared_prefix_decode(c.q, c.pool.k, c.pool.v, c.table, c.prefix,

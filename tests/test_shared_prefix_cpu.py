@@ -23,12 +23,6 @@ def test_plain_form_equals_the_oracle_of_the_paged_decode():
     assert_close(cpu, want.float(), tensor_cores=False)
 
 
-def test_plain_form_of_a_split_prefix():
-    """A prefix that ends inside a page equals the same tokens in pages of one."""
-    cpu = case(2, 4, 2, 16, 8, 13, [4, 9], torch.float64, seed=4)
-    assert torch.isfinite(plain(cpu)[0]).all()
-
-
 def _args(**kw):
     from b200attn import _lib
 
