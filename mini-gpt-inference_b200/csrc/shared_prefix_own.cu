@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kWarps * 32)
     const bool edge = key < lo || key + kStep > hi;
     const bool in0 = !edge || (key + gq >= lo && key + gq < hi);
     const bool in1 = !edge || (key + gq + 8 >= lo && key + gq + 8 < hi);
-    uint32_t pb[NQ][2];
+    uint32_t pb[NQ][2], pl[NQ][2];  // the weights in bf16, and what that left
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
       float x[4];
@@ -293,9 +293,14 @@ __global__ void __launch_bounds__(kWarps * 32)
       const float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
       l[c][0] += p0 + p2;
       l[c][1] += p1 + p3;
-      // The weights are rounded to bf16 for the product alone; l keeps them whole.
-      pb[c][0] = transpose8x8(pack_bf16(p0, p1));
-      pb[c][1] = transpose8x8(pack_bf16(p2, p3));
+      // The weights take part in bf16, what that rounding leaves as a second
+      // product: there is time for it.
+      const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
+      const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
+      pb[c][0] = transpose8x8(h0);
+      pb[c][1] = transpose8x8(h1);
+      pl[c][0] = transpose8x8(pack_bf16(p0 - f0.x, p1 - f0.y));
+      pl[c][1] = transpose8x8(pack_bf16(p2 - f1.x, p3 - f1.y));
     }
     // V rows of masked keys may hold anything, and 0 * NaN is NaN.
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -314,7 +319,10 @@ __global__ void __launch_bounds__(kWarps * 32)
       a[2] &= keep1;
       a[3] &= keep1;
 #pragma unroll
-      for (int c = 0; c < NQ; ++c) mma16816(o[c][i], a, pb[c][0], pb[c][1]);
+      for (int c = 0; c < NQ; ++c) {
+        mma16816(o[c][i], a, pb[c][0], pb[c][1]);
+        mma16816(o[c][i], a, pl[c][0], pl[c][1]);
+      }
     }
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue(issued++);

@@ -23,6 +23,11 @@
 // P V.  With at most 128 rows there is one row tile and the two softmax groups
 // take its key tiles in turn, each with its own O; group 0 adds them up.
 //
+// The weights are rounded to bf16 for P V.  Two row tiles are bound by the
+// products and leave it at that; one row tile is bound by the bytes, and what
+// the rounding left takes part as a second bf16 product (rows then differ from
+// exact ones by their own rounding alone).
+//
 // TMEM (512 columns): S_w / P_w at 128 w, O_w at 256 + 128 w.
 // V rows behind the prefix are cleared in shared memory before they are
 // used: unwritten pool rows can hold NaN, and 0 * NaN is NaN.
@@ -31,7 +36,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 
 #include "common.cuh"
 #include "host_util.h"
@@ -50,7 +54,6 @@ struct TcParams {
   int64_t units;
   int32_t unit_tiles;  // key tiles per unit
   int32_t unit_pairs;  // units per key head
-  int32_t one_tile;    // at most 128 rows per key head
   int32_t rbox, rb_shift;
   int32_t q_vec;
   int32_t zero_count;  // counters to clear for the own-key kernel
@@ -86,17 +89,23 @@ __device__ __forceinline__ void wait_ld32(float* v) {
 }
 
 // Weights 2^(v scale - ref) of 32 scores as bf16 pairs; returns their sum
-// before the rounding.
-__device__ __forceinline__ float weights32(const float* v, float scale, float ref, uint32_t* pk) {
+// before the rounding.  LO: also what the rounding left, as bf16 pairs.
+template <bool LO>
+__device__ __forceinline__ float weights32(const float* v, float scale, float ref, uint32_t* pk, uint32_t* lo) {
   const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-ref, -ref), one2 = make_float2(1.f, 1.f);
   float2 q[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) q[e] = ffma2(make_float2(v[2 * e], v[2 * e + 1]), sc2, nm2);
 #pragma unroll
   for (int e = 0; e < 16; ++e) q[e] = make_float2(ex2(q[e].x), ex2(q[e].y));
-  // bf16 for the product alone; the sum keeps the weights whole.
 #pragma unroll
-  for (int e = 0; e < 16; ++e) pk[e] = pack_bf16(q[e].x, q[e].y);
+  for (int e = 0; e < 16; ++e) {
+    pk[e] = pack_bf16(q[e].x, q[e].y);
+    if constexpr (LO) {
+      const float2 hi = bf16x2_to_float2(pk[e]);
+      lo[e] = pack_bf16(q[e].x - hi.x, q[e].y - hi.y);
+    }
+  }
 #pragma unroll
   for (int w = 8; w >= 1; w >>= 1)
 #pragma unroll
@@ -232,7 +241,8 @@ struct RowWriter {
   }
 };
 
-template <int DP>
+// ONE: at most 128 rows per key head.
+template <int DP, bool ONE>
 __global__ void __launch_bounds__(kThreads, 1)
     shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmk,
                             const __grid_constant__ CUtensorMap tmv, const __grid_constant__ TcParams p) {
@@ -286,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const bool one = p.one_tile != 0;
+  constexpr bool one = ONE;
   auto unit_rows = [&](int unit) { return (unit % p.unit_pairs) * 2 * kBM; };  // its first row
   auto give_up = [&]() {
     report(s.status, B200_DEV_WAIT_TIMEOUT);
@@ -400,11 +410,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
               (w ? np1 : np0) += 1;
               tc_fence_after();
-              uint64_t dv = dv0 + static_cast<uint64_t>((ev % NS) * (L::TILE >> 4));
               uint32_t tp = tmem + w * 128;
+#pragma unroll 1
+              for (int part = 0; part < (one ? 2 : 1); ++part) {
+                uint64_t dv = dv0 + static_cast<uint64_t>((ev % NS) * (L::TILE >> 4));
 #pragma unroll 8
-              for (int kk = 0; kk < kBN / 16; ++kk, dv += 128, tp += 8)
-                mma_bf16_ts(tmem + 256 + w * 128, tp, dv, idesc_o, t >= lead || kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < kBN / 16; ++kk, dv += 128, tp += 8)
+                  mma_bf16_ts(tmem + 256 + w * 128, tp, dv, idesc_o, t >= lead || part + kk > 0 ? 1u : 0u);
+              }
               if (last) mma_commit(&empty[ev % NS]);
               if (t + lead >= n) mma_commit(&o_full[w]);
             }
@@ -495,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
           }
-          uint32_t pk[kBN / 2];
+          uint32_t pk[kBN / 2], lo[ONE ? kBN / 2 : 1];
           float add, alpha = 1.f;
 #pragma unroll 1
           for (bool fresh = k == 0;; fresh = true) {
@@ -537,12 +550,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < kBN; c += 32) {
               wait_ld32(v[(c >> 5) & 1]);
               if (c + 32 < kBN) tmem_ld32(ts + c + 32, v[(c >> 5 & 1) ^ 1]);
-              add += weights32(v[(c >> 5) & 1], scale, ref, pk + (c >> 1));
+              add += weights32<ONE>(v[(c >> 5) & 1], scale, ref, pk + (c >> 1), lo + (ONE ? c >> 1 : 0));
             }
             if (fresh || !__any_sync(0xffffffffu, !(add < 65536.f))) break;
           }
 #pragma unroll
-          for (int c = 0; c < kBN / 2; c += 16) tmem_st16(ts + c, pk + c);
+          for (int c = 0; c < kBN / 2; c += 16) {
+            tmem_st16(ts + c, pk + c);
+            if constexpr (ONE) tmem_st16(ts + kBN / 2 + c, lo + c);
+          }
           l = l * alpha + add;
           tmem_wait_st();
         }
@@ -663,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int DP>
+template <int DP, bool ONE>
 int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const DeviceInfo& dev,
            cudaStream_t stream) {
   const int smem = TcSmem<DP>::BYTES + 1024;
@@ -683,12 +699,12 @@ int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const Device
   if (rc != B200_OK) return rc;
   static std::atomic<int> configured[64];
   if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(shared_prefix_tc_kernel<DP>,
+    cudaError_t e = cudaFuncSetAttribute(shared_prefix_tc_kernel<DP, ONE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
     if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
   }
-  shared_prefix_tc_kernel<DP><<<static_cast<unsigned>(ctas), kThreads, smem, stream>>>(tk, tv, p);
+  shared_prefix_tc_kernel<DP, ONE><<<static_cast<unsigned>(ctas), kThreads, smem, stream>>>(tk, tv, p);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix launch");
 }
@@ -731,13 +747,14 @@ int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, c
   p.units = t.units;
   p.unit_tiles = t.unit_tiles;
   p.unit_pairs = t.unit_pairs;
-  p.one_tile = s.rows <= kBM;
   p.rbox = static_cast<int32_t>(std::min<int64_t>(s.S, kBN));
   p.rb_shift = log2i(p.rbox);
   p.q_vec = s.qs2 == 1 && reinterpret_cast<uintptr_t>(s.q) % 16 == 0 && s.qs0 % 8 == 0 && s.qs1 % 8 == 0;
   p.zero_count = zero_count;
-  if (s.D <= 64) return launch<64>(p, pool, t.ctas, dev, stream);
-  return launch<128>(p, pool, t.ctas, dev, stream);
+  const bool one = s.rows <= kBM;
+  if (s.D <= 64)
+    return one ? launch<64, true>(p, pool, t.ctas, dev, stream) : launch<64, false>(p, pool, t.ctas, dev, stream);
+  return one ? launch<128, true>(p, pool, t.ctas, dev, stream) : launch<128, false>(p, pool, t.ctas, dev, stream);
 }
 
 }  // namespace b200

@@ -93,11 +93,11 @@ def bound(c, want, spread, big, tensor_cores):
     weights, their sum and the outputs are then float32 sums of at most n
     terms: n * 2^-24 each in the worst order; both numerator and denominator
     carry it.  On tensor cores the weights are rounded to bf16 for the product
-    with v: half a step, 2^-8 relative (the sum keeps them whole)."""
+    with v: half a step, 2^-8 relative (the sum keeps them whole).  "split": what
+    that leaves, at most 2^-8, is rounded to bf16 too and takes part: 2^-16."""
     n = float(c.lens.max())
     rel = 2 * (132 * 2.0 ** -24 * big + 2.0 ** -22 + n * 2.0 ** -24)
-    if tensor_cores:
-        rel = rel + 2.0 ** -8
+    rel = rel + {False: 0.0, True: 2.0 ** -8, "split": 2.0 ** -16}[tensor_cores]
     half = torch.finfo(c.q.dtype).eps / 2
     tiny = 2.0 ** -25 if c.q.dtype == torch.float16 else 1e-30
     return rel[..., None] * spread * (1 + half) + half * want.abs() + tiny

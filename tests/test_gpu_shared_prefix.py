@@ -204,6 +204,14 @@ def test_scores_that_keep_growing(dtype):
     _check(cpu)
 
 
+@pytest.mark.parametrize("size", [(1, 1, 1, 64, 16, 300, [9]), (4, 32, 8, 128, 16, 2048, [1, 64, 17, 33]),
+                                  (64, 4, 2, 80, 32, 500, [i for i in range(64)]),
+                                  (3, 40, 4, 96, 16, 1000, [0, 200, 31])], ids=str)
+def test_few_rows_differ_by_their_own_rounding_alone(size):
+    """At most 128 rows to a key head: what the weights' rounding leaves takes part."""
+    _check(case(*size, BF16, seed=22), tensor_cores="split")
+
+
 def test_a_long_prefix_in_several_runs_to_a_cta():
     """Two row tiles, units that end inside a CTA's run, a prefix that ends
     inside a key tile."""
