@@ -32,6 +32,15 @@
 // V rows behind the prefix are cleared in shared memory before they are
 // used: unwritten pool rows can hold NaN, and 0 * NaN is NaN.
 // Every wait is bounded; after one runs out all roles leave.
+//
+// Measured (32 query heads of 128 over 8 key heads): 256 sequences over 16384
+// keys 73 us, of which 53 us are 28 tile pairs of 1.9 us a CTA (the products
+// alone, at this GPU's rate for them, 1.4 us) and the rest the segments'
+// beginnings and ends; 64 over 32768 45 us (21 us at the copy rate).  A softmax
+// of two threads to a row (16 warps), of rows whose weights go to the products
+// quarter by quarter, of weights by polynomial on the FMA pipes, and turns of
+// the two groups at the exponential unit were all built and measured: 2 to 2.6
+// us a tile pair.
 #include <math.h>
 
 #include <algorithm>
@@ -166,7 +175,7 @@ struct Segments {
 // The 32 query rows from row0 on of key head g (zeros from `rows` on) into
 // rows r0 .. r0 + 31 of a swizzled tile, by one warp: whole rows by neighbouring
 // lanes, all loads on their way before the first store.  (A row per lane, 32
-// lines to a load, took 7 us for a tile; this takes <q>.)
+// lines to a load, took 7 us for both tiles; this takes 3.)
 template <int DP>
 __device__ __forceinline__ void load_q_rows(uint8_t* tile, int r0, const SharedParams& s, int row0, int g,
                                             int q_vec) {
@@ -209,7 +218,7 @@ __device__ __forceinline__ void load_q_rows(uint8_t* tile, int r0, const SharedP
 // `pitch` floats through shared memory (32 x W floats, 16-byte chunks permuted
 // by row so that neither side meets a bank twice): W / 4 neighbouring lanes
 // write consecutive bytes of a row.  (16 bytes a lane, straight from the
-// lane's row, took 9 us for a tile; this takes <w>.)
+// lane's row, took 9 us for both tiles; this takes 4.)
 template <int W>
 struct RowWriter {
   static constexpr int CH = W / 4;
@@ -306,151 +315,151 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Registers: 384 threads start with 168 each (64512 in all); 128 x 56 +
   // 256 x 224 is the same sum.  A softmax thread works on a row of 128 scores.
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    const int box_bytes = 64 * p.rbox * 2;
-    const int boxes_per_tile = kBN / p.rbox;  // <= 16
-    const int64_t table_len = (s.prefix + s.S - 1) >> s.s_shift;
-    uint32_t it = 0;
-    bool ok = true;
-    Segments sg(p);
-    while (ok && sg.next()) {
-      const int g = sg.unit / p.unit_pairs;
-      // Lane i looks up block i of a tile (16 at most), one tile ahead.
-      auto blocks = [&](int j) {
-        return static_cast<int>(min(static_cast<int64_t>(boxes_per_tile),
-                                    (s.prefix - static_cast<int64_t>(j) * kBN + p.rbox - 1) >> p.rb_shift));
-      };
-      auto entry = [&](int j) -> int64_t {
-        if (j >= sg.j0 + sg.n || lane >= blocks(j)) return 0;
-        const int64_t page = (static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift)) >> s.s_shift;
-        return page < table_len ? load_index(s.prefix_table, page * s.pt_stride, s.pt_i64) : -1;
-      };
-      int64_t next = entry(sg.j0);
-      for (int j = sg.j0; ok && j < sg.j0 + sg.n; ++j) {
-        const int nb = blocks(j);
-        int64_t phys = next;
-        next = entry(j + 1);
-        if (lane < nb && (phys < 0 || phys >= s.P)) {
-          report(s.status, B200_DEV_BAD_BLOCK);
-          phys = 0;  // an in-bounds page; the status word tells
-        }
-        const int64_t key = static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift);
-        const int row = static_cast<int>(s.layer_row0 + phys * s.S + (key & (s.S - 1)));
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++it) {
-          const int st = static_cast<int>(it % NS);
-          int good = 1;
-          if (lane == 0) good = mbar_wait(&empty[st], ((it / NS) & 1u) ^ 1u) ? 1 : 0;
-          good = __shfl_sync(0xffffffffu, good, 0);
-          if (!good || *abort_flag) {
-            if (!good && lane == 0) give_up();
-            ok = false;
-            break;
-          }
-          if (lane == 0)
-            mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(nb * L::HALVES * box_bytes));
-          __syncwarp();
-          if (lane < nb) {
-            uint8_t* dst = smem + L::RING + st * L::TILE + lane * p.rbox * 128;
-#pragma unroll
-            for (int h = 0; h < L::HALVES; ++h)
-              tma_load_3d(dst + h * L::HALF, kv == 0 ? &tmk : &tmv, &full[st], h * 64, g, row);
-          }
-        }
-      }
-    }
-    // Copies in flight land before the CTA ends.
-    if (lane == 0) {
-      for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i)
-        if (!mbar_wait(&full[i % NS], (i / NS) & 1u)) {
-          give_up();
-          break;
-        }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ products
-    // The whole warp, so that descriptors stay in uniform registers (one lane
-    // issues), in small loops: this code shares its instruction cache with the
-    // softmax warps, and a step that has to be fetched again is late.
-    {
-      constexpr uint32_t idesc_s = idesc_bf16(128, kBN, false);
-      constexpr uint32_t idesc_o = idesc_bf16(128, DP, true);
-      const uint64_t dq0 = smem_desc_sw128(smem_u32(smem + L::Q0), 16, 1024);
-      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::RING), 16, 1024);
-      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::RING), L::HALF, 1024);
-      uint32_t first = 0;         // ring entry of the segment's first K
-      uint32_t np0 = 0, np1 = 0;  // P tiles of group w awaited so far
-      uint32_t nq0 = 0, nq1 = 0;  // Q tiles awaited so far
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads
+      const int box_bytes = 64 * p.rbox * 2;
+      const int boxes_per_tile = kBN / p.rbox;  // <= 16
+      const int64_t table_len = (s.prefix + s.S - 1) >> s.s_shift;
+      uint32_t it = 0;
       bool ok = true;
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
-      };
-      auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
       Segments sg(p);
       while (ok && sg.next()) {
-        const int n = sg.n;
-        const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
-        ok = wait_all(&q_full[0], nq0++ & 1u) && (!two || wait_all(&q_full[1], nq1++ & 1u)) &&
-             *abort_flag == 0;
-        // Step t: P V of tile t, then S of tile t + lead for the same group, which
-        // frees the columns in that order.  Two row tiles: both groups, one tile
-        // ahead; one row tile: the groups alternate, two tiles ahead.
-        const int lead = one ? 2 : 1, groups = two ? 2 : 1;
-#pragma unroll 1
-        for (int t = -lead; ok && t < n; ++t) {
-          const uint32_t ev = first + 2 * t + 1, ek = first + 2 * (t + lead);
-#pragma unroll 1
-          for (int i = 0; ok && i < groups; ++i) {
-            const int w = one ? t & 1 : i;
-            const bool last = i == groups - 1;
-            if (t >= 0) {
-              ok = wait_all(&p_full[w], (w ? np1 : np0) & 1u) && (i > 0 || wait_entry(ev));
-              if (!ok) break;
-              (w ? np1 : np0) += 1;
-              tc_fence_after();
-              uint32_t tp = tmem + w * 128;
-#pragma unroll 1
-              for (int part = 0; part < (one ? 2 : 1); ++part) {
-                uint64_t dv = dv0 + static_cast<uint64_t>((ev % NS) * (L::TILE >> 4));
-#pragma unroll 8
-                for (int kk = 0; kk < kBN / 16; ++kk, dv += 128, tp += 8)
-                  mma_bf16_ts(tmem + 256 + w * 128, tp, dv, idesc_o, t >= lead || part + kk > 0 ? 1u : 0u);
-              }
-              if (last) mma_commit(&empty[ev % NS]);
-              if (t + lead >= n) mma_commit(&o_full[w]);
+        const int g = sg.unit / p.unit_pairs;
+        // Lane i looks up block i of a tile (16 at most), one tile ahead.
+        auto blocks = [&](int j) {
+          return static_cast<int>(min(static_cast<int64_t>(boxes_per_tile),
+                                      (s.prefix - static_cast<int64_t>(j) * kBN + p.rbox - 1) >> p.rb_shift));
+        };
+        auto entry = [&](int j) -> int64_t {
+          if (j >= sg.j0 + sg.n || lane >= blocks(j)) return 0;
+          const int64_t page = (static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift)) >> s.s_shift;
+          return page < table_len ? load_index(s.prefix_table, page * s.pt_stride, s.pt_i64) : -1;
+        };
+        int64_t next = entry(sg.j0);
+        for (int j = sg.j0; ok && j < sg.j0 + sg.n; ++j) {
+          const int nb = blocks(j);
+          int64_t phys = next;
+          next = entry(j + 1);
+          if (lane < nb && (phys < 0 || phys >= s.P)) {
+            report(s.status, B200_DEV_BAD_BLOCK);
+            phys = 0;  // an in-bounds page; the status word tells
+          }
+          const int64_t key = static_cast<int64_t>(j) * kBN + (static_cast<int64_t>(lane) << p.rb_shift);
+          const int row = static_cast<int>(s.layer_row0 + phys * s.S + (key & (s.S - 1)));
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++it) {
+            const int st = static_cast<int>(it % NS);
+            int good = 1;
+            if (lane == 0) good = mbar_wait(&empty[st], ((it / NS) & 1u) ^ 1u) ? 1 : 0;
+            good = __shfl_sync(0xffffffffu, good, 0);
+            if (!good || *abort_flag) {
+              if (!good && lane == 0) give_up();
+              ok = false;
+              break;
             }
-            if (t + lead < n) {
-              ok = i > 0 || wait_entry(ek);
-              if (!ok) break;
-              tc_fence_after();
-              uint64_t dq = dq0 + static_cast<uint64_t>(i * (L::TILE >> 4));
-              uint64_t dk = dk0 + static_cast<uint64_t>((ek % NS) * (L::TILE >> 4));
-#pragma unroll 8
-              for (int kk = 0; kk < DP / 16; ++kk) {
-                mma_bf16(tmem + w * 128, dq, dk, idesc_s, kk > 0 ? 1u : 0u);
-                const uint64_t step = kk == 3 ? (L::HALF - 96) >> 4 : 2;  // 16 d on, or the other half
-                dq += step;
-                dk += step;
-              }
-              mma_commit(&s_full[w]);
-              if (last) mma_commit(&empty[ek % NS]);
+            if (lane == 0)
+              mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(nb * L::HALVES * box_bytes));
+            __syncwarp();
+            if (lane < nb) {
+              uint8_t* dst = smem + L::RING + st * L::TILE + lane * p.rbox * 128;
+#pragma unroll
+              for (int h = 0; h < L::HALVES; ++h)
+                tma_load_3d(dst + h * L::HALF, kv == 0 ? &tmk : &tmv, &full[st], h * 64, g, row);
             }
           }
-          ok = ok && *abort_flag == 0;
         }
-        first += 2 * n;
       }
-      if (!ok && lane == 0) give_up();
-      mma_commit(idle);  // every product issued has ended before TMEM is freed
-      if (!wait_all(idle, 0) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
-      __syncwarp();
+      // Copies in flight land before the CTA ends.
+      if (lane == 0) {
+        for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i)
+          if (!mbar_wait(&full[i % NS], (i / NS) & 1u)) {
+            give_up();
+            break;
+          }
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ products
+      // The whole warp, so that descriptors stay in uniform registers (one lane
+      // issues), in small loops: this code shares its instruction cache with the
+      // softmax warps, and a step that has to be fetched again is late.
+      {
+        constexpr uint32_t idesc_s = idesc_bf16(128, kBN, false);
+        constexpr uint32_t idesc_o = idesc_bf16(128, DP, true);
+        const uint64_t dq0 = smem_desc_sw128(smem_u32(smem + L::Q0), 16, 1024);
+        const uint64_t dk0 = smem_desc_sw128(smem_u32(smem + L::RING), 16, 1024);
+        const uint64_t dv0 = smem_desc_sw128(smem_u32(smem + L::RING), L::HALF, 1024);
+        uint32_t first = 0;         // ring entry of the segment's first K
+        uint32_t np0 = 0, np1 = 0;  // P tiles of group w awaited so far
+        uint32_t nq0 = 0, nq1 = 0;  // Q tiles awaited so far
+        bool ok = true;
+        auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+          return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+        };
+        auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
+        Segments sg(p);
+        while (ok && sg.next()) {
+          const int n = sg.n;
+          const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
+          ok = wait_all(&q_full[0], nq0++ & 1u) && (!two || wait_all(&q_full[1], nq1++ & 1u)) &&
+               *abort_flag == 0;
+          // Step t: P V of tile t, then S of tile t + lead for the same group, which
+          // frees the columns in that order.  Two row tiles: both groups, one tile
+          // ahead; one row tile: the groups alternate, two tiles ahead.
+          const int lead = one ? 2 : 1, groups = two ? 2 : 1;
+#pragma unroll 1
+          for (int t = -lead; ok && t < n; ++t) {
+            const uint32_t ev = first + 2 * t + 1, ek = first + 2 * (t + lead);
+#pragma unroll 1
+            for (int i = 0; ok && i < groups; ++i) {
+              const int w = one ? t & 1 : i;
+              const bool last = i == groups - 1;
+              if (t >= 0) {
+                ok = wait_all(&p_full[w], (w ? np1 : np0) & 1u) && (i > 0 || wait_entry(ev));
+                if (!ok) break;
+                (w ? np1 : np0) += 1;
+                tc_fence_after();
+                uint32_t tp = tmem + w * 128;
+#pragma unroll 1
+                for (int part = 0; part < (one ? 2 : 1); ++part) {
+                  uint64_t dv = dv0 + static_cast<uint64_t>((ev % NS) * (L::TILE >> 4));
+#pragma unroll 8
+                  for (int kk = 0; kk < kBN / 16; ++kk, dv += 128, tp += 8)
+                    mma_bf16_ts(tmem + 256 + w * 128, tp, dv, idesc_o, t >= lead || part + kk > 0 ? 1u : 0u);
+                }
+                if (last) mma_commit(&empty[ev % NS]);
+                if (t + lead >= n) mma_commit(&o_full[w]);
+              }
+              if (t + lead < n) {
+                ok = i > 0 || wait_entry(ek);
+                if (!ok) break;
+                tc_fence_after();
+                uint64_t dq = dq0 + static_cast<uint64_t>(i * (L::TILE >> 4));
+                uint64_t dk = dk0 + static_cast<uint64_t>((ek % NS) * (L::TILE >> 4));
+#pragma unroll 8
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                  mma_bf16(tmem + w * 128, dq, dk, idesc_s, kk > 0 ? 1u : 0u);
+                  const uint64_t step = kk == 3 ? (L::HALF - 96) >> 4 : 2;  // 16 d on, or the other half
+                  dq += step;
+                  dk += step;
+                }
+                mma_commit(&s_full[w]);
+                if (last) mma_commit(&empty[ek % NS]);
+              }
+            }
+            ok = ok && *abort_flag == 0;
+          }
+          first += 2 * n;
+        }
+        if (!ok && lane == 0) give_up();
+        mma_commit(idle);  // every product issued has ended before TMEM is freed
+        if (!wait_all(idle, 0) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
+        __syncwarp();
+      }
+    } else {
+      // Counters of the kernel that follows on the stream.
+      for (int i = blockIdx.x * 64 + threadIdx.x - 64; i < p.zero_count; i += gridDim.x * 64) s.cnt[i] = 0;
     }
-  } else {
-    // Counters of the kernel that follows on the stream.
-    for (int i = blockIdx.x * 64 + threadIdx.x - 64; i < p.zero_count; i += gridDim.x * 64) s.cnt[i] = 0;
-  }
   } else {
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
