@@ -66,7 +66,8 @@ enum {
 /* Bits ORed into the optional device status word by the kernels. */
 enum {
   B200_DEV_BAD_BLOCK = 1,    /* block-table entry outside [0, P)           */
-  B200_DEV_BAD_LENGTH = 2,   /* context length < 1 or > M*S                */
+  B200_DEV_BAD_LENGTH = 2,   /* context length < 1 or > M*S (shared prefix:
+                                or shorter than the prefix)               */
   B200_DEV_BAD_SLOT = 4,     /* slot outside [0, P*S)                      */
   B200_DEV_WAIT_TIMEOUT = 8, /* a bounded pipeline wait gave up            */
   B200_DEV_SLOT_MISMATCH = 16, /* fused write: slot is not the slot of the
@@ -370,7 +371,8 @@ typedef struct {
   int64_t table_width;              /* M >= 1 (columns of block_tables)     */
   const void* q;                    /* [B, Hq, D] any strides               */
   int64_t q_stride[3];
-  void* out;                        /* [B, Hq, D] strides                   */
+  void* out;                        /* [B, Hq, D] strides; q itself (same type,
+                                       pointer, strides) or apart from it   */
   int64_t out_stride[3];
   const void* prefix_table;         /* device [>= ceil(prefix_len / S)]     */
   int64_t prefix_table_len;

@@ -156,6 +156,17 @@ def _status_ptr(status, index: int):
     return status.data_ptr()
 
 
+def _index_arg(x, device: torch.device, index: int, name: str) -> torch.Tensor:
+    """An integer tensor of the device, or a host sequence copied there.  A
+    captured copy would read host memory that is gone at the replay, so a
+    graph takes tensors only."""
+    if isinstance(x, torch.Tensor) and x.dtype in _INDEX and x.get_device() == index:
+        return x
+    if not isinstance(x, torch.Tensor) and torch.cuda.is_current_stream_capturing():
+        raise ValueError(f"{name} must be a CUDA tensor while a graph is captured")
+    return _index_tensor(x, device, name)
+
+
 def _pool_fields(pool, index: int, layer_idx: int):
     """The checked fields of _lib.KVPool, and the block size, heads and head
     dimension."""

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch,
+from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_arg, _inference_only, _launch,
                   _pool_fields, _status_ptr)
 
 _PACK_ROPE = _lib.packer(_lib.QkNormRopeArgs).pack
@@ -60,10 +60,15 @@ def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
 
 
 def _check_out(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None:
-    """An output is ``like``'s shape, dtype and device, and either exactly
-    ``like`` itself or apart from every input."""
+    """An output is ``like``'s shape, dtype and device, and see _check_place."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have the shape, dtype and device of its input")
+    _check_place(out, like, name, inputs)
+
+
+def _check_place(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None:
+    """An output writes no element twice, and is either exactly ``like`` or
+    apart from every input."""
     if out.numel() == 0:
         return
     # A permutation of contiguous rows, or rows apart: no element twice.
@@ -73,7 +78,8 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None
             raise ValueError(f"{name} must not overlap itself")
         extent += stride * (n - 1)
     for t in inputs:
-        same = t is like and t.data_ptr() == out.data_ptr() and t.stride() == out.stride()
+        same = (t is like and t.dtype == out.dtype and t.data_ptr() == out.data_ptr()
+                and t.stride() == out.stride())
         if not same and not _apart(out, t):
             raise ValueError(f"{name} must be its input itself or not overlap the inputs")
 
@@ -166,7 +172,7 @@ def qk_norm_rope_b200(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     and k_out k itself.  A token whose position lies outside the table gets
     zero rows and sets DEV_BAD_POSITION in ``status``.
     """
-    _inference_only(q, k, q_weight, k_weight)
+    _inference_only(q, k, cos_sin, q_weight, k_weight)
     lib = _lib.load()
     fields, q_out, k_out, index = _rope_fields(q, k, None, positions, cos_sin, q_weight, k_weight,
                                                eps, interleaved, q_out, k_out, status)
@@ -189,15 +195,15 @@ def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool,
 
     pool[layer, slot // S, slot % S] = normed and rotated k / v as it is, for
     each of the T tokens, rounded once to the pool's dtype (float32 or
-    bfloat16); v: [T, Hkv, D]; slot_mapping: [T] integer CUDA tensor or a host
-    sequence.  Returns the normed and rotated q ([T, Hq, D], in q.dtype).
+    bfloat16); v: [T, Hkv, D]; slot_mapping: [T] integer CUDA tensor or (not
+    while a graph is captured) a host sequence.  Returns the normed and rotated q ([T, Hq, D], in q.dtype).
 
     A slot outside the pool, or a position outside the table, skips that
     token's k and v and sets DEV_BAD_SLOT / DEV_BAD_POSITION in ``status``.
     Slots of one call are distinct, except those that nothing reads (padding
     rows that share a scratch slot).
     """
-    _inference_only(q, k, v, q_weight, k_weight)
+    _inference_only(q, k, v, cos_sin, q_weight, k_weight)
     lib = _lib.load()
     if v.shape != k.shape or v.dtype != k.dtype or v.get_device() != k.get_device():
         raise ValueError("k and v must have matching shape [T,Hkv,D], dtype and device")
@@ -206,9 +212,7 @@ def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool,
     pool_fields = _pool_fields(pool, index, layer_idx)
     if pool_fields[5] != fields[2] or pool_fields[6] != fields[3]:
         raise ValueError("k/v head dimensions do not match the KV pool")
-    slots = slot_mapping
-    if not (isinstance(slots, torch.Tensor) and slots.dtype in _INDEX and slots.get_device() == index):
-        slots = _index_tensor(slots, q.device, "slot_mapping")
+    slots = _index_arg(slot_mapping, q.device, index, "slot_mapping")
     if slots.shape != (fields[0],):
         raise ValueError("slot_mapping must have shape [T]")
     args = _PACK_APPEND(*fields, *pool_fields, layer_idx, v.data_ptr(), *v.stride(),

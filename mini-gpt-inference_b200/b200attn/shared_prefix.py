@@ -11,8 +11,9 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_tensor, _inference_only, _launch,
+from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_arg, _inference_only, _launch,
                   _pool_fields, _status_ptr)
+from .rope import _check_place
 
 _PACK = _lib.packer(_lib.SharedPrefixArgs).pack
 
@@ -26,7 +27,8 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     q: [B, Hq, D] (any strides), Hq a multiple of the pool's heads H (query
     head h reads head h // (Hq // H)); pool.k / pool.v: contiguous
     [L, P, S, H, D], float32 or bfloat16; prefix_table: the blocks of the
-    first ``prefix_len`` positions, 1-D integer CUDA tensor or host ints;
+    first ``prefix_len`` positions, 1-D integer CUDA tensor or (not
+    while a graph is captured) host ints;
     block_tables: [B, M] int32/int64, whose columns from
     ``prefix_len // S`` on hold the sequences' own blocks (earlier entries
     are not read); context_lengths: [B], prefix included.  The new token's K/V
@@ -36,7 +38,8 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     ``prefix_len % S`` of the sequence's own block of that column.
     ``prefix_len`` 0 is a plain paged decode.  A sequence shorter than the
     prefix (a padding row) or longer than its table gets zero rows and sets
-    DEV_BAD_LENGTH in ``status``.  Returns [B, Hq, D] in q.dtype, or fills ``out``.
+    DEV_BAD_LENGTH in ``status``.  Returns [B, Hq, D] in q.dtype, or fills
+    ``out`` (any float dtype; q itself, or apart from it).
     """
     _inference_only(q)
     lib = _lib.load()
@@ -67,9 +70,7 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
         raise ValueError("prefix_len must be >= 0")
     if block_tables.get_device() != index or context_lengths.get_device() != index:
         raise ValueError("all inputs must reside on same CUDA device")
-    table = prefix_table
-    if not (isinstance(table, torch.Tensor) and table.dtype in _INDEX and table.get_device() == index):
-        table = _index_tensor(table, q.device, "prefix_table")
+    table = _index_arg(prefix_table, q.device, index, "prefix_table")
     if table.ndim != 1:
         raise ValueError("prefix_table must be 1-D")
     entries = table.shape[0]
@@ -80,6 +81,8 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
         out = q.new_empty((b, hq, d))
     elif out.shape != (b, hq, d) or out.dtype not in _DTYPES or out.get_device() != index:
         raise ValueError("out must be a [B,Hq,D] tensor on the q device")
+    else:
+        _check_place(out, q, "out", (q,))
     qd = _DTYPES[q.dtype]
     # A workspace of the call's own, from the allocator of the current stream
     # (or of the graph being captured): calls on other streams, and other

@@ -380,10 +380,10 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
 // kernel's own).
 template <typename Kernel>
 int allow_smem(Kernel kern, int bytes, int device, std::atomic<int>* state) {
-  if (bytes <= 48 * 1024 || device >= 64 || state[device].load(std::memory_order_acquire)) return B200_OK;
+  if (bytes <= 48 * 1024 || (device < 64 && state[device].load(std::memory_order_acquire))) return B200_OK;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared prefix)");
-  state[device].store(1, std::memory_order_release);
+  if (device < 64) state[device].store(1, std::memory_order_release);
   return B200_OK;
 }
 

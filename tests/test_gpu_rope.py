@@ -227,6 +227,19 @@ def test_no_tokens_and_host_slots():
     assert torch.equal(pool.v[0, [0, 1, 2, 3], [0, 1, 2, 3]], v)
 
 
+def test_host_slots_are_refused_while_a_graph_is_captured():
+    from b200attn import rope_kv_append_b200
+
+    q, k, v, qw, kw, pos, table = _inputs(4, 4, 2, 64, 64, BF16, 14)
+    pool = _pool(1, 4, 4, 2, 64, BF16, 61)
+    with pytest.raises(ValueError, match="slot_mapping must be a CUDA tensor"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            rope_kv_append_b200(q, k, v, pool, [0, 5, 10, 15], pos, table, 0)
+    torch.cuda.synchronize()
+    rope_kv_append_b200(q, k, v, pool, [0, 5, 10, 15], pos, table, 0)
+    assert torch.equal(pool.v[0, [0, 1, 2, 3], [0, 1, 2, 3]], v)
+
+
 def test_prepared_call_graph_replay_and_other_stream():
     from b200attn import rope_kv_append_b200
 

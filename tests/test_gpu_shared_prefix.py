@@ -286,3 +286,45 @@ def test_decode_steps_of_a_rotary_model_behind_one_prompt(dtype):
         at = (0, slots // block, slots % block)
         assert torch.equal(dev.v[at].cpu(), v)
     assert torch.isfinite(plain(c)[0]).all()
+
+
+@pytest.mark.parametrize("size", [(70, 4, 2, 64, 16, 300, [i % 37 for i in range(70)]),
+                                  (5, 32, 8, 128, 16, 2048, [1, 64, 170, 33, 0])], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_queries_that_are_no_numbers_stay_in_their_rows(size, dtype):
+    cpu = case(*size, dtype, seed=41)
+    c = to_device(cpu)
+    clean = _run(c)
+    odd = torch.zeros(size[:2], dtype=torch.bool, device="cuda")
+    odd[1, 2] = odd[3, 0] = odd[4, 3] = True
+    c.q[1, 2, 5], c.q[3, 0], c.q[4, 3, 7] = float("nan"), float("inf"), float("-inf")
+    out = _run(c)
+    assert out[odd].isnan().all()
+    out[odd] = clean[odd]
+    assert_close(cpu, out, tensor_cores=dtype == BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_out_may_be_q_itself(dtype):
+    cpu = case(6, 16, 2, 128, 16, 700, [600, 3, 0, 40, 1300, 77], dtype, seed=42)
+    c = to_device(cpu)
+    want = _run(c)
+    for _ in range(3):
+        c.q.copy_(cpu.q)
+        assert _run(c, out=c.q).data_ptr() == c.q.data_ptr()
+        assert torch.equal(c.q, want)
+    wide = torch.empty(6, 16, 128, device="cuda")
+    c.q.copy_(cpu.q)
+    assert torch.equal(_run(c, out=wide).to(dtype), want)
+
+
+def test_a_host_list_is_refused_while_a_graph_is_captured():
+    c = to_device(case(2, 4, 2, 64, 16, 70, [10, 20], BF16, seed=43))
+    want = _run(c)
+    tensor, c.table = c.table, c.table.tolist()
+    with pytest.raises(ValueError, match="prefix_table must be a CUDA tensor"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            _run(c)
+    torch.cuda.synchronize()
+    c.table = tensor
+    assert torch.equal(_run(c), want)

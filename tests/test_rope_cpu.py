@@ -142,6 +142,9 @@ def test_python_entries_refuse():
     with pytest.raises(RuntimeError, match="inference"):
         qk_norm_rope_b200(q, k, pos, table, q_weight=torch.ones(32, requires_grad=True))
 
+    with pytest.raises(RuntimeError, match="inference"):
+        qk_norm_rope_b200(q, k, pos, table.clone().requires_grad_())
+
     def refuse(match, q=q, k=k, pos=pos, table=table, **kw):
         with pytest.raises(ValueError, match=match):
             qk_norm_rope_b200(_Cuda(q), k, pos, table, **kw)

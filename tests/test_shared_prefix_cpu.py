@@ -127,6 +127,10 @@ def test_python_entry_refuses():
     refuse("integer", table=cpu.table.float())
     refuse("status", status=torch.zeros(1))
     refuse("out must", out=torch.zeros(3, 8, 16))
+    refuse("overlap itself", out=torch.zeros(1, 1, 32).expand(3, 8, 32))
+    refuse("overlap the inputs", q=(both := torch.zeros(4, 8, 32))[:3], out=both[1:])
+    half = torch.zeros(3, 8, 64, dtype=torch.bfloat16)
+    refuse("overlap the inputs", q=half.view(torch.float32), out=half[..., :32])
     pool = SimpleNamespace(k=cpu.pool.k.half(), v=cpu.pool.v.half(), block_size=16)
     refuse("dtype", pool=pool)
 
