@@ -328,7 +328,9 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
 
 // ------------------------------------------------------------------ host
 struct SharedPlan {
-  bool mma, tc;  // own keys by warp-level products, prefix on tcgen05
+  bool mma;  // own keys by warp-level products,
+  bool few;  // the prefix too
+  bool tc;   // or on tcgen05
   TcSplit split;
   int np, own_splits, own_min, row_chunks;
   int64_t prefix_per;
@@ -346,15 +348,34 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
   // types, and f32 pools, would lose bits there.
   // (Pages of fewer than 8 tokens would make swizzled boxes of less than 1 KB.)
   pl.mma = kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16 && S >= 8;
-  pl.tc = pl.mma && prefix > 0;
-  const bool mma = pl.mma;
   const int64_t rep = Hq / Hkv, rows = B * rep;
+  const bool mma = pl.mma;
+  // Few rows leave most of a tensor tile empty: there the prefix is worked off
+  // eight rows at a time like own keys, which reads it (from L2) once for each
+  // eight.  That starts and ends faster and is up to 16 rows ahead at any length
+  // (4 sequences of 8 x 4 heads over 2048 keys: 10 us against 15; over 32768: 32
+  // against 43; 1 of 32 x 1: 83 against 116).  Above, it is as long as little is
+  // read: 64 rows to each of 8 heads, 1024 keys 13 us against 17, 2048 the same,
+  // 8192 30 against 23.  (16 rows at a time by the wide form of the kernel, whose
+  // longer code has to be fetched first: 12 us where two times eight take 8.)
+  const int64_t eights = ceil_div(rows, 8) * Hkv;
+  pl.few = mma && prefix > 0 && (rows <= 16 || eights * prefix < (int64_t(1) << 17));
+  pl.tc = mma && prefix > 0 && !pl.few;
   // Prefix: parts of whole key tiles that give about two CTAs per SM.
   pl.np = 0;
   pl.prefix_per = 0;
   if (pl.tc) {
     pl.split = shared_tc_split(rows, Hkv, prefix, num_sms);
     pl.np = pl.split.np;
+  } else if (pl.few) {
+    // Two CTAs per SM, three where much is read more than once; at least 64
+    // keys a part, and above 16 parts, which the join has to read, 256 (2048
+    // keys of 8 heads: 16 parts 9.8 us, 8 and 32 parts 10.8).
+    const int per_sm = rows <= 8 || eights * prefix < (int64_t(1) << 18) ? 2 : 3;
+    int64_t parts = std::min({per_sm * num_sms / eights, ceil_div(prefix, 64),
+                              std::max<int64_t>(16, ceil_div(prefix, 256)), int64_t(32)});
+    pl.prefix_per = ceil_div(ceil_div(prefix, std::max<int64_t>(parts, 1)), 16) * 16;
+    pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   } else if (prefix > 0) {
     const int64_t units = ceil_div(rows, 64) * Hkv;
     int64_t parts = std::min<int64_t>(ceil_div(2 * num_sms, units), ceil_div(prefix, 4 * kKeys));
@@ -515,6 +536,8 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
   const bool f32 = a.pool.dtype == B200_DTYPE_F32;
   if (pl.tc)
     rc = launch_shared_prefix_tc(p, a.pool, pl.split, counters, stream);
+  else if (pl.few)
+    rc = launch_shared_prefix_mma(p, a.pool, counters, stream);
   else if (pl.np > 0)
     rc = f32 ? launch_prefix_elem_d<float>(p, pl, counters, dev.device, stream)
              : launch_prefix_elem_d<__nv_bfloat16>(p, pl, counters, dev.device, stream);

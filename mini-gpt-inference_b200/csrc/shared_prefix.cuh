@@ -52,6 +52,9 @@ struct SharedParams {
 int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
                           cudaStream_t stream);
 int shared_own_rows(int64_t rep);
+// The prefix's parts for few rows, eight rows at a time.
+int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
+                             cudaStream_t stream);
 
 // The prefix on tensor cores: how its key tiles are cut.
 struct TcSplit {

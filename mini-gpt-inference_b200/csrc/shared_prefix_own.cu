@@ -1,5 +1,6 @@
 // shared_prefix_own.cu -- the sequences' own keys of the shared-prefix decode
-// for bf16 pools and queries, and the join with the prefix's parts.
+// for bf16 pools and queries, and the join with the prefix's parts; and, where
+// there are few query rows, the prefix itself, eight rows at a time.
 //
 // For the rep query rows of one (sequence, key head) this is a matrix-vector
 // product per row: bound by the bytes of K and V, each read once for all rep
@@ -72,6 +73,7 @@ struct OwnParams {
   int32_t rbox, rb_shift;  // rows per TMA box: min(S, 16)
   int32_t q_vec;           // 4-byte access to pairs of q is legal
   int32_t out_vec;         // 8-byte access to four elements of bf16 out is legal
+  int32_t zero_count;      // PREFIX: counters to clear
 };
 
 template <int DP, int NQ>
@@ -92,7 +94,8 @@ struct OwnSmem {
 };
 
 // NQ groups of 8 query rows; DP: head dimension rounded up to 64 or 128.
-template <int DP, int NQ>
+// PREFIX: the keys are a part of the prefix's, the rows all sequences'.
+template <int DP, int NQ, bool PREFIX>
 __global__ void __launch_bounds__(kWarps * 32)
     shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const __grid_constant__ OwnParams op) {
@@ -111,13 +114,19 @@ __global__ void __launch_bounds__(kWarps * 32)
   idx /= p.Hkv;
   const int chunk = static_cast<int>(idx % p.row_chunks);
   idx /= p.row_chunks;
-  const int split = static_cast<int>(idx % p.own_splits);
-  const int b = static_cast<int>(idx / p.own_splits);
-  const int row0 = b * p.rep + chunk * R;
-  const int nrows = min(R, p.rep - chunk * R);
-  const int head0 = g * p.rep + chunk * R;
-  const int64_t ctx = load_index(p.lens, b * p.len_stride, p.lens_i64);
-  if (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S) {
+  const int split = static_cast<int>(PREFIX ? idx : idx % p.own_splits);
+  const int b = static_cast<int>(PREFIX ? 0 : idx / p.own_splits);
+  const int row0 = (PREFIX ? 0 : b * p.rep) + chunk * R;
+  const int nrows = min(R, (PREFIX ? p.rows : p.rep) - chunk * R);
+  const int head0 = g * p.rep + chunk * R;  // own keys only
+  if constexpr (PREFIX) {
+    let_next_start();
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kWarps * 32) + threadIdx.x; i < op.zero_count;
+         i += static_cast<int64_t>(gridDim.x) * (kWarps * 32))
+      p.cnt[i] = 0;  // of the own-key kernel
+  }
+  const int64_t ctx = PREFIX ? p.prefix : load_index(p.lens, b * p.len_stride, p.lens_i64);
+  if (!PREFIX && (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S)) {
     if (split == 0) {
       if (threadIdx.x == 0) report(p.status, B200_DEV_BAD_LENGTH);
       for (int i = threadIdx.x; i < nrows * p.D; i += kWarps * 32)
@@ -128,16 +137,22 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
   // Steps lie on multiples of 16 positions, so that no step's box leaves its
   // page; the keys outside [lo, hi) of the first and last one are masked.
-  const int64_t origin = p.prefix & ~int64_t(kStep - 1);
-  int64_t k0, hi;
-  const int parts = own_range(p, ctx > p.prefix ? ctx - origin : 0, split, &k0, &hi);
-  if (split >= parts) {
-    end_after_previous();
-    return;
+  int64_t k0, hi, lo;
+  int parts = 1;
+  if constexpr (PREFIX) {
+    lo = k0 = static_cast<int64_t>(split) * p.prefix_per;
+    hi = min(p.prefix, k0 + p.prefix_per);
+  } else {
+    const int64_t origin = p.prefix & ~int64_t(kStep - 1);
+    parts = own_range(p, ctx > p.prefix ? ctx - origin : 0, split, &k0, &hi);
+    if (split >= parts) {
+      end_after_previous();
+      return;
+    }
+    k0 += origin;
+    hi += origin;
+    lo = max(k0, p.prefix);
   }
-  k0 += origin;
-  hi += origin;
-  const int64_t lo = max(k0, p.prefix);
   const int steps = static_cast<int>((hi - k0 + kStep - 1) / kStep);
   const int mine = (steps - warp + kWarps - 1) / kWarps;  // of this warp: warp, warp + 4, ...
 
@@ -155,7 +170,8 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * (n + lane / nb)) * kStep +
                         ((lane % nb) << op.rb_shift);
     if (n + lane / nb >= mine || key >= hi || key + op.rbox <= lo) return -1;
-    int64_t e = load_index(p.tables, b * p.ts0 + (key >> p.s_shift) * p.ts1, p.tables_i64);
+    int64_t e = PREFIX ? load_index(p.prefix_table, (key >> p.s_shift) * p.pt_stride, p.pt_i64)
+                       : load_index(p.tables, b * p.ts0 + (key >> p.s_shift) * p.ts1, p.tables_i64);
     if (e < 0 || e >= p.P) {
       report(p.status, B200_DEV_BAD_BLOCK);
       e = 0;  // an in-bounds page; the status word tells
@@ -198,8 +214,10 @@ __global__ void __launch_bounds__(kWarps * 32)
         const int r = 8 * n + gq, d = 16 * i + 2 * t + 8 * u;
         uint32_t x = 0;
         if (r < nrows && d < p.D) {
+          const int seq = PREFIX ? (row0 + r) / p.rep : b;
+          const int head = PREFIX ? g * p.rep + (row0 + r) - seq * p.rep : head0 + r;
           const __nv_bfloat16* q =
-              static_cast<const __nv_bfloat16*>(p.q) + b * p.qs0 + (head0 + r) * p.qs1 + d * p.qs2;
+              static_cast<const __nv_bfloat16*>(p.q) + seq * p.qs0 + head * p.qs1 + d * p.qs2;
           if (op.q_vec) {
             x = *reinterpret_cast<const uint32_t*>(q);
           } else {
@@ -355,10 +373,10 @@ __global__ void __launch_bounds__(kWarps * 32)
 
   // So far nothing came from the prefix's kernel, whose end this kernel
   // overlaps; its parts, and the counters that it cleared, do.
-  wait_for_previous();
+  if constexpr (!PREFIX) wait_for_previous();
   const int64_t slot_row = (static_cast<int64_t>(g) * p.rows + row0) * p.ns;
   int warps = kWarps, slots = p.np;  // what is joined: the warps' states, slots of the workspace
-  if (parts > 1) {
+  if (PREFIX || parts > 1) {
     // This part goes to its slot; the last one to arrive joins all.
     for (int i = threadIdx.x; i < nrows * (p.D / 4); i += kWarps * 32) {
       const int r = i / (p.D / 4), d = (i % (p.D / 4)) * 4;
@@ -374,10 +392,11 @@ __global__ void __launch_bounds__(kWarps * 32)
         sum = fmaf(f, ml.y, sum);
         a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
       }
-      const int64_t at = slot_row + static_cast<int64_t>(r) * p.ns + p.np + split;
+      const int64_t at = slot_row + static_cast<int64_t>(r) * p.ns + (PREFIX ? split : p.np + split);
       *reinterpret_cast<float4*>(p.acc + at * p.D + d) = a;
       if (d == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(M, sum);
     }
+    if constexpr (PREFIX) return;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -453,11 +472,11 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-template <int DP, int NQ>
+template <int DP, int NQ, bool PREFIX>
 int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
            cudaStream_t stream) {
   const SharedParams& p = op.s;
-  const int64_t grid = static_cast<int64_t>(p.B) * p.own_splits * p.row_chunks * p.Hkv;
+  const int64_t grid = static_cast<int64_t>(PREFIX ? p.np : p.B * p.own_splits) * p.row_chunks * p.Hkv;
   if (p.np + p.own_splits + kWarps > kMaxSlots)
     return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
   const int smem = OwnSmem<DP, NQ>::BYTES + 1024;
@@ -473,7 +492,7 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
   rc = encode_tensor_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.v, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != B200_OK) return rc;
-  auto kern = shared_own_mma_kernel<DP, NQ>;
+  auto kern = shared_own_mma_kernel<DP, NQ, PREFIX>;
   static std::atomic<int> configured[64];
   if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -488,6 +507,17 @@ bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
          s1 % (bytes / 2) == 0;
 }
 
+OwnParams own_params(const SharedParams& p, int zero_count) {
+  OwnParams op;
+  op.s = p;
+  op.rbox = static_cast<int32_t>(std::min<int64_t>(p.S, kStep));
+  op.rb_shift = log2i(op.rbox);
+  op.q_vec = aligned(p.q, p.qs0, p.qs1, p.qs2, 4);
+  op.out_vec = p.out_dtype == B200_DTYPE_BF16 && aligned(p.out, p.os0, p.os1, p.os2, 8);
+  op.zero_count = zero_count;
+  return op;
+}
+
 }  // namespace
 
 int shared_own_rows(int64_t rep) { return rep <= 8 ? 8 : 16; }
@@ -497,16 +527,24 @@ int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, boo
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc != B200_OK) return rc;
-  OwnParams op;
-  op.s = p;
-  op.rbox = static_cast<int32_t>(std::min<int64_t>(p.S, kStep));
-  op.rb_shift = log2i(op.rbox);
-  op.q_vec = aligned(p.q, p.qs0, p.qs1, p.qs2, 4);
-  op.out_vec = p.out_dtype == B200_DTYPE_BF16 && aligned(p.out, p.os0, p.os1, p.os2, 8);
+  const OwnParams op = own_params(p, 0);
   const bool wide = shared_own_rows(p.rep) == 16;
   if (p.D <= 64)
-    return wide ? launch<64, 2>(op, pool, dev, overlap, stream) : launch<64, 1>(op, pool, dev, overlap, stream);
-  return wide ? launch<128, 2>(op, pool, dev, overlap, stream) : launch<128, 1>(op, pool, dev, overlap, stream);
+    return wide ? launch<64, 2, false>(op, pool, dev, overlap, stream)
+                : launch<64, 1, false>(op, pool, dev, overlap, stream);
+  return wide ? launch<128, 2, false>(op, pool, dev, overlap, stream)
+              : launch<128, 1, false>(op, pool, dev, overlap, stream);
+}
+
+int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
+                             cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc != B200_OK) return rc;
+  OwnParams op = own_params(p, zero_count);
+  op.s.row_chunks = static_cast<int32_t>(ceil_div(p.rows, 8));
+  if (p.D <= 64) return launch<64, 1, true>(op, pool, dev, false, stream);
+  return launch<128, 1, true>(op, pool, dev, false, stream);
 }
 
 }  // namespace b200

@@ -1,5 +1,6 @@
 // shared_prefix_tc.cu -- the prefix's part of the shared-prefix decode on
-// tcgen05 tensor cores (bf16 pools and queries, block size >= 8).
+// tcgen05 tensor cores (bf16 pools and queries, block size >= 8, and rows and
+// keys enough).
 //
 // For a key head g the rows q[b, h] of all sequences and of g's query heads
 // form one matrix of B * rep rows: S = Q K^T, P = 2^(S - max), O = P V over
@@ -720,18 +721,17 @@ int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const Device
 
 }  // namespace
 
-// One CTA per SM, at least two key tiles and at most kMaxParts CTAs to a unit
-// (each leaves a part that the join reads).
+// One CTA per SM; where the work is less, whole shares of a unit of at least two
+// key tiles (a CTA that also has to begin another unit takes 7 us longer), and at
+// most kMaxParts of them (each leaves a part that the join reads).
 TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) {
   constexpr int64_t kMinTiles = 2, kMaxParts = 32;
   TcSplit t{};
   t.unit_pairs = static_cast<int>(ceil_div(rows, 2 * kBM));
   t.unit_tiles = static_cast<int>(ceil_div(prefix, kBN));
   t.units = Hkv * t.unit_pairs;
-  const int64_t total = t.units * t.unit_tiles;
-  const int64_t ctas = std::min<int64_t>({static_cast<int64_t>(num_sms), ceil_div(total, kMinTiles),
-                                          t.units * kMaxParts});
-  t.ctas = static_cast<int>(std::max<int64_t>(ctas, 1));
+  const int64_t shares = std::min(ceil_div(t.unit_tiles, kMinTiles), kMaxParts);
+  t.ctas = static_cast<int>(std::min<int64_t>(num_sms, t.units * shares));
   // The most CTAs that share a unit (an upper bound where the units are many).
   int64_t most = 1;
   if (t.units <= 1024) {

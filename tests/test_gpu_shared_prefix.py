@@ -58,6 +58,29 @@ def test_shared_prefix(size, types):
     _check(case(*size, *types, seed=size[0] + size[3]))
 
 
+# Of bf16, with rows and keys enough for the prefix's tensor tiles.
+TILES = [
+    (20, 16, 16, 64, 16, 3001, [i % 7 for i in range(20)]),     # 20 rows to a key head
+    (5, 64, 16, 128, 16, 2801, [1, 64, 17, 33, 0]),             # four heads to each, 20 rows
+    (17, 64, 64, 16, 64, 700, [i for i in range(17)]),          # short heads
+    (37, 20, 4, 80, 32, 3001, [9 * i for i in range(37)]),      # a second tile, partly full
+    (70, 4, 2, 64, 16, 7400, [i % 37 for i in range(70)]),
+    (128, 8, 8, 128, 8, 1100, [i % 3 for i in range(128)]),     # one tile, just full
+    (129, 8, 8, 32, 16, 1000, [i % 2 for i in range(129)]),     # a row more
+    (256, 32, 32, 128, 16, 130, [i % 5 for i in range(256)]),   # two keys in the last key tile
+    (257, 32, 32, 64, 16, 128, [1] * 257),                      # one key tile; a row in the third tile
+]
+
+
+@pytest.mark.parametrize("size", TILES, ids=lambda s: str(s[:6]))
+def test_shared_prefix_tiles(size):
+    _check(case(*size, seed=size[0]))
+
+
+# A small and a large size for the tests below.
+BOTH = pytest.mark.parametrize("heads", [(8, 2, 700), (64, 16, 2900)], ids=str)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=str)
 def test_other_layer_strides_and_index_types(dtype, index):
@@ -76,17 +99,21 @@ def test_other_layer_strides_and_index_types(dtype, index):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
-def test_large_scores_keep_their_maximum(dtype):
+@BOTH
+def test_large_scores_keep_their_maximum(heads, dtype):
     # Scores of a few hundred: only a running maximum keeps the exponentials finite.
-    _check(case(4, 8, 2, 128, 16, 700, [3, 90, 0, 41], dtype, seed=9, scale=30.0))
+    hq, hkv, prefix = heads
+    _check(case(5, hq, hkv, 128, 16, prefix, [3, 90, 0, 41, 7], dtype, seed=9, scale=30.0))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
-def test_rows_without_a_valid_length_are_zero_and_told(dtype):
+@BOTH
+def test_rows_without_a_valid_length_are_zero_and_told(heads, dtype):
     from b200attn import _lib
 
-    cpu = case(5, 8, 2, 64, 16, 40, [4, 9, 0, 30, 7], dtype, seed=6)
-    cpu.lens[1] = 39  # shorter than the prefix: a padding row
+    hq, hkv, prefix = heads
+    cpu = case(5, hq, hkv, 64, 16, prefix, [4, 9, 0, 30, 7], dtype, seed=6)
+    cpu.lens[1] = prefix - 1  # shorter than the prefix: a padding row
     cpu.lens[3] = 16 * cpu.tables.shape[1] + 1
     cpu.lens[4] = 0
     c = to_device(cpu)
@@ -99,21 +126,24 @@ def test_rows_without_a_valid_length_are_zero_and_told(dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("where", ["prefix", "own"])
-def test_bad_pages_are_told_and_touch_no_other_sequence(dtype, where):
+@BOTH
+def test_bad_pages_are_told_and_touch_no_other_sequence(heads, dtype, where):
     from b200attn import _lib
 
-    cpu = case(3, 4, 2, 128, 16, 64, [20, 33, 5], dtype, seed=7, poison=False)
+    hq, hkv, prefix = heads
+    cpu = case(5, hq, hkv, 128, 16, prefix, [20, 33, 5, 0, 1], dtype, seed=7, poison=False)
     c = to_device(cpu)
     if where == "prefix":
         c.table[2] = cpu.pool.k.shape[1]
     else:
-        c.tables[1, 5] = -1
+        c.tables[1, prefix // 16 + 1] = -1
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     out = _run(c, status=status)
     assert int(status) == _lib.DEV_BAD_BLOCK
     if where == "own":
         want = _run(to_device(cpu))
-        assert torch.equal(out[[0, 2]], want[[0, 2]])
+        rest = [0, 2, 3, 4]
+        assert torch.equal(out[rest], want[rest])
 
 
 def test_unread_table_entries_and_prefix_table_as_host_list():
@@ -125,17 +155,20 @@ def test_unread_table_entries_and_prefix_table_as_host_list():
     assert torch.equal(_run(c), want)
 
 
-def test_results_repeat_bit_for_bit():
-    cpu = case(9, 32, 8, 128, 16, 1000, [i * 30 for i in range(9)], BF16, seed=10)
+@BOTH
+def test_results_repeat_bit_for_bit(heads):
+    cpu = case(9, *heads[:2], 128, 16, heads[2], [i * 30 for i in range(9)], BF16, seed=10)
     c = to_device(cpu)
     first = _run(c)
     for _ in range(5):
         assert torch.equal(_run(c), first)
 
 
-def test_graph_replays_and_streams_have_their_own_workspaces():
-    a = to_device(case(5, 8, 2, 128, 16, 500, [1, 70, 200, 3, 0], BF16, seed=11))
-    b = to_device(case(5, 8, 2, 128, 16, 500, [9, 0, 10, 300, 2], BF16, seed=12))
+@BOTH
+def test_graph_replays_and_streams_have_their_own_workspaces(heads):
+    hq, hkv, prefix = heads
+    a = to_device(case(5, hq, hkv, 128, 16, prefix, [1, 70, 200, 3, 0], BF16, seed=11))
+    b = to_device(case(5, hq, hkv, 128, 16, prefix, [9, 0, 10, 300, 2], BF16, seed=12))
     want = [_run(a), _run(b)]
     torch.cuda.synchronize()
     graphs, outs = [], []
@@ -173,12 +206,13 @@ def test_graph_replays_and_streams_have_their_own_workspaces():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
-def test_calls_back_to_back_in_one_stream(dtype):
+@pytest.mark.parametrize("prefix", [3000, 4200])
+def test_calls_back_to_back_in_one_stream(prefix, dtype):
     """Kernels of a call overlap; calls must not: memory that one call has given
     back serves the next, also where no row of a call is valid."""
-    a = to_device(case(33, 8, 2, 128, 16, 3000, [i for i in range(33)], dtype, seed=16))
+    a = to_device(case(33, 8, 2, 128, 16, prefix, [i for i in range(33)], dtype, seed=16))
     b = to_device(case(3, 8, 2, 128, 16, 700, [9, 0, 10], dtype, seed=17))
-    none = to_device(case(33, 8, 2, 128, 16, 3000, [5] * 33, dtype, seed=18))
+    none = to_device(case(33, 8, 2, 128, 16, prefix, [5] * 33, dtype, seed=18))
     none.lens.fill_(1)
     want_a, want_b = _run(a), _run(b)
     torch.cuda.synchronize()
@@ -191,22 +225,26 @@ def test_calls_back_to_back_in_one_stream(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
-def test_scores_that_keep_growing(dtype):
+@BOTH
+def test_scores_that_keep_growing(heads, dtype):
     """Each key's score exceeds the last's: the reference moves again and again."""
-    cpu = case(5, 8, 2, 64, 16, 1500, [3, 0, 40, 100, 7], dtype, seed=19)
+    hq, hkv, prefix = heads
+    cpu = case(5, hq, hkv, 64, 16, prefix, [3, 0, 40, 100, 7], dtype, seed=19)
     k = cpu.pool.k.float()
-    at = torch.arange(1500)
+    at = torch.arange(prefix)
     rows = cpu.table[at // 16]
-    step = (at / 1500 * 60)[:, None, None]
+    step = (at / prefix * 60)[:, None, None]
     q = cpu.q.float()
-    k[0, rows, at % 16] = step * q[0, :2][None] / q[0, :2].square().sum(-1, keepdim=True) * 8
+    k[0, rows, at % 16] = step * q[0, :hkv][None] / q[0, :hkv].square().sum(-1, keepdim=True) * 8
     cpu.pool.k = k.to(cpu.pool.k.dtype)
     _check(cpu)
 
 
 @pytest.mark.parametrize("size", [(1, 1, 1, 64, 16, 300, [9]), (4, 32, 8, 128, 16, 2048, [1, 64, 17, 33]),
                                   (64, 4, 2, 80, 32, 500, [i for i in range(64)]),
-                                  (3, 40, 4, 96, 16, 1000, [0, 200, 31])], ids=str)
+                                  (3, 40, 4, 96, 16, 1000, [0, 200, 31]), TILES[0], TILES[1],
+                                  (128, 8, 8, 128, 8, 1100, [i % 3 for i in range(128)]),
+                                  (40, 6, 2, 96, 64, 6000, [i for i in range(40)])], ids=str)
 def test_few_rows_differ_by_their_own_rounding_alone(size):
     """At most 128 rows to a key head: what the weights' rounding leaves takes part."""
     _check(case(*size, BF16, seed=22), tensor_cores="split")
@@ -289,7 +327,8 @@ def test_decode_steps_of_a_rotary_model_behind_one_prompt(dtype):
 
 
 @pytest.mark.parametrize("size", [(70, 4, 2, 64, 16, 300, [i % 37 for i in range(70)]),
-                                  (5, 32, 8, 128, 16, 2048, [1, 64, 170, 33, 0])], ids=str)
+                                  (5, 32, 8, 128, 16, 2048, [1, 64, 170, 33, 0]), TILES[1], TILES[3]],
+                         ids=str)
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_queries_that_are_no_numbers_stay_in_their_rows(size, dtype):
     cpu = case(*size, dtype, seed=41)
@@ -305,15 +344,17 @@ def test_queries_that_are_no_numbers_stay_in_their_rows(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
-def test_out_may_be_q_itself(dtype):
-    cpu = case(6, 16, 2, 128, 16, 700, [600, 3, 0, 40, 1300, 77], dtype, seed=42)
+@BOTH
+def test_out_may_be_q_itself(heads, dtype):
+    hq, hkv, prefix = heads
+    cpu = case(6, hq, hkv, 128, 16, prefix, [600, 3, 0, 40, 1300, 77], dtype, seed=42)
     c = to_device(cpu)
     want = _run(c)
     for _ in range(3):
         c.q.copy_(cpu.q)
         assert _run(c, out=c.q).data_ptr() == c.q.data_ptr()
         assert torch.equal(c.q, want)
-    wide = torch.empty(6, 16, 128, device="cuda")
+    wide = torch.empty(6, hq, 128, device="cuda")
     c.q.copy_(cpu.q)
     assert torch.equal(_run(c, out=wide).to(dtype), want)
 
