@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
   __syncthreads();
   if (!last) return;
   __threadfence();
-  for (int r = threadIdx.x >> 5; r < nrows; r += 4)
-    join_row(p, g, row0 + r, parts);
+  static_assert(ElemSmem<R, DP>::ROWS >= kJoinFloats, "the join's shared memory");
+  join_rows(p, g, row0, nrows, parts, sm);
 }
 
 // ------------------------------------------------------------------ host

@@ -113,61 +113,97 @@ int launch_own(void (*kern)(Params...), int64_t grid, int block, int smem, cudaS
   return e == cudaSuccess ? B200_OK : cuda_fail(e, "shared prefix own-key launch");
 }
 
-// The joined row (g, R), by one warp: sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s -
-// M) l_s over the prefix's slots and the first `parts` own ones (at most 96 in
-// all).  A lane holds the factors of every 32nd part and four elements of the
-// row; eight parts' loads are on their way together.
-__device__ __forceinline__ void join_row(const SharedParams& p, int g, int R, int parts) {
-  constexpr int kHeld = 3;
-  const int lane = threadIdx.x & 31;
-  const int64_t slot0 = (static_cast<int64_t>(g) * p.rows + R) * p.ns;
-  const int n = p.np + parts;
-  const float2* ml = reinterpret_cast<const float2*>(p.ml) + slot0;
-  float2 v[kHeld];
-  float M = -INFINITY, sum = 0.f, f[kHeld];
+// The joined rows row0 .. row0 + nrows - 1 (at most 8) of key head g, by a block
+// of 128 threads: sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the
+// prefix's slots and the first `parts` own ones (at most 96 in all).  `sm`:
+// kJoinFloats of shared memory that the block is done with.  Four elements of a
+// row are a thread's, or, where the rows are short or few, several threads' that
+// share the parts out; the first loads are on their way before the factors are
+// known.
+constexpr int kJoinParts = 96, kJoinAhead = 8;
+constexpr int kJoinFloats = 8 * kJoinParts + 128 * 4;
+__device__ __forceinline__ void join_rows(const SharedParams& p, int g, int row0, int nrows, int parts,
+                                          float* sm) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = p.np + parts, quads = p.D / 4, items = nrows * quads;
+  const int sharers = max(1, 128 / items);
+  const int first = tid / items;  // of this thread's parts (sharers > 1)
+  const int64_t slot0 = (static_cast<int64_t>(g) * p.rows + row0) * p.ns;
+  float4 v[kJoinAhead];
+  auto fetch = [&](int i, int j0) {
+    const float* acc = p.acc + (slot0 + static_cast<int64_t>(i / quads) * p.ns + j0) * p.D + (i % quads) * 4;
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    v[i] = lane + 32 * i < n ? __ldcg(ml + lane + 32 * i) : make_float2(-INFINITY, 0.f);
-    M = fmaxf(M, v[i].x);
-  }
+    for (int k = 0; k < kJoinAhead; ++k)
+      if (j0 + k * sharers < n)
+        v[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(k * sharers) * p.D));
+  };
+  const int item0 = sharers > 1 ? tid % items : tid;
+  const bool works = sharers > 1 ? first < sharers : tid < items;
+  const int part0 = sharers > 1 ? first : 0;
+  if (works) fetch(item0, part0);
+  for (int r = warp; r < nrows; r += 4) {  // factors, a warp per row
+    const float2* ml = reinterpret_cast<const float2*>(p.ml) + slot0 + static_cast<int64_t>(r) * p.ns;
+    float2 x[kJoinParts / 32];
+    float M = -INFINITY, sum = 0.f;
 #pragma unroll
-  for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    // A part without a weight (no key, or a slot that stays unused) has no factor.
-    f[i] = v[i].x == -INFINITY ? (v[i].y == 0.f ? 0.f : 1.f) : exp2f(v[i].x - M);
-    sum = fmaf(f[i], v[i].y, sum);
-  }
-#pragma unroll
-  for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-  const float inv = 1.0f / sum;
-  const bool mine = lane * 4 < p.D;
-  const float* acc = p.acc + slot0 * p.D + lane * 4;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j0 = 0; j0 < n; j0 += 8) {
-    float4 x[8];
-    float fj[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int j = j0 + k;
-      fj[k] = __shfl_sync(0xffffffffu, j < 32 ? f[0] : j < 64 ? f[1] : f[2], j & 31) * inv;
-      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (j < n && fj[k] != 0.f && mine)
-        x[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(j) * p.D));
+    for (int i = 0; i < kJoinParts / 32; ++i) {
+      x[i] = lane + 32 * i < n ? __ldcg(ml + lane + 32 * i) : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, x[i].x);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      a.x = fmaf(fj[k], x[k].x, a.x), a.y = fmaf(fj[k], x[k].y, a.y);
-      a.z = fmaf(fj[k], x[k].z, a.z), a.w = fmaf(fj[k], x[k].w, a.w);
+    for (int w = 16; w >= 1; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+#pragma unroll
+    for (int i = 0; i < kJoinParts / 32; ++i) {
+      // A part without a weight (no key, or a slot that stays unused) has no factor.
+      const float f = x[i].x == -INFINITY ? (x[i].y == 0.f ? 0.f : 1.f) : exp2f(x[i].x - M);
+      sum = fmaf(f, x[i].y, sum);
+      x[i].x = f;
     }
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < kJoinParts / 32; ++i) sm[r * kJoinParts + lane + 32 * i] = x[i].x * inv;
   }
-  if (!mine) return;
-  const int b = R / p.rep, h = g * p.rep + R % p.rep;
-  const int64_t at = b * p.os0 + h * p.os1 + lane * 4 * p.os2;
-  store_elem(p.out, at, p.out_dtype, a.x);
-  store_elem(p.out, at + p.os2, p.out_dtype, a.y);
-  store_elem(p.out, at + 2 * p.os2, p.out_dtype, a.z);
-  store_elem(p.out, at + 3 * p.os2, p.out_dtype, a.w);
+  __syncthreads();
+  auto store = [&](int i, const float4& a) {
+    const int R = row0 + i / quads, b = R / p.rep, h = g * p.rep + R % p.rep;
+    const int64_t at = b * p.os0 + h * p.os1 + (i % quads) * 4 * p.os2;
+    store_elem(p.out, at, p.out_dtype, a.x);
+    store_elem(p.out, at + p.os2, p.out_dtype, a.y);
+    store_elem(p.out, at + 2 * p.os2, p.out_dtype, a.z);
+    store_elem(p.out, at + 3 * p.os2, p.out_dtype, a.w);
+  };
+  float4* share = reinterpret_cast<float4*>(sm + 8 * kJoinParts);
+  if (works)
+    for (int i = item0; i < items; i += sharers > 1 ? items : 128) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j0 = part0; j0 < n; j0 += kJoinAhead * sharers) {
+        if (i != item0 || j0 != part0) fetch(i, j0);
+#pragma unroll
+        for (int k = 0; k < kJoinAhead; ++k) {
+          const int j = j0 + k * sharers;
+          const float f = j < n ? sm[i / quads * kJoinParts + j] : 0.f;
+          if (f == 0.f) continue;  // an unused slot holds anything
+          a.x = fmaf(f, v[k].x, a.x), a.y = fmaf(f, v[k].y, a.y);
+          a.z = fmaf(f, v[k].z, a.z), a.w = fmaf(f, v[k].w, a.w);
+        }
+      }
+      if (sharers > 1)
+        share[tid] = a;
+      else
+        store(i, a);
+    }
+  if (sharers == 1) return;
+  __syncthreads();
+  if (tid < items) {
+    float4 a = share[tid];
+    for (int k = 1; k < sharers; ++k) {
+      const float4 x = share[tid + k * items];
+      a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+    }
+    store(tid, a);
+  }
 }
 
 }  // namespace b200

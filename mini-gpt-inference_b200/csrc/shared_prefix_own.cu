@@ -32,6 +32,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStep = 16;      // keys a warp takes at a time
+constexpr int kAhead = 8;      // parts of a row that the join loads together (4 and 16: 1 to 5 % slower at
+                               // many parts, and at many short joins)
 constexpr int kMaxSlots = 72;  // parts of a row: 33 of the prefix, 32 own ones, 4 warps
 
 __device__ __forceinline__ float ex2(float x) {
@@ -371,9 +373,9 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
   __syncthreads();
 
-  // So far nothing came from the prefix's kernel, whose end this kernel
-  // overlaps; its parts, and the counters that it cleared, do.
-  if constexpr (!PREFIX) wait_for_previous();
+  // Nothing so far, nor this part's way to its slot, comes from the prefix's
+  // kernel, whose end this kernel overlaps; its parts, and the counters that it
+  // cleared, do.
   const int64_t slot_row = (static_cast<int64_t>(g) * p.rows + row0) * p.ns;
   int warps = kWarps, slots = p.np;  // what is joined: the warps' states, slots of the workspace
   if (PREFIX || parts > 1) {
@@ -397,6 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       if (d == 0) *reinterpret_cast<float2*>(p.ml + at * 2) = make_float2(M, sum);
     }
     if constexpr (PREFIX) return;
+    wait_for_previous();
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -408,7 +411,22 @@ __global__ void __launch_bounds__(kWarps * 32)
     __threadfence();
     warps = 0;
     slots = p.np + parts;
+  } else {
+    wait_for_previous();
   }
+
+  // Two accesses to memory, one behind the other, would be most of a small call's
+  // join, so a thread's first parts are on their way before their factors are
+  // known (slots that stay unused hold anything: their factor is 0).
+  const int items = nrows * (p.D / 4);
+  float4 v[kAhead];
+  auto fetch = [&](int i, int j0) {
+    const float* acc = p.acc + (slot_row + static_cast<int64_t>(i / (p.D / 4)) * p.ns + j0) * p.D + (i % (p.D / 4)) * 4;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (j0 + k < slots) v[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(k) * p.D));
+  };
+  if (threadIdx.x < items) fetch(threadIdx.x, 0);
 
   // Factors 2^(m - M) / L of every part of every row, a warp per row.
   const int total = warps + slots;
@@ -437,27 +455,21 @@ __global__ void __launch_bounds__(kWarps * 32)
     for (int j = lane; j < total; j += 32) s_ml[j * R + r].x *= inv;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nrows * (p.D / 4); i += kWarps * 32) {
+  for (int i = threadIdx.x; i < items; i += kWarps * 32) {
     const int r = i / (p.D / 4), d = (i % (p.D / 4)) * 4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float f, const float4& v) {
-      a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+    auto add = [&](float f, const float4& x) {
+      a.x = fmaf(f, x.x, a.x), a.y = fmaf(f, x.y, a.y), a.z = fmaf(f, x.z, a.z), a.w = fmaf(f, x.w, a.w);
     };
     for (int j = 0; j < warps; ++j)
       add(s_ml[j * R + r].x, *reinterpret_cast<const float4*>(s_o + (j * R + r) * L::LD + d));
-    const float* acc = p.acc + (slot_row + static_cast<int64_t>(r) * p.ns) * p.D + d;
-    for (int j0 = 0; j0 < slots; j0 += 8) {  // eight loads on their way together
-      float4 v[8];
-      float f[8];
+    for (int j0 = 0; j0 < slots; j0 += kAhead) {
+      if (i != threadIdx.x || j0 > 0) fetch(i, j0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int j = j0 + k;
-        f[k] = j < slots ? s_ml[(warps + j) * R + r].x : 0.f;
-        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (f[k] != 0.f) v[k] = __ldcg(reinterpret_cast<const float4*>(acc + static_cast<int64_t>(j) * p.D));
+      for (int k = 0; k < kAhead; ++k) {
+        const float f = j0 + k < slots ? s_ml[(warps + j0 + k) * R + r].x : 0.f;
+        if (f != 0.f) add(f, v[k]);
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) add(f[k], v[k]);
     }
     const int64_t at = b * p.os0 + (head0 + r) * p.os1 + d * p.os2;
     if (op.out_vec) {
