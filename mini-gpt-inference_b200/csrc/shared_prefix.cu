@@ -369,11 +369,14 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     pl.np = pl.split.np;
   } else if (pl.few) {
     // Two CTAs per SM, three where much is read more than once; at least 64
-    // keys a part, and above 16 parts, which the join has to read, 256 (2048
-    // keys of 8 heads: 16 parts 9.8 us, 8 and 32 parts 10.8).
+    // keys a part, above 16 parts, which the join has to read, 256 (2048 keys of
+    // 8 heads: 16 parts 9.8 us, 8 and 32 parts 10.8), and above 32 parts 1024
+    // (131072 keys of 2 heads: 64 parts 43 us, 32 parts 59; 32768 keys of 4: 29
+    // and 26).
     const int per_sm = rows <= 8 || eights * prefix < (int64_t(1) << 18) ? 2 : 3;
     int64_t parts = std::min({per_sm * num_sms / eights, ceil_div(prefix, 64),
-                              std::max<int64_t>(16, ceil_div(prefix, 256)), int64_t(32)});
+                              std::max({int64_t(16), std::min<int64_t>(ceil_div(prefix, 256), 32),
+                                        std::min<int64_t>(ceil_div(prefix, 1024), 64)})});
     pl.prefix_per = ceil_div(ceil_div(prefix, std::max<int64_t>(parts, 1)), 16) * 16;
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   } else if (prefix > 0) {

@@ -34,7 +34,7 @@ constexpr int kWarps = 4;
 constexpr int kStep = 16;      // keys a warp takes at a time
 constexpr int kAhead = 8;      // parts of a row that the join loads together (4 and 16: 1 to 5 % slower at
                                // many parts, and at many short joins)
-constexpr int kMaxSlots = 72;  // parts of a row: 33 of the prefix, 32 own ones, 4 warps
+constexpr int kMaxSlots = 102;  // parts of a row: 65 of the prefix, 32 own ones, 4 warps
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -722,15 +722,17 @@ int launch(const TcParams& p, const b200_kv_pool_t& pool, int ctas, const Device
 }  // namespace
 
 // One CTA per SM; where the work is less, whole shares of a unit of at least two
-// key tiles (a CTA that also has to begin another unit takes 7 us longer), and at
-// most kMaxParts of them (each leaves a part that the join reads).
+// key tiles (a CTA that also has to begin another unit takes 7 us longer); each
+// leaves a part that the join reads, so that more than 32 of them are of at least
+// four tiles, and there are at most 64 (64 rows of one head, 131072 keys: 53 us,
+// with 32 shares 75).
 TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) {
-  constexpr int64_t kMinTiles = 2, kMaxParts = 32;
   TcSplit t{};
   t.unit_pairs = static_cast<int>(ceil_div(rows, 2 * kBM));
   t.unit_tiles = static_cast<int>(ceil_div(prefix, kBN));
   t.units = Hkv * t.unit_pairs;
-  const int64_t shares = std::min(ceil_div(t.unit_tiles, kMinTiles), kMaxParts);
+  const int64_t shares = std::max(std::min<int64_t>(ceil_div(t.unit_tiles, 2), 32),
+                                  std::min<int64_t>(ceil_div(t.unit_tiles, 4), 64));
   t.ctas = static_cast<int>(std::min<int64_t>(num_sms, t.units * shares));
   // The most CTAs that share a unit (an upper bound where the units are many).
   int64_t most = 1;

@@ -257,6 +257,11 @@ def test_a_long_prefix_in_several_runs_to_a_cta():
     _check(case(9, 8, 8, 64, 32, 20011, [i for i in range(9)], BF16, seed=21))
 
 
+@pytest.mark.parametrize("size", [(2, 4, 1, 128, 64, 66001, [0, 150]), (5, 8, 1, 64, 256, 67000, [1] * 5)], ids=str)
+def test_one_key_head_and_the_most_parts(size):
+    _check(case(*size, BF16, seed=44), tensor_cores="split")
+
+
 def test_torch_op_matches_direct_call():
     c = to_device(case(3, 4, 2, 64, 16, 70, [10, 20, 1], BF16, seed=13))
     got = torch.ops.b200attn.shared_prefix_decode(c.q, c.pool.k, c.pool.v, c.table, c.prefix,

@@ -89,7 +89,7 @@ def test_workspace_size_is_bounded_by_the_parts():
     assert size(4, 8, 16, 128, 0, 4, 16, bf16, bf16) == 0  # fewer query heads than heads
     assert size(4, 32, 8, 128, 2048, 132, 16, bf16, bf16) > 0
     # A row has at most 64 parts of the prefix and 32 of its own.
-    for b, width in ((1, 1), (3, 4096), (64, 4096), (256, 65536)):
+    for b, width in ((1, 1), (3, 4096), (64, 4096), (256, 65536), (3, 65536)):
         for prefix in (0, 1, 4096, width * 16):
             got = size(b, 32, 8, 128, prefix, width, 16, bf16, bf16)
             assert 0 < got <= b * 32 * 96 * (128 + 2) * 4 + b * 8 * 4 + 4 * 256
