@@ -8,6 +8,9 @@ also takes grouped heads (several query heads to a key/value head).
 """
 from __future__ import annotations
 
+import functools
+import operator
+
 import torch
 
 from . import _lib
@@ -16,6 +19,13 @@ from .ops import (_DTYPES, _INDEX, _DeviceCall, _index_arg, _inference_only, _la
 from .rope import _check_place
 
 _PACK = _lib.packer(_lib.SharedPrefixArgs).pack
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(index: int, *sizes) -> int:
+    """The workspace that a call of these sizes needs on device ``index``."""
+    with torch.cuda.device(index):
+        return _lib.load().b200_shared_prefix_decode_workspace_size(*sizes)
 
 
 def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: int,
@@ -66,6 +76,7 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
         raise ValueError("context_lengths must have shape [B]")
     if block_tables.dtype not in _INDEX or context_lengths.dtype not in _INDEX:
         raise ValueError("block_tables and context_lengths must contain integers")
+    prefix_len = operator.index(prefix_len)
     if prefix_len < 0:
         raise ValueError("prefix_len must be >= 0")
     if block_tables.get_device() != index or context_lengths.get_device() != index:
@@ -87,8 +98,7 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     # A workspace of the call's own, from the allocator of the current stream
     # (or of the graph being captured): calls on other streams, and other
     # graphs' replays, have others.
-    nbytes = lib.b200_shared_prefix_decode_workspace_size(b, hq, h, d, prefix_len, width, block,
-                                                          kv_dtype, qd)
+    nbytes = _workspace_bytes(index, b, hq, h, d, prefix_len, width, block, kv_dtype, qd)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     args = _PACK(
         *pool_fields, layer_idx, b, hq, prefix_len, width, q.data_ptr(), *q.stride(), out.data_ptr(),

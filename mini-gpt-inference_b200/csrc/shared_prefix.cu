@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 
 #include "common.cuh"
 #include "host_util.h"
