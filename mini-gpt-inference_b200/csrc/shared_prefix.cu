@@ -9,7 +9,8 @@
 // are a matrix-vector product per sequence; parts are joined by their running
 // maximum and sum.
 //
-// Element kernels (any pool and query type, exact f32): a tile of R query
+// Element kernels (any pool and query type in f32; f32 pools, and pages of fewer
+// than 8 tokens): a tile of R query
 // rows in shared memory, key tiles of 32, thread tiles of scores and outputs
 // in registers, online softmax in the log2 domain.
 #include <math.h>
@@ -343,10 +344,11 @@ size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix, int64_t max_own,
                      int64_t S, int kv_dtype, int q_dtype, int num_sms) {
   SharedPlan pl{};
-  // bf16 throughout: the products may run on tensor cores.  Queries of other
-  // types, and f32 pools, would lose bits there.
+  // A bf16 pool's products run on tensor cores: the large tiles take bf16
+  // queries, the warp-level form any, f16 and f32 ones in exact pieces.  f32
+  // pools would lose bits there.
   // (Pages of fewer than 8 tokens would make swizzled boxes of less than 1 KB.)
-  pl.mma = kv_dtype == B200_DTYPE_BF16 && q_dtype == B200_DTYPE_BF16 && S >= 8;
+  pl.mma = kv_dtype == B200_DTYPE_BF16 && S >= 8;
   const int64_t rep = Hq / Hkv, rows = B * rep;
   const bool mma = pl.mma;
   // Few rows leave most of a tensor tile empty: there the prefix is worked off
@@ -358,7 +360,8 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
   // 8192 30 against 23.  (16 rows at a time by the wide form of the kernel, whose
   // longer code has to be fetched first: 12 us where two times eight take 8.)
   const int64_t eights = ceil_div(rows, 8) * Hkv;
-  pl.few = mma && prefix > 0 && (rows <= 16 || eights * prefix < (int64_t(1) << 17));
+  pl.few = mma && prefix > 0 &&
+           (q_dtype != B200_DTYPE_BF16 || rows <= 16 || eights * prefix < (int64_t(1) << 17));
   pl.tc = mma && prefix > 0 && !pl.few;
   // Prefix: parts of whole key tiles that give about two CTAs per SM.
   pl.np = 0;
@@ -376,7 +379,8 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     int64_t parts = std::min({per_sm * num_sms / eights, ceil_div(prefix, 64),
                               std::max({int64_t(16), std::min<int64_t>(ceil_div(prefix, 256), 32),
                                         std::min<int64_t>(ceil_div(prefix, 1024), 64)})});
-    pl.prefix_per = ceil_div(ceil_div(prefix, std::max<int64_t>(parts, 1)), 16) * 16;
+    parts = std::max(parts, std::min<int64_t>(ceil_div(prefix, 4096), 32));
+    pl.prefix_per = ceil_div(ceil_div(prefix, parts), 16) * 16;
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   } else if (prefix > 0) {
     const int64_t units = ceil_div(rows, 64) * Hkv;
@@ -386,7 +390,7 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   }
   // Own keys: enough parts to fill the GPU, none much longer than 1024 keys.
-  pl.row_chunks = static_cast<int>(ceil_div(rep, mma ? shared_own_rows(rep) : 8));
+  pl.row_chunks = static_cast<int>(ceil_div(rep, mma ? shared_own_rows(rep, q_dtype) : 8));
   pl.own_min = mma ? 128 : 64;
   const int64_t units = B * Hkv * pl.row_chunks;
   int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));

@@ -47,12 +47,12 @@ struct SharedParams {
   float qscale;  // log2(e) / sqrt(D)
 };
 
-// Own keys and join, bf16 pool and queries; the rows of a key head one CTA
+// Own keys and join, bf16 pool; the rows of a key head one CTA
 // takes.  `overlap`: the kernel ahead on the stream is the prefix's.
 int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
                           cudaStream_t stream);
-int shared_own_rows(int64_t rep);
-// The prefix's parts for few rows, eight rows at a time.
+int shared_own_rows(int64_t rep, int q_dtype);
+// The prefix's parts, eight rows at a time.
 int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
                              cudaStream_t stream);
 

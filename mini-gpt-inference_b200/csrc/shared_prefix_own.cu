@@ -1,6 +1,6 @@
 // shared_prefix_own.cu -- the sequences' own keys of the shared-prefix decode
-// for bf16 pools and queries, and the join with the prefix's parts; and, where
-// there are few query rows, the prefix itself, eight rows at a time.
+// for bf16 pools, and the join with the prefix's parts; and, for few query rows
+// and for f16 and f32 queries, the prefix itself, eight rows at a time.
 //
 // For the rep query rows of one (sequence, key head) this is a matrix-vector
 // product per row: bound by the bytes of K and V, each read once for all rep
@@ -17,7 +17,9 @@
 // CTAs fit an SM, so that one's beginning and join pass beside the others'
 // loads.  64 sequences of 32 heads with up to 1024 own keys (537 MB): 87 us,
 // 6.2 TB/s; with three stages, and two CTAs, 95 us; with the operands loaded
-// straight into registers, one step a warp, 213 us.
+// straight into registers, one step a warp, 213 us.  f16 and f32 queries cost
+// little more, and far less than f32 arithmetic: 64 sequences of 8 x 4 heads behind
+// 4096 keys 84 and 90 us (element kernels 219), 4 behind 32768 42 and 46 (185).
 #include <algorithm>
 #include <atomic>
 
@@ -97,12 +99,16 @@ struct OwnSmem {
 
 // NQ groups of 8 query rows; DP: head dimension rounded up to 64 or 128.
 // PREFIX: the keys are a part of the prefix's, the rows all sequences'.
-template <int DP, int NQ, bool PREFIX>
+// QP: bf16 pieces that a query element is the exact sum of: 1 for bf16, 2 for
+// f16 (11 bits), 3 for f32 (24 bits).  A piece is another product, and there is
+// time for them.  The weights take part in as many pieces, and at least in two:
+// what is left of them is 2^-16, with three 2^-24.
+template <int DP, int NQ, bool PREFIX, int QP>
 __global__ void __launch_bounds__(kWarps * 32)
     shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const __grid_constant__ OwnParams op) {
   using L = OwnSmem<DP, NQ>;
-  constexpr int NS = L::STAGES, R = L::R;
+  constexpr int NS = L::STAGES, R = L::R, PP = QP == 3 ? 3 : 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const SharedParams& p = op.s;
@@ -206,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   for (int n = 0; n < issued; ++n) issue(n);
 
   // Query fragments: row 8n + gq, d = 16 i + 2t + {0, 1} and + 8.
-  uint32_t qf[NQ][DP / 16][2];
+  uint32_t qf[QP][NQ][DP / 16][2];
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -214,20 +220,25 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int r = 8 * n + gq, d = 16 * i + 2 * t + 8 * u;
-        uint32_t x = 0;
+#pragma unroll
+        for (int c = 0; c < QP; ++c) qf[c][n][i][u] = 0;
         if (r < nrows && d < p.D) {
           const int seq = PREFIX ? (row0 + r) / p.rep : b;
           const int head = PREFIX ? g * p.rep + (row0 + r) - seq * p.rep : head0 + r;
-          const __nv_bfloat16* q =
-              static_cast<const __nv_bfloat16*>(p.q) + seq * p.qs0 + head * p.qs1 + d * p.qs2;
-          if (op.q_vec) {
-            x = *reinterpret_cast<const uint32_t*>(q);
+          const int64_t at = seq * p.qs0 + head * p.qs1 + d * p.qs2;
+          if (QP == 1 && op.q_vec) {
+            qf[0][n][i][u] = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
           } else {
-            const __nv_bfloat162 h = __halves2bfloat162(q[0], q[p.qs2]);
-            x = *reinterpret_cast<const uint32_t*>(&h);
+            constexpr int type = QP == 1 ? B200_DTYPE_BF16 : QP == 2 ? B200_DTYPE_F16 : B200_DTYPE_F32;
+            float x = load_elem(p.q, at, type), y = load_elem(p.q, at + p.qs2, type);
+#pragma unroll
+            for (int c = 0; c < QP; ++c) {
+              qf[c][n][i][u] = pack_bf16(x, y);
+              const float2 f = bf16x2_to_float2(qf[c][n][i][u]);
+              x -= f.x, y -= f.y;
+            }
           }
         }
-        qf[n][i][u] = x;
       }
 
   // Row 8n + 2t + u: m[n][u] (the same in its 8 lanes) and this lane's l;
@@ -268,13 +279,15 @@ __global__ void __launch_bounds__(kWarps * 32)
       const uint32_t ch = (2 * i + k_hi) & 7;
       ldmatrix4(a, kt + (i / 4) * L::HALF + k_row + ((ch ^ sw) << 4));
 #pragma unroll
-      for (int c = 0; c < NQ; ++c) mma16816(s[c][i & 1], a, qf[c][i][0], qf[c][i][1]);
+      for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int w = 0; w < QP; ++w) mma16816(s[c][i & 1], a, qf[w][c][i][0], qf[w][c][i][1]);
     }
     const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * n) * kStep;
     const bool edge = key < lo || key + kStep > hi;
     const bool in0 = !edge || (key + gq >= lo && key + gq < hi);
     const bool in1 = !edge || (key + gq + 8 >= lo && key + gq + 8 < hi);
-    uint32_t pb[NQ][2], pl[NQ][2];  // the weights in bf16, and what that left
+    uint32_t pb[PP][NQ][2];  // the weights in bf16, and what that left
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
       float x[4];
@@ -309,18 +322,18 @@ __global__ void __launch_bounds__(kWarps * 32)
       }
       const float ref0 = m[c][0] == -INFINITY ? 0.f : m[c][0];
       const float ref1 = m[c][1] == -INFINITY ? 0.f : m[c][1];
-      const float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
-      const float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
+      float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
+      float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
       l[c][0] += p0 + p2;
       l[c][1] += p1 + p3;
-      // The weights take part in bf16, what that rounding leaves as a second
-      // product: there is time for it.
-      const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
-      const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
-      pb[c][0] = transpose8x8(h0);
-      pb[c][1] = transpose8x8(h1);
-      pl[c][0] = transpose8x8(pack_bf16(p0 - f0.x, p1 - f0.y));
-      pl[c][1] = transpose8x8(pack_bf16(p2 - f1.x, p3 - f1.y));
+#pragma unroll
+      for (int w = 0; w < PP; ++w) {
+        const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
+        pb[w][c][0] = transpose8x8(h0);
+        pb[w][c][1] = transpose8x8(h1);
+        const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
+        p0 -= f0.x, p1 -= f0.y, p2 -= f1.x, p3 -= f1.y;
+      }
     }
     // V rows of masked keys may hold anything, and 0 * NaN is NaN.
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -339,10 +352,9 @@ __global__ void __launch_bounds__(kWarps * 32)
       a[2] &= keep1;
       a[3] &= keep1;
 #pragma unroll
-      for (int c = 0; c < NQ; ++c) {
-        mma16816(o[c][i], a, pb[c][0], pb[c][1]);
-        mma16816(o[c][i], a, pl[c][0], pl[c][1]);
-      }
+      for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int w = 0; w < PP; ++w) mma16816(o[c][i], a, pb[w][c][0], pb[w][c][1]);
     }
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue(issued++);
@@ -484,8 +496,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-template <int DP, int NQ, bool PREFIX>
-int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
+template <int DP, int NQ, bool PREFIX, int QP>
+int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
            cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(PREFIX ? p.np : p.B * p.own_splits) * p.row_chunks * p.Hkv;
@@ -504,7 +516,7 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
   rc = encode_tensor_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.v, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != B200_OK) return rc;
-  auto kern = shared_own_mma_kernel<DP, NQ, PREFIX>;
+  auto kern = shared_own_mma_kernel<DP, NQ, PREFIX, QP>;
   static std::atomic<int> configured[64];
   if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -512,6 +524,25 @@ int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& de
     if (dev.device < 64) configured[dev.device].store(1, std::memory_order_release);
   }
   return launch_own(kern, grid, kWarps * 32, smem, stream, overlap, tk, tv, op);
+}
+
+// 16 rows at a time for bf16 queries alone: pieces take registers.
+template <bool PREFIX>
+int launch(const OwnParams& op, const b200_kv_pool_t& pool, bool wide, const DeviceInfo& dev, bool overlap,
+           cudaStream_t stream) {
+  const bool d64 = op.s.D <= 64;
+  if (op.s.q_dtype == B200_DTYPE_F16)
+    return d64 ? launch_one<64, 1, PREFIX, 2>(op, pool, dev, overlap, stream)
+               : launch_one<128, 1, PREFIX, 2>(op, pool, dev, overlap, stream);
+  if (op.s.q_dtype == B200_DTYPE_F32)
+    return d64 ? launch_one<64, 1, PREFIX, 3>(op, pool, dev, overlap, stream)
+               : launch_one<128, 1, PREFIX, 3>(op, pool, dev, overlap, stream);
+  if constexpr (!PREFIX)
+    if (wide)
+      return d64 ? launch_one<64, 2, PREFIX, 1>(op, pool, dev, overlap, stream)
+                 : launch_one<128, 2, PREFIX, 1>(op, pool, dev, overlap, stream);
+  return d64 ? launch_one<64, 1, PREFIX, 1>(op, pool, dev, overlap, stream)
+             : launch_one<128, 1, PREFIX, 1>(op, pool, dev, overlap, stream);
 }
 
 bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
@@ -532,20 +563,14 @@ OwnParams own_params(const SharedParams& p, int zero_count) {
 
 }  // namespace
 
-int shared_own_rows(int64_t rep) { return rep <= 8 ? 8 : 16; }
+int shared_own_rows(int64_t rep, int q_dtype) { return rep <= 8 || q_dtype != B200_DTYPE_BF16 ? 8 : 16; }
 
 int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
                           cudaStream_t stream) {
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc != B200_OK) return rc;
-  const OwnParams op = own_params(p, 0);
-  const bool wide = shared_own_rows(p.rep) == 16;
-  if (p.D <= 64)
-    return wide ? launch<64, 2, false>(op, pool, dev, overlap, stream)
-                : launch<64, 1, false>(op, pool, dev, overlap, stream);
-  return wide ? launch<128, 2, false>(op, pool, dev, overlap, stream)
-              : launch<128, 1, false>(op, pool, dev, overlap, stream);
+  return launch<false>(own_params(p, 0), pool, shared_own_rows(p.rep, p.q_dtype) == 16, dev, overlap, stream);
 }
 
 int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
@@ -555,8 +580,7 @@ int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, 
   if (rc != B200_OK) return rc;
   OwnParams op = own_params(p, zero_count);
   op.s.row_chunks = static_cast<int32_t>(ceil_div(p.rows, 8));
-  if (p.D <= 64) return launch<64, 1, true>(op, pool, dev, false, stream);
-  return launch<128, 1, true>(op, pool, dev, false, stream);
+  return launch<true>(op, pool, false, dev, false, stream);
 }
 
 }  // namespace b200

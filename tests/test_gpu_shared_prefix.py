@@ -24,8 +24,8 @@ def _check(cpu, tensor_cores=None, **kw):
     out = _run(c, status=status, **kw)
     torch.cuda.synchronize()
     assert int(status) == 0
-    if tensor_cores is None:  # weights in bf16 where everything is
-        tensor_cores = cpu.q.dtype == cpu.pool.k.dtype == BF16
+    if tensor_cores is None:  # weights in bf16 where everything is, in two pieces for f16
+        tensor_cores = cpu.pool.k.dtype == BF16 and {BF16: True, F16: "split", F32: False}[cpu.q.dtype]
     assert_close(cpu, out, tensor_cores=tensor_cores)
     return c, out
 
@@ -75,6 +75,26 @@ TILES = [
 @pytest.mark.parametrize("size", TILES, ids=lambda s: str(s[:6]))
 def test_shared_prefix_tiles(size):
     _check(case(*size, seed=size[0]))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("size", [TILES[1], TILES[3], (33, 64, 4, 128, 16, 9001, [40 * i for i in range(33)]),
+                                  (2, 8, 1, 128, 64, 40000, [0, 150])], ids=lambda s: str(s[:6]))
+def test_other_queries_of_a_bf16_pool(size, dtype):
+    """f16 and f32 queries meet a bf16 pool in exact pieces, whatever the sizes;
+    three f32 pieces keep what f32 sums keep."""
+    _check(case(*size, dtype, BF16, seed=50))
+
+
+def test_queries_of_all_their_bits_against_one_key():
+    """One key, so that the output is its value whatever the score; and two keys
+    whose weights follow from a difference that only the last pieces show."""
+    cpu = case(1, 8, 1, 64, 16, 0, [2], F32, BF16, seed=51)
+    k = torch.zeros(2, 64)
+    k[0, 0], k[1, 0], k[1, 1] = 1.0, 1.0, 1.0
+    cpu.pool.k[0, cpu.tables[0, 0], :2, 0] = k.to(BF16)
+    cpu.q[..., 1] = torch.tensor([1.0 + 2.0 ** -23 * (2 * i + 1) for i in range(8)]) * 8
+    _check(cpu)
 
 
 # A small and a large size for the tests below.
