@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(128) shared_prefix_elem_kernel(const __grid_co
 // Own keys and the join: CTA ((sequence, key head, chunk of 8 rows), part).
 template <typename KV, int DP>
 __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_constant__ SharedParams p) {
-  constexpr int R = 8;
+  constexpr int R = kOwnRows;
   extern __shared__ float4 sm4[];
   float* sm = reinterpret_cast<float*>(sm4);
   __shared__ int last;
@@ -357,9 +357,8 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
   // (4 sequences of 8 x 4 heads over 2048 keys: 10 us against 15; over 32768: 32
   // against 43; 1 of 32 x 1: 83 against 116).  Above, it is as long as little is
   // read: 64 rows to each of 8 heads, 1024 keys 13 us against 17, 2048 the same,
-  // 8192 30 against 23.  (16 rows at a time by the wide form of the kernel, whose
-  // longer code has to be fetched first: 12 us where two times eight take 8.)
-  const int64_t eights = ceil_div(rows, 8) * Hkv;
+  // 8192 30 against 23.
+  const int64_t eights = ceil_div(rows, kOwnRows) * Hkv;
   pl.few = mma && prefix > 0 &&
            (q_dtype != B200_DTYPE_BF16 || rows <= 16 || eights * prefix < (int64_t(1) << 17));
   pl.tc = mma && prefix > 0 && !pl.few;
@@ -390,7 +389,7 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   }
   // Own keys: enough parts to fill the GPU, none much longer than 1024 keys.
-  pl.row_chunks = static_cast<int>(ceil_div(rep, mma ? shared_own_rows(rep, q_dtype) : 8));
+  pl.row_chunks = static_cast<int>(ceil_div(rep, kOwnRows));
   pl.own_min = mma ? 128 : 64;
   const int64_t units = B * Hkv * pl.row_chunks;
   int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));

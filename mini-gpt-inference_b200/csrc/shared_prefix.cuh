@@ -47,11 +47,14 @@ struct SharedParams {
   float qscale;  // log2(e) / sqrt(D)
 };
 
-// Own keys and join, bf16 pool; the rows of a key head one CTA
-// takes.  `overlap`: the kernel ahead on the stream is the prefix's.
+// Own keys and join, bf16 pool, kOwnRows rows of a key head to a CTA.  (16 rows
+// take twice the registers and a longer code that has to be fetched first: 16
+// query heads to each of 4 key heads, 64 sequences behind 4096 keys 45 us, two
+// CTAs of eight rows 37 us.)  `overlap`: the kernel ahead on the stream is the
+// prefix's.
+constexpr int kOwnRows = 8;
 int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
                           cudaStream_t stream);
-int shared_own_rows(int64_t rep, int q_dtype);
 // The prefix's parts, eight rows at a time.
 int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
                              cudaStream_t stream);

@@ -80,7 +80,7 @@ struct OwnParams {
   int32_t zero_count;      // PREFIX: counters to clear
 };
 
-template <int DP, int NQ>
+template <int DP>
 struct OwnSmem {
   static constexpr int HALVES = DP / 64;
   static constexpr int HALF = kStep * 128;        // 16 keys x 64 d
@@ -88,7 +88,7 @@ struct OwnSmem {
   static constexpr int STAGE = 2 * TILE;
   static constexpr int STAGES = DP == 128 ? 2 : 4;
   static constexpr int RING = kWarps * STAGES * STAGE;
-  static constexpr int R = 8 * NQ;
+  static constexpr int R = kOwnRows;
   static constexpr int LD = DP + 4;               // 2 LD = 8 mod 32: no bank is hit twice
   static constexpr int MERGE = kWarps * R * LD * 4;  // the warps' O, over the ring
   static constexpr int BAR = RING > MERGE ? RING : MERGE;
@@ -97,17 +97,17 @@ struct OwnSmem {
   static_assert(RING % 1024 == 0 && STAGE % 1024 == 0, "swizzled tiles start on 1024 bytes");
 };
 
-// NQ groups of 8 query rows; DP: head dimension rounded up to 64 or 128.
+// DP: head dimension rounded up to 64 or 128.
 // PREFIX: the keys are a part of the prefix's, the rows all sequences'.
 // QP: bf16 pieces that a query element is the exact sum of: 1 for bf16, 2 for
 // f16 (11 bits), 3 for f32 (24 bits).  A piece is another product, and there is
 // time for them.  The weights take part in as many pieces, and at least in two:
 // what is left of them is 2^-16, with three 2^-24.
-template <int DP, int NQ, bool PREFIX, int QP>
+template <int DP, bool PREFIX, int QP>
 __global__ void __launch_bounds__(kWarps * 32)
     shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const __grid_constant__ OwnParams op) {
-  using L = OwnSmem<DP, NQ>;
+  using L = OwnSmem<DP>;
   constexpr int NS = L::STAGES, R = L::R, PP = QP == 3 ? 3 : 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -211,48 +211,41 @@ __global__ void __launch_bounds__(kWarps * 32)
   int issued = min(mine, NS);
   for (int n = 0; n < issued; ++n) issue(n);
 
-  // Query fragments: row 8n + gq, d = 16 i + 2t + {0, 1} and + 8.
-  uint32_t qf[QP][NQ][DP / 16][2];
+  // Query fragments: row gq, d = 16 i + 2t + {0, 1} and + 8.
+  uint32_t qf[QP][DP / 16][2];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
+  for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
+    for (int u = 0; u < 2; ++u) {
+      const int r = gq, d = 16 * i + 2 * t + 8 * u;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = 8 * n + gq, d = 16 * i + 2 * t + 8 * u;
+      for (int c = 0; c < QP; ++c) qf[c][i][u] = 0;
+      if (r < nrows && d < p.D) {
+        const int seq = PREFIX ? (row0 + r) / p.rep : b;
+        const int head = PREFIX ? g * p.rep + (row0 + r) - seq * p.rep : head0 + r;
+        const int64_t at = seq * p.qs0 + head * p.qs1 + d * p.qs2;
+        if (QP == 1 && op.q_vec) {
+          qf[0][i][u] = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
+        } else {
+          constexpr int type = QP == 1 ? B200_DTYPE_BF16 : QP == 2 ? B200_DTYPE_F16 : B200_DTYPE_F32;
+          float x = load_elem(p.q, at, type), y = load_elem(p.q, at + p.qs2, type);
 #pragma unroll
-        for (int c = 0; c < QP; ++c) qf[c][n][i][u] = 0;
-        if (r < nrows && d < p.D) {
-          const int seq = PREFIX ? (row0 + r) / p.rep : b;
-          const int head = PREFIX ? g * p.rep + (row0 + r) - seq * p.rep : head0 + r;
-          const int64_t at = seq * p.qs0 + head * p.qs1 + d * p.qs2;
-          if (QP == 1 && op.q_vec) {
-            qf[0][n][i][u] = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
-          } else {
-            constexpr int type = QP == 1 ? B200_DTYPE_BF16 : QP == 2 ? B200_DTYPE_F16 : B200_DTYPE_F32;
-            float x = load_elem(p.q, at, type), y = load_elem(p.q, at + p.qs2, type);
-#pragma unroll
-            for (int c = 0; c < QP; ++c) {
-              qf[c][n][i][u] = pack_bf16(x, y);
-              const float2 f = bf16x2_to_float2(qf[c][n][i][u]);
-              x -= f.x, y -= f.y;
-            }
+          for (int c = 0; c < QP; ++c) {
+            qf[c][i][u] = pack_bf16(x, y);
+            const float2 f = bf16x2_to_float2(qf[c][i][u]);
+            x -= f.x, y -= f.y;
           }
         }
       }
+    }
 
-  // Row 8n + 2t + u: m[n][u] (the same in its 8 lanes) and this lane's l;
-  // o[n][i]: d = 16 i + gq (+ 8) of rows 2t, 2t + 1.
-  float m[NQ][2], l[NQ][2], o[NQ][DP / 16][4];
+  // Row 2t + u: m[u] (the same in its 8 lanes) and this lane's l;
+  // o[i]: d = 16 i + gq (+ 8) of rows 2t, 2t + 1.
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DP / 16][4];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
+  for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
-  }
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   // Byte offsets of this lane's ldmatrix row and its chunk's swizzle.  K: keys
   // (lane & 15), chunks 2 i + (lane >> 4); V: keys (lane & 7) + 8 (lane >> 4),
   // chunks 2 i + (lane >> 3 & 1).
@@ -268,72 +261,65 @@ __global__ void __launch_bounds__(kWarps * 32)
       break;
     }
     const uint32_t kt = smem_u32(ring + st * L::STAGE), vt = kt + L::TILE;
-    float s[NQ][2][4];  // two chains of products
+    float s[2][4];  // two chains of products
 #pragma unroll
-    for (int c = 0; c < NQ; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[c][e >> 2][e & 3] = 0.f;
+    for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = 0.f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       uint32_t a[4];
       const uint32_t ch = (2 * i + k_hi) & 7;
       ldmatrix4(a, kt + (i / 4) * L::HALF + k_row + ((ch ^ sw) << 4));
 #pragma unroll
-      for (int c = 0; c < NQ; ++c)
-#pragma unroll
-        for (int w = 0; w < QP; ++w) mma16816(s[c][i & 1], a, qf[w][c][i][0], qf[w][c][i][1]);
+      for (int w = 0; w < QP; ++w) mma16816(s[i & 1], a, qf[w][i][0], qf[w][i][1]);
     }
     const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * n) * kStep;
     const bool edge = key < lo || key + kStep > hi;
     const bool in0 = !edge || (key + gq >= lo && key + gq < hi);
     const bool in1 = !edge || (key + gq + 8 >= lo && key + gq + 8 < hi);
-    uint32_t pb[PP][NQ][2];  // the weights in bf16, and what that left
+    uint32_t pb[PP][2];  // the weights in bf16, and what that left
+    float x[4];
 #pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-      float x[4];
+    for (int e = 0; e < 4; ++e)
+      x[e] = (e < 2 ? in0 : in1) ? (s[0][e] + s[1][e]) * p.qscale : -INFINITY;
+    const float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+    // The reference point moves only when a score exceeds it by more than
+    // 2^8: weights stay below 2^8 and l and o stay exact relative to it.
+    if (__any_sync(0xffffffffu, mx0 > m[0] + 8.f || mx1 > m[1] + 8.f)) {
+      float r0 = mx0, r1 = mx1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[e] = (e < 2 ? in0 : in1) ? (s[c][0][e] + s[c][1][e]) * p.qscale : -INFINITY;
-      const float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
-      // The reference point moves only when a score exceeds it by more than
-      // 2^8: weights stay below 2^8 and l and o stay exact relative to it.
-      if (__any_sync(0xffffffffu, mx0 > m[c][0] + 8.f || mx1 > m[c][1] + 8.f)) {
-        float r0 = mx0, r1 = mx1;
-#pragma unroll
-        for (int w = 4; w <= 16; w <<= 1) {
-          r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, w));
-          r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, w));
-        }
-        r0 = fmaxf(m[c][0], r0);
-        r1 = fmaxf(m[c][1], r1);
-        const float a0 = m[c][0] == -INFINITY ? 0.f : ex2(m[c][0] - r0);
-        const float a1 = m[c][1] == -INFINITY ? 0.f : ex2(m[c][1] - r1);
-        m[c][0] = r0;
-        m[c][1] = r1;
-        l[c][0] *= a0;
-        l[c][1] *= a1;
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          o[c][i][0] *= a0;
-          o[c][i][1] *= a1;
-          o[c][i][2] *= a0;
-          o[c][i][3] *= a1;
-        }
+      for (int w = 4; w <= 16; w <<= 1) {
+        r0 = fmaxf(r0, __shfl_xor_sync(0xffffffffu, r0, w));
+        r1 = fmaxf(r1, __shfl_xor_sync(0xffffffffu, r1, w));
       }
-      const float ref0 = m[c][0] == -INFINITY ? 0.f : m[c][0];
-      const float ref1 = m[c][1] == -INFINITY ? 0.f : m[c][1];
-      float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
-      float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
-      l[c][0] += p0 + p2;
-      l[c][1] += p1 + p3;
+      r0 = fmaxf(m[0], r0);
+      r1 = fmaxf(m[1], r1);
+      const float a0 = m[0] == -INFINITY ? 0.f : ex2(m[0] - r0);
+      const float a1 = m[1] == -INFINITY ? 0.f : ex2(m[1] - r1);
+      m[0] = r0;
+      m[1] = r1;
+      l[0] *= a0;
+      l[1] *= a1;
 #pragma unroll
-      for (int w = 0; w < PP; ++w) {
-        const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
-        pb[w][c][0] = transpose8x8(h0);
-        pb[w][c][1] = transpose8x8(h1);
-        const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
-        p0 -= f0.x, p1 -= f0.y, p2 -= f1.x, p3 -= f1.y;
+      for (int i = 0; i < DP / 16; ++i) {
+        o[i][0] *= a0;
+        o[i][1] *= a1;
+        o[i][2] *= a0;
+        o[i][3] *= a1;
       }
+    }
+    const float ref0 = m[0] == -INFINITY ? 0.f : m[0];
+    const float ref1 = m[1] == -INFINITY ? 0.f : m[1];
+    float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
+    float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
+    l[0] += p0 + p2;
+    l[1] += p1 + p3;
+#pragma unroll
+    for (int w = 0; w < PP; ++w) {
+      const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
+      pb[w][0] = transpose8x8(h0);
+      pb[w][1] = transpose8x8(h1);
+      const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
+      p0 -= f0.x, p1 -= f0.y, p2 -= f1.x, p3 -= f1.y;
     }
     // V rows of masked keys may hold anything, and 0 * NaN is NaN.
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -352,9 +338,7 @@ __global__ void __launch_bounds__(kWarps * 32)
       a[2] &= keep1;
       a[3] &= keep1;
 #pragma unroll
-      for (int c = 0; c < NQ; ++c)
-#pragma unroll
-        for (int w = 0; w < PP; ++w) mma16816(o[c][i], a, pb[w][c][0], pb[w][c][1]);
+      for (int w = 0; w < PP; ++w) mma16816(o[i], a, pb[w][0], pb[w][1]);
     }
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue(issued++);
@@ -370,19 +354,17 @@ __global__ void __launch_bounds__(kWarps * 32)
   float2* s_ml = reinterpret_cast<float2*>(smem + L::ML);
   int* s_last = reinterpret_cast<int*>(smem + L::ML + kMaxSlots * R * 8);
 #pragma unroll
-  for (int c = 0; c < NQ; ++c)
+  for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int w = 4; w <= 16; w <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], w);
+    const int r = 2 * t + u;
+    if (gq == 0) s_ml[warp * R + r] = make_float2(m[u], l[u]);
 #pragma unroll
-      for (int w = 4; w <= 16; w <<= 1) l[c][u] += __shfl_xor_sync(0xffffffffu, l[c][u], w);
-      const int r = 8 * c + 2 * t + u;
-      if (gq == 0) s_ml[warp * R + r] = make_float2(m[c][u], l[c][u]);
-#pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        s_o[(warp * R + r) * L::LD + 16 * i + gq] = o[c][i][u];
-        s_o[(warp * R + r) * L::LD + 16 * i + gq + 8] = o[c][i][u + 2];
-      }
+    for (int i = 0; i < DP / 16; ++i) {
+      s_o[(warp * R + r) * L::LD + 16 * i + gq] = o[i][u];
+      s_o[(warp * R + r) * L::LD + 16 * i + gq + 8] = o[i][u + 2];
     }
+  }
   __syncthreads();
 
   // Nothing so far, nor this part's way to its slot, comes from the prefix's
@@ -496,14 +478,14 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-template <int DP, int NQ, bool PREFIX, int QP>
+template <int DP, bool PREFIX, int QP>
 int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
            cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(PREFIX ? p.np : p.B * p.own_splits) * p.row_chunks * p.Hkv;
   if (p.np + p.own_splits + kWarps > kMaxSlots)
     return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
-  const int smem = OwnSmem<DP, NQ>::BYTES + 1024;
+  const int smem = OwnSmem<DP>::BYTES + 1024;
   CUtensorMap tk, tv;
   const uint64_t dims[3] = {static_cast<uint64_t>(pool.head_dim), static_cast<uint64_t>(pool.num_heads),
                             static_cast<uint64_t>(pool.num_layers * pool.num_blocks * pool.block_size)};
@@ -516,7 +498,7 @@ int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo
   rc = encode_tensor_map(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, pool.v, dims, strides, box,
                          CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != B200_OK) return rc;
-  auto kern = shared_own_mma_kernel<DP, NQ, PREFIX, QP>;
+  auto kern = shared_own_mma_kernel<DP, PREFIX, QP>;
   static std::atomic<int> configured[64];
   if (dev.device >= 64 || !configured[dev.device].load(std::memory_order_acquire)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -526,23 +508,18 @@ int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo
   return launch_own(kern, grid, kWarps * 32, smem, stream, overlap, tk, tv, op);
 }
 
-// 16 rows at a time for bf16 queries alone: pieces take registers.
 template <bool PREFIX>
-int launch(const OwnParams& op, const b200_kv_pool_t& pool, bool wide, const DeviceInfo& dev, bool overlap,
+int launch(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo& dev, bool overlap,
            cudaStream_t stream) {
   const bool d64 = op.s.D <= 64;
   if (op.s.q_dtype == B200_DTYPE_F16)
-    return d64 ? launch_one<64, 1, PREFIX, 2>(op, pool, dev, overlap, stream)
-               : launch_one<128, 1, PREFIX, 2>(op, pool, dev, overlap, stream);
+    return d64 ? launch_one<64, PREFIX, 2>(op, pool, dev, overlap, stream)
+               : launch_one<128, PREFIX, 2>(op, pool, dev, overlap, stream);
   if (op.s.q_dtype == B200_DTYPE_F32)
-    return d64 ? launch_one<64, 1, PREFIX, 3>(op, pool, dev, overlap, stream)
-               : launch_one<128, 1, PREFIX, 3>(op, pool, dev, overlap, stream);
-  if constexpr (!PREFIX)
-    if (wide)
-      return d64 ? launch_one<64, 2, PREFIX, 1>(op, pool, dev, overlap, stream)
-                 : launch_one<128, 2, PREFIX, 1>(op, pool, dev, overlap, stream);
-  return d64 ? launch_one<64, 1, PREFIX, 1>(op, pool, dev, overlap, stream)
-             : launch_one<128, 1, PREFIX, 1>(op, pool, dev, overlap, stream);
+    return d64 ? launch_one<64, PREFIX, 3>(op, pool, dev, overlap, stream)
+               : launch_one<128, PREFIX, 3>(op, pool, dev, overlap, stream);
+  return d64 ? launch_one<64, PREFIX, 1>(op, pool, dev, overlap, stream)
+             : launch_one<128, PREFIX, 1>(op, pool, dev, overlap, stream);
 }
 
 bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int bytes) {
@@ -563,14 +540,12 @@ OwnParams own_params(const SharedParams& p, int zero_count) {
 
 }  // namespace
 
-int shared_own_rows(int64_t rep, int q_dtype) { return rep <= 8 || q_dtype != B200_DTYPE_BF16 ? 8 : 16; }
-
 int launch_shared_own_mma(const SharedParams& p, const b200_kv_pool_t& pool, bool overlap,
                           cudaStream_t stream) {
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc != B200_OK) return rc;
-  return launch<false>(own_params(p, 0), pool, shared_own_rows(p.rep, p.q_dtype) == 16, dev, overlap, stream);
+  return launch<false>(own_params(p, 0), pool, dev, overlap, stream);
 }
 
 int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, int zero_count,
@@ -579,8 +554,8 @@ int launch_shared_prefix_mma(const SharedParams& p, const b200_kv_pool_t& pool, 
   int rc = current_device_info(&dev);
   if (rc != B200_OK) return rc;
   OwnParams op = own_params(p, zero_count);
-  op.s.row_chunks = static_cast<int32_t>(ceil_div(p.rows, 8));
-  return launch<true>(op, pool, false, dev, false, stream);
+  op.s.row_chunks = static_cast<int32_t>(ceil_div(p.rows, kOwnRows));
+  return launch<true>(op, pool, dev, false, stream);
 }
 
 }  // namespace b200
