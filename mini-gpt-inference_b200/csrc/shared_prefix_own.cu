@@ -12,14 +12,18 @@
 //
 // What bounds it is the bytes in flight: a row of one head is 256 bytes in a
 // place of its own.  Each of the four warps takes every fourth step of 16
-// keys, has its own ring of two stages (K and V of a step, 8 KB at D = 128)
-// filled by TMA page by page, and needs no other warp until the end.  Three
-// CTAs fit an SM, so that one's beginning and join pass beside the others'
-// loads.  64 sequences of 32 heads with up to 1024 own keys (537 MB): 87 us,
-// 6.2 TB/s; with three stages, and two CTAs, 95 us; with the operands loaded
-// straight into registers, one step a warp, 213 us.  f16 and f32 queries cost
-// little more, and far less than f32 arithmetic: 64 sequences of 8 x 4 heads behind
-// 4096 keys 84 and 90 us (element kernels 219), 4 behind 32768 42 and 46 (185).
+// keys, has its own ring of three entries (K of a step, its V, K of the next: 4
+// KB each at D = 128) filled by TMA page by page, and needs no other warp until
+// the end.  Four CTAs fit an SM, so that one's beginning and join, 6 us for a
+// few keys, pass beside the others' loads.  64 sequences of 32 heads with up to
+// 1024 own keys (537 MB): 90 us, 6.1 TB/s; 256 of up to 64 keys, behind 256, 99
+// us in all.  With entries of K and V, two to a warp, and three CTAs 89 and 116
+// us; with three of them, and two CTAs, the first 95 us; with the operands loaded
+// straight into registers, one step a warp, 213 us.  (The prefix's parts, which
+// are long and few, keep the larger entries: a wait less in each step.)  f16 and
+// f32 queries cost little more, and far less than f32 arithmetic: 64 sequences of
+// 8 x 4 heads behind 4096 keys 80 and 90 us (element kernels 219), 4 behind 32768
+// 42 and 45 (185).
 #include <algorithm>
 #include <atomic>
 
@@ -80,21 +84,24 @@ struct OwnParams {
   int32_t zero_count;      // PREFIX: counters to clear
 };
 
-template <int DP>
+template <int DP, bool PREFIX, int QP>
 struct OwnSmem {
   static constexpr int HALVES = DP / 64;
   static constexpr int HALF = kStep * 128;        // 16 keys x 64 d
   static constexpr int TILE = HALVES * HALF;      // K or V of a step
-  static constexpr int STAGE = 2 * TILE;
-  static constexpr int STAGES = DP == 128 ? 2 : 4;
-  static constexpr int RING = kWarps * STAGES * STAGE;
+  // Ring entries: K or V of a step where three of them leave room for four CTAs on
+  // an SM (own keys, where registers do too), else both, twice (see above).
+  static constexpr bool SPLIT = !PREFIX && QP <= 2;
+  static constexpr int ENTRY = SPLIT ? TILE : 2 * TILE;
+  static constexpr int ENTRIES = (SPLIT ? 3 : 2) * (DP == 128 ? 1 : 2);
+  static constexpr int RING = kWarps * ENTRIES * ENTRY;
   static constexpr int R = kOwnRows;
   static constexpr int LD = DP + 4;               // 2 LD = 8 mod 32: no bank is hit twice
   static constexpr int MERGE = kWarps * R * LD * 4;  // the warps' O, over the ring
   static constexpr int BAR = RING > MERGE ? RING : MERGE;
-  static constexpr int ML = BAR + kWarps * STAGES * 8;  // float2 [kMaxSlots][R]
+  static constexpr int ML = BAR + kWarps * ENTRIES * 8;  // float2 [kMaxSlots][R]
   static constexpr int BYTES = ML + kMaxSlots * R * 8 + 16;
-  static_assert(RING % 1024 == 0 && STAGE % 1024 == 0, "swizzled tiles start on 1024 bytes");
+  static_assert(TILE % 1024 == 0, "swizzled tiles start on 1024 bytes");
 };
 
 // DP: head dimension rounded up to 64 or 128.
@@ -107,8 +114,8 @@ template <int DP, bool PREFIX, int QP>
 __global__ void __launch_bounds__(kWarps * 32)
     shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
                           const __grid_constant__ CUtensorMap tmv, const __grid_constant__ OwnParams op) {
-  using L = OwnSmem<DP>;
-  constexpr int NS = L::STAGES, R = L::R, PP = QP == 3 ? 3 : 2;
+  using L = OwnSmem<DP, PREFIX, QP>;
+  constexpr int NS = L::ENTRIES, R = L::R, PP = QP == 3 ? 3 : 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const SharedParams& p = op.s;
@@ -165,7 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int mine = (steps - warp + kWarps - 1) / kWarps;  // of this warp: warp, warp + 4, ...
 
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR) + warp * NS;
-  uint8_t* ring = smem + warp * (NS * L::STAGE);
+  uint8_t* ring = smem + warp * (NS * L::ENTRY);
   if (lane < NS) mbar_init(&full[lane], 1);
   fence_mbar_init();
   __syncwarp();
@@ -189,26 +196,30 @@ __global__ void __launch_bounds__(kWarps * 32)
   int rows = lookup(0);
   int rows_next = mine > per_batch ? lookup(per_batch) : -1;
   int batch = 0;
-  auto issue = [&](int n) {
+  constexpr bool split_kv = L::SPLIT;
+  auto issue = [&](int e) {  // entry e: K (even) or V of step e / 2, or step e
+    const int n = split_kv ? e >> 1 : e, st = e % NS;
     if (n >= batch + per_batch) {
       batch += per_batch;
       rows = rows_next;
       rows_next = batch + per_batch < mine ? lookup(batch + per_batch) : -1;
     }
-    const int st = n % NS;
-    // Lane: box, half, K or V.
-    const int box = lane % nb, rest = lane / nb;
-    const int half = rest % L::HALVES, kv = rest / L::HALVES;
+    const int box = lane % nb, rest = lane / nb;  // of this lane
+    const int half = rest % L::HALVES, kv = split_kv ? e & 1 : rest / L::HALVES;
     const int row = __shfl_sync(0xffffffffu, rows, (n - batch) * nb + box);
     const unsigned there = __ballot_sync(0xffffffffu, lane < nb && row >= 0);
     if (lane == 0)
-      mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(__popc(there) * 2 * L::HALVES * op.rbox * 128));
+      mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(__popc(there) * (L::ENTRY / L::HALF) * op.rbox * 128));
     __syncwarp();
-    if (kv < 2 && row >= 0)
-      tma_load_3d(ring + st * L::STAGE + kv * L::TILE + half * L::HALF + box * op.rbox * 128,
-                  kv == 0 ? &tmk : &tmv, &full[st], half * 64, g, row);
+    if (rest < L::ENTRY / L::HALF && row >= 0)
+      tma_load_3d(ring + st * L::ENTRY + rest * L::HALF + box * op.rbox * 128, kv == 0 ? &tmk : &tmv, &full[st],
+                  half * 64, g, row);
   };
-  int issued = min(mine, NS);
+  auto arrived = [&](int e) {
+    return __all_sync(0xffffffffu, mbar_wait(&full[e % NS], static_cast<uint32_t>(e / NS) & 1u)) != 0;
+  };
+  const int entries = split_kv ? 2 * mine : mine;
+  int issued = min(entries, NS);
   for (int n = 0; n < issued; ++n) issue(n);
 
   // Query fragments: row gq, d = 16 i + 2t + {0, 1} and + 8.
@@ -255,12 +266,11 @@ __global__ void __launch_bounds__(kWarps * 32)
 
   bool ok = true;
   for (int n = 0; n < mine; ++n) {
-    const int st = n % NS;
-    if (!__all_sync(0xffffffffu, mbar_wait(&full[st], static_cast<uint32_t>(n / NS) & 1u))) {
-      ok = false;
-      break;
-    }
-    const uint32_t kt = smem_u32(ring + st * L::STAGE), vt = kt + L::TILE;
+    const int e = split_kv ? 2 * n : n;
+    ok = arrived(e);
+    if (!ok) break;
+    const uint32_t kt = smem_u32(ring + e % NS * L::ENTRY);
+    const uint32_t vt = split_kv ? smem_u32(ring + (e + 1) % NS * L::ENTRY) : kt + L::TILE;
     float s[2][4];  // two chains of products
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e >> 2][e & 3] = 0.f;
@@ -271,6 +281,10 @@ __global__ void __launch_bounds__(kWarps * 32)
       ldmatrix4(a, kt + (i / 4) * L::HALF + k_row + ((ch ^ sw) << 4));
 #pragma unroll
       for (int w = 0; w < QP; ++w) mma16816(s[i & 1], a, qf[w][i][0], qf[w][i][1]);
+    }
+    if constexpr (split_kv) {
+      __syncwarp();  // every lane has read K
+      if (issued < entries) issue(issued++);
     }
     const int64_t key = k0 + static_cast<int64_t>(warp + kWarps * n) * kStep;
     const bool edge = key < lo || key + kStep > hi;
@@ -328,6 +342,10 @@ __global__ void __launch_bounds__(kWarps * 32)
       keep0 = (in(2 * t) ? 0xffffu : 0u) | (in(2 * t + 1) ? 0xffff0000u : 0u);
       keep1 = (in(2 * t + 8) ? 0xffffu : 0u) | (in(2 * t + 9) ? 0xffff0000u : 0u);
     }
+    if constexpr (split_kv) {
+      ok = arrived(e + 1);
+      if (!ok) break;
+    }
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       uint32_t a[4];
@@ -340,12 +358,12 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
       for (int w = 0; w < PP; ++w) mma16816(o[i], a, pb[w][0], pb[w][1]);
     }
-    __syncwarp();  // every lane has read the stage
-    if (issued < mine) issue(issued++);
+    __syncwarp();  // every lane has read V, or both
+    if (issued < entries) issue(issued++);
   }
   if (!ok) {
     if (lane == 0) report(p.status, B200_DEV_WAIT_TIMEOUT);
-    for (int n = max(0, issued - NS); n < issued; ++n) mbar_wait(&full[n % NS], static_cast<uint32_t>(n / NS) & 1u);
+    for (int e = max(0, issued - NS); e < issued; ++e) mbar_wait(&full[e % NS], static_cast<uint32_t>(e / NS) & 1u);
   }
 
   // Whole sums of the rows' weights; the warps' states meet in shared memory.
@@ -485,7 +503,7 @@ int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo
   const int64_t grid = static_cast<int64_t>(PREFIX ? p.np : p.B * p.own_splits) * p.row_chunks * p.Hkv;
   if (p.np + p.own_splits + kWarps > kMaxSlots)
     return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
-  const int smem = OwnSmem<DP>::BYTES + 1024;
+  const int smem = OwnSmem<DP, PREFIX, QP>::BYTES + 1024;
   CUtensorMap tk, tv;
   const uint64_t dims[3] = {static_cast<uint64_t>(pool.head_dim), static_cast<uint64_t>(pool.num_heads),
                             static_cast<uint64_t>(pool.num_layers * pool.num_blocks * pool.block_size)};
