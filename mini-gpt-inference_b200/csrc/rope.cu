@@ -56,18 +56,22 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
   return d;
 }
 
-// One 16-byte chunk of the input type: N elements, as N / 2 pairs of floats.
-template <typename T>
+// One chunk (16 or 8 bytes) of the input type: N elements, as N / 2 pairs of floats.
+template <typename T, int BYTES>
 struct Chunk {
-  static constexpr int N = 16 / sizeof(T);
-  __device__ __forceinline__ static void unpack(const uint4& c, float2* f) {
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  static constexpr int N = BYTES / sizeof(T);
+  using Raw = std::conditional_t<BYTES == 16, uint4, uint2>;
+  __device__ __forceinline__ static void unpack(const Raw& c, float2* f) {
+    uint32_t w[BYTES / 4];
+    w[0] = c.x, w[1] = c.y;
+    if constexpr (BYTES == 16) w[2] = c.z, w[3] = c.w;
     if constexpr (sizeof(T) == 4) {
-      f[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
-      f[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        f[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < N / 2; ++i) {
         if constexpr (std::is_same<T, __half>::value)
           f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         else
@@ -76,6 +80,21 @@ struct Chunk {
     }
   }
 };
+
+// P pairs of floats, 16 bytes at a time where P is even.
+template <int P>
+__device__ __forceinline__ void load_floats(const float* src, float2* f) {
+  if constexpr (P == 1) {
+    f[0] = __ldg(reinterpret_cast<const float2*>(src));
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; i += 2) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(src + 2 * i));
+      f[i] = make_float2(x.x, x.y);
+      f[i + 1] = make_float2(x.z, x.w);
+    }
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float2 f) {
@@ -88,33 +107,33 @@ __device__ __forceinline__ uint32_t pack2(float2 f) {
   }
 }
 
-// Stores P (2 or 4) pairs as T.
+// Stores P (1, 2 or 4) pairs as T.
 template <typename T, int P>
 __device__ __forceinline__ void store_chunk(T* dst, const float2* f) {
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 4 && P == 1) {
+    *reinterpret_cast<float2*>(dst) = f[0];
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < P; i += 2)
       *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(f[i].x, f[i].y, f[i + 1].x, f[i + 1].y);
   } else if constexpr (P == 4) {
     *reinterpret_cast<uint4*>(dst) =
         make_uint4(pack2<T>(f[0]), pack2<T>(f[1]), pack2<T>(f[2]), pack2<T>(f[3]));
-  } else {
+  } else if constexpr (P == 2) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(f[0]), pack2<T>(f[1]));
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = pack2<T>(f[0]);
   }
 }
 
 // The weights of one chunk (input type or f32).
-template <typename In>
+template <typename In, int BYTES>
 __device__ __forceinline__ void load_weight(const void* w, int weight_dtype, int e0, float2* f) {
-  constexpr int P = Chunk<In>::N / 2;
-  if (weight_dtype == B200_DTYPE_F32) {
-#pragma unroll
-    for (int i = 0; i < P; i += 2)
-      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(w) + e0 + 2 * i)),
-                           f + i);
-  } else {
-    Chunk<In>::unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const In*>(w) + e0)), f);
-  }
+  using C = Chunk<In, BYTES>;
+  if (weight_dtype == B200_DTYPE_F32)
+    load_floats<C::N / 2>(static_cast<const float*>(w) + e0, f);
+  else
+    C::unpack(__ldg(reinterpret_cast<const typename C::Raw*>(static_cast<const In*>(w) + e0)), f);
 }
 
 enum RowKind { kRowQ = 0, kRowK = 1, kRowV = 2 };
@@ -125,7 +144,7 @@ constexpr int kJobWarps = 4;  // warps per CTA
 // Vector path.  A round is the head rows a warp takes side by side, a job up to
 // U rounds of one kind (queries, keys, values) of a token; a warp per job,
 // tokens' jobs end to end.  LPH lanes (a power of two)
-// share a head row, lane j owning two 16-byte chunks: (j, j + R/2) of the
+// share a head row, lane j owning two chunks of 16 (or 8) bytes: (j, j + R/2) of the
 // rotated part in the split form, (2j, 2j + 1) otherwise, so that both elements
 // of every pair are in one lane, and the pairs of lane j are i = j N .. j N + N
 // - 1 in either form.  Norm weight and rotation are combined once per job into
@@ -139,11 +158,13 @@ constexpr int kJobWarps = 4;  // warps per CTA
 // instructions.  U: 4 where the warps fill the GPU all the same (with 2: 38 and
 // 78 us), else 2 (64 tokens: 2.8 us, with 4: 3.3 us).
 // SHIFT: log2(LPH) where it is known (heads of 128), else -1.
-template <typename In, typename PoolT, bool INTER, int SHIFT, int U>
+template <typename In, typename PoolT, bool INTER, int SHIFT, int U, int BYTES>
 __global__ void __launch_bounds__(kJobWarps * 32)
     rope_vec_kernel(const __grid_constant__ RopeParams p, const int shift_arg, const uint32_t jobs_q,
                     const uint32_t jobs_k, const uint32_t jobs, const uint32_t all_jobs, const int64_t t0) {
-  constexpr int N = Chunk<In>::N, P = N / 2;
+  using Ch = Chunk<In, BYTES>;
+  using Raw = typename Ch::Raw;
+  constexpr int N = Ch::N, P = N / 2;
   const int lph_shift = SHIFT >= 0 ? SHIFT : shift_arg;
   const int lane = threadIdx.x & 31;
   const uint32_t index = blockIdx.x * kJobWarps + (threadIdx.x >> 5);
@@ -174,13 +195,13 @@ __global__ void __launch_bounds__(kJobWarps * 32)
                                   : static_cast<const In*>(p.v) + t * p.vs0;
   const int64_t step = kind == kRowQ ? p.qs1 : kind == kRowK ? p.ks1 : p.vs1;
   src += row0 * step;
-  uint4 ca[U], cb[U];
+  Raw ca[U], cb[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    ca[u] = cb[u] = make_uint4(0, 0, 0, 0);
+    ca[u] = cb[u] = Raw{};
     if (mine && row0 + u * rpw < rows) {
-      ca[u] = *reinterpret_cast<const uint4*>(src + u * rpw * step + ea);
-      cb[u] = *reinterpret_cast<const uint4*>(src + u * rpw * step + eb);
+      ca[u] = *reinterpret_cast<const Raw*>(src + u * rpw * step + ea);
+      cb[u] = *reinterpret_cast<const Raw*>(src + u * rpw * step + eb);
     }
   }
   const bool pos_ok = pos >= 0 && pos < p.table_rows;
@@ -217,13 +238,13 @@ __global__ void __launch_bounds__(kJobWarps * 32)
       if (!mine || row0 + u * rpw >= rows) continue;
       PoolT* dst = pool + static_cast<int64_t>(u * rpw) * p.D;
       if constexpr (std::is_same<In, PoolT>::value) {  // values as they are
-        *reinterpret_cast<uint4*>(dst + ea) = ca[u];
-        *reinterpret_cast<uint4*>(dst + eb) = cb[u];
+        *reinterpret_cast<Raw*>(dst + ea) = ca[u];
+        *reinterpret_cast<Raw*>(dst + eb) = cb[u];
       } else {
         float2 f[P];
-        Chunk<In>::unpack(ca[u], f);
+        Ch::unpack(ca[u], f);
         store_chunk<PoolT, P>(dst + ea, f);
-        Chunk<In>::unpack(cb[u], f);
+        Ch::unpack(cb[u], f);
         store_chunk<PoolT, P>(dst + eb, f);
       }
     }
@@ -236,17 +257,14 @@ __global__ void __launch_bounds__(kJobWarps * 32)
 #pragma unroll
   for (int i = 0; i < P; ++i) A[i] = C[i] = make_float2(1.f, 1.f);
   if (weight != nullptr && mine) {
-    load_weight<In>(weight, p.weight_dtype, ea, A);
-    load_weight<In>(weight, p.weight_dtype, eb, C);
+    load_weight<In, BYTES>(weight, p.weight_dtype, ea, A);
+    load_weight<In, BYTES>(weight, p.weight_dtype, eb, C);
   }
   if (rot) {
     float2 c[P], s[P];
     const float* row = p.cos_sin + pos * p.R + j * N;
-#pragma unroll
-    for (int i = 0; i < P; i += 2) {
-      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + 2 * i)), c + i);
-      Chunk<float>::unpack(__ldg(reinterpret_cast<const uint4*>(row + p.R / 2 + 2 * i)), s + i);
-    }
+    load_floats<P>(row, c);
+    load_floats<P>(row + p.R / 2, s);
     if constexpr (!INTER) {  // a' = a wa c - b wb s,  b' = b wb c + a wa s
 #pragma unroll
       for (int i = 0; i < P; ++i) {
@@ -260,8 +278,8 @@ __global__ void __launch_bounds__(kJobWarps * 32)
       for (int i = 0; i < P; ++i) {
         // Pair i of chunk a and pair P + i of the lane (chunk b).
         const float ca_ = i & 1 ? c[i / 2].y : c[i / 2].x, sa_ = i & 1 ? s[i / 2].y : s[i / 2].x;
-        const float cb_ = i & 1 ? c[(P + i) / 2].y : c[(P + i) / 2].x;
-        const float sb_ = i & 1 ? s[(P + i) / 2].y : s[(P + i) / 2].x;
+        const float cb_ = (P + i) & 1 ? c[(P + i) / 2].y : c[(P + i) / 2].x;
+        const float sb_ = (P + i) & 1 ? s[(P + i) / 2].y : s[(P + i) / 2].x;
         B[i] = make_float2(-A[i].y * sa_, A[i].x * sa_);
         D[i] = make_float2(-C[i].y * sb_, C[i].x * sb_);
         A[i] = make_float2(A[i].x * ca_, A[i].y * ca_);
@@ -276,8 +294,8 @@ __global__ void __launch_bounds__(kJobWarps * 32)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float2 a[P], b[P];
-    Chunk<In>::unpack(ca[u], a);
-    Chunk<In>::unpack(cb[u], b);
+    Ch::unpack(ca[u], a);
+    Ch::unpack(cb[u], b);
     if (weight != nullptr) {  // the same for the whole warp
       float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
@@ -397,27 +415,27 @@ __global__ void __launch_bounds__(256) rope_any_kernel(const RopeParams p) {
   }
 }
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// 16-byte access to every row of a [T, H, D] tensor.
-bool rows_vec(const void* p, const int64_t* st, size_t es) {
-  return st[2] == 1 && aligned16(p) && (st[0] * static_cast<int64_t>(es)) % 16 == 0 &&
-         (st[1] * static_cast<int64_t>(es)) % 16 == 0;
+// Access in chunks of `bytes` to every row of a [T, H, D] tensor.
+bool rows_vec(const void* p, const int64_t* st, size_t es, int bytes) {
+  return st[2] == 1 && aligned(p, bytes) && (st[0] * static_cast<int64_t>(es)) % bytes == 0 &&
+         (st[1] * static_cast<int64_t>(es)) % bytes == 0;
 }
 
-template <typename In, typename PoolT, int U>
+template <typename In, typename PoolT, int U, int BYTES>
 int launch_jobs(const RopeParams& p, int64_t tokens, cudaStream_t stream) {
-  constexpr int N = Chunk<In>::N;
-  constexpr int kShift128 = N == 8 ? 3 : 4;
+  constexpr int N = Chunk<In, BYTES>::N;
+  constexpr int kShift128 = BYTES < 16 ? -1 : N == 8 ? 3 : 4;
   const int shift = log2i(p.D / (2 * N));
   const int per_job = U * (32 >> shift);
   const uint32_t jobs_q = static_cast<uint32_t>(ceil_div(p.Hq, per_job));
   const uint32_t jobs_k = static_cast<uint32_t>(ceil_div(p.Hkv, per_job));
   const uint32_t jobs = jobs_q + jobs_k * (p.append ? 2 : 1);
-  auto kern = shift == kShift128 ? (p.interleaved ? rope_vec_kernel<In, PoolT, true, kShift128, U>
-                                                  : rope_vec_kernel<In, PoolT, false, kShift128, U>)
-                                 : (p.interleaved ? rope_vec_kernel<In, PoolT, true, -1, U>
-                                                  : rope_vec_kernel<In, PoolT, false, -1, U>);
+  auto kern = shift == kShift128 ? (p.interleaved ? rope_vec_kernel<In, PoolT, true, kShift128, U, BYTES>
+                                                  : rope_vec_kernel<In, PoolT, false, kShift128, U, BYTES>)
+                                 : (p.interleaved ? rope_vec_kernel<In, PoolT, true, -1, U, BYTES>
+                                                  : rope_vec_kernel<In, PoolT, false, -1, U, BYTES>);
   // Job numbers are 32-bit: very many tokens take several launches.
   const int64_t most = (int64_t(1) << 31) / jobs;
   for (int64_t t0 = 0; t0 < tokens; t0 += most) {
@@ -429,12 +447,14 @@ int launch_jobs(const RopeParams& p, int64_t tokens, cudaStream_t stream) {
 }
 
 template <typename In, typename PoolT>
-int launch_vec(const RopeParams& p, int64_t tokens, int num_sms, cudaStream_t stream) {
-  const int shift = log2i(p.D / (2 * Chunk<In>::N));
+int launch_vec(const RopeParams& p, int bytes, int64_t tokens, int num_sms, cudaStream_t stream) {
+  const int shift = log2i(p.D / (2 * bytes / static_cast<int>(sizeof(In))));
   const int64_t rounds = tokens * (ceil_div(p.rows, 32 >> shift));
   // About 20 warps of four rounds to an SM.
-  if (rounds >= int64_t(4) * 20 * num_sms) return launch_jobs<In, PoolT, 4>(p, tokens, stream);
-  return launch_jobs<In, PoolT, 2>(p, tokens, stream);
+  const bool four = rounds >= int64_t(4) * 20 * num_sms;
+  if (bytes == 16)
+    return four ? launch_jobs<In, PoolT, 4, 16>(p, tokens, stream) : launch_jobs<In, PoolT, 2, 16>(p, tokens, stream);
+  return four ? launch_jobs<In, PoolT, 4, 8>(p, tokens, stream) : launch_jobs<In, PoolT, 2, 8>(p, tokens, stream);
 }
 
 }  // namespace
@@ -472,9 +492,6 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
   p.interleaved = a.interleaved != 0;
   p.eps = a.eps;
   p.inv_d = 1.0f / static_cast<float>(a.head_dim);
-  const size_t es = dtype_size(a.dtype);
-  bool vec = rows_vec(a.q, a.q_stride, es) && rows_vec(a.k, a.k_stride, es) &&
-             rows_vec(a.q_out, a.q_out_stride, es) && aligned16(a.cos_sin);
   if (append != nullptr) {
     p.append = 1;
     p.v = append->v;
@@ -488,34 +505,42 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
     p.pool_slots = append->pool.num_blocks * append->pool.block_size;
     p.layer_row0 = append->layer_idx * p.pool_slots;
     p.rows += p.Hkv;
-    vec = vec && rows_vec(append->v, append->v_stride, es);
-  } else {
-    vec = vec && rows_vec(a.k_out, a.k_out_stride, es);
   }
-  // Whole chunk pairs: no lane holds half of a rotated pair.
-  const int n = static_cast<int>(16 / es);
-  vec = vec && p.D % (2 * n) == 0 && p.R % (2 * n) == 0;
-  if (a.q_weight != nullptr || a.k_weight != nullptr)
-    vec = vec && (a.weight_dtype == a.dtype || a.weight_dtype == B200_DTYPE_F32) &&
-          (a.q_weight == nullptr || aligned16(a.q_weight)) &&
-          (a.k_weight == nullptr || aligned16(a.k_weight));
-  if (vec) {
+  // Chunks that every row's address and stride allow, in whole pairs: no lane
+  // holds half of a rotated pair, and a warp at least a row.  (8192 tokens of 32 +
+  // 8 heads of 80, 40 rotated, bf16: 34 us in chunks of 8 bytes, by elements 356.)
+  const size_t es = dtype_size(a.dtype);
+  auto fits = [&](int bytes) {
+    const int n = bytes / static_cast<int>(es);
+    if (!rows_vec(a.q, a.q_stride, es, bytes) || !rows_vec(a.k, a.k_stride, es, bytes) ||
+        !rows_vec(a.q_out, a.q_out_stride, es, bytes) || !aligned(a.cos_sin, 16) ||
+        !(append != nullptr ? rows_vec(append->v, append->v_stride, es, bytes)
+                            : rows_vec(a.k_out, a.k_out_stride, es, bytes)))
+      return false;
+    if (p.D % (2 * n) != 0 || p.R % (2 * n) != 0 || p.D / (2 * n) > 32) return false;
+    if (a.q_weight == nullptr && a.k_weight == nullptr) return true;
+    return (a.weight_dtype == a.dtype || a.weight_dtype == B200_DTYPE_F32) &&
+           (a.q_weight == nullptr || aligned(a.q_weight, 16)) &&
+           (a.k_weight == nullptr || aligned(a.k_weight, 16));
+  };
+  const int vec = fits(16) ? 16 : fits(8) ? 8 : 0;
+  if (vec != 0) {
     const bool pool_f32 = p.pool_dtype == B200_DTYPE_F32;
     if (a.dtype == B200_DTYPE_F32) {
       if (pool_f32)
-        rc = launch_vec<float, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<float, float>(p, vec, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<float, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<float, __nv_bfloat16>(p, vec, a.num_tokens, dev.num_sms, stream);
     } else if (a.dtype == B200_DTYPE_BF16) {
       if (pool_f32)
-        rc = launch_vec<__nv_bfloat16, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__nv_bfloat16, float>(p, vec, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<__nv_bfloat16, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__nv_bfloat16, __nv_bfloat16>(p, vec, a.num_tokens, dev.num_sms, stream);
     } else {
       if (pool_f32)
-        rc = launch_vec<__half, float>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__half, float>(p, vec, a.num_tokens, dev.num_sms, stream);
       else
-        rc = launch_vec<__half, __nv_bfloat16>(p, a.num_tokens, dev.num_sms, stream);
+        rc = launch_vec<__half, __nv_bfloat16>(p, vec, a.num_tokens, dev.num_sms, stream);
     }
     return rc;
   } else {

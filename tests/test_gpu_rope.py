@@ -52,6 +52,10 @@ SIZES = [  # t, hq, hkv, d, rot
     (4, 6, 2, 80, 32),     # chunk pairs not a power of two
     (3, 3, 3, 96, 48),
     (2, 4, 2, 256, 256),   # the widest head
+    (5, 8, 2, 80, 40),     # 16-bit rows in chunks of 8 bytes
+    (4, 33, 1, 72, 24),
+    (3, 4, 2, 84, 44),     # fp32 rows in chunks of 8 bytes
+    (5, 6, 2, 80, 20),
     (6, 2, 1, 64, 2),      # one pair: the element path
     (3, 2, 1, 10, 6),      # rows that are not whole chunks
     (2, 3, 1, 254, 100),
@@ -91,7 +95,7 @@ def test_norm_rope_layouts(layout, wdtype, index):
     assert_close(ko, norm_rope(k, pos, table, kw, 1e-3), BF16, 64, False, "k")
 
 
-@pytest.mark.parametrize("size", [(5, 32, 8, 128, 128), (3, 2, 1, 10, 6)], ids=str)
+@pytest.mark.parametrize("size", [(5, 32, 8, 128, 128), (7, 8, 2, 80, 40), (3, 2, 1, 10, 6)], ids=str)
 def test_norm_rope_in_place_gives_the_same(size):
     from b200attn import qk_norm_rope_b200
 
@@ -105,6 +109,8 @@ def test_norm_rope_in_place_gives_the_same(size):
 
 @pytest.mark.parametrize("size,dtype,interleaved", [((1301, 32, 8, 128, 128), BF16, False),
                                                     ((3001, 20, 4, 80, 32), F32, True),
+                                                    ((2600, 32, 8, 80, 40), BF16, False),
+                                                    ((2700, 12, 4, 80, 20), F32, True),
                                                     ((2999, 9, 3, 64, 64), F16, False)], ids=str)
 def test_many_tokens_equal_few(size, dtype, interleaved):
     """Large calls give a warp more rows; every row comes out the same."""
