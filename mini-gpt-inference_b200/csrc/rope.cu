@@ -56,14 +56,15 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
   return d;
 }
 
-// One chunk (16 or 8 bytes) of the input type: N elements, as N / 2 pairs of floats.
+// One chunk (16, 8 or, of 16-bit types, 4 bytes) of the input type: N elements, as N / 2 pairs of floats.
 template <typename T, int BYTES>
 struct Chunk {
   static constexpr int N = BYTES / sizeof(T);
-  using Raw = std::conditional_t<BYTES == 16, uint4, uint2>;
+  using Raw = std::conditional_t<BYTES == 16, uint4, std::conditional_t<BYTES == 8, uint2, uint32_t>>;
   __device__ __forceinline__ static void unpack(const Raw& c, float2* f) {
     uint32_t w[BYTES / 4];
-    w[0] = c.x, w[1] = c.y;
+    if constexpr (BYTES == 4) w[0] = c;
+    if constexpr (BYTES >= 8) w[0] = c.x, w[1] = c.y;
     if constexpr (BYTES == 16) w[2] = c.z, w[3] = c.w;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -144,7 +145,7 @@ constexpr int kJobWarps = 4;  // warps per CTA
 // Vector path.  A round is the head rows a warp takes side by side, a job up to
 // U rounds of one kind (queries, keys, values) of a token; a warp per job,
 // tokens' jobs end to end.  LPH lanes (a power of two)
-// share a head row, lane j owning two chunks of 16 (or 8) bytes: (j, j + R/2) of the
+// share a head row, lane j owning two chunks of 16 (8, 4) bytes: (j, j + R/2) of the
 // rotated part in the split form, (2j, 2j + 1) otherwise, so that both elements
 // of every pair are in one lane, and the pairs of lane j are i = j N .. j N + N
 // - 1 in either form.  Norm weight and rotation are combined once per job into
@@ -454,6 +455,9 @@ int launch_vec(const RopeParams& p, int bytes, int64_t tokens, int num_sms, cuda
   const bool four = rounds >= int64_t(4) * 20 * num_sms;
   if (bytes == 16)
     return four ? launch_jobs<In, PoolT, 4, 16>(p, tokens, stream) : launch_jobs<In, PoolT, 2, 16>(p, tokens, stream);
+  if constexpr (sizeof(In) == 2)
+    if (bytes == 4)
+      return four ? launch_jobs<In, PoolT, 4, 4>(p, tokens, stream) : launch_jobs<In, PoolT, 2, 4>(p, tokens, stream);
   return four ? launch_jobs<In, PoolT, 4, 8>(p, tokens, stream) : launch_jobs<In, PoolT, 2, 8>(p, tokens, stream);
 }
 
@@ -508,7 +512,8 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
   }
   // Chunks that every row's address and stride allow, in whole pairs: no lane
   // holds half of a rotated pair, and a warp at least a row.  (8192 tokens of 32 +
-  // 8 heads of 80, 40 rotated, bf16: 34 us in chunks of 8 bytes, by elements 356.)
+  // 8 heads of 80, 40 rotated, bf16: 34 us in chunks of 8 bytes, by elements 356;
+  // 20 rotated: 57 us in chunks of 4, by elements 412.)
   const size_t es = dtype_size(a.dtype);
   auto fits = [&](int bytes) {
     const int n = bytes / static_cast<int>(es);
@@ -523,7 +528,7 @@ int launch_qk_norm_rope(const b200_qk_norm_rope_args_t& a, const b200_rope_kv_ap
            (a.q_weight == nullptr || aligned(a.q_weight, 16)) &&
            (a.k_weight == nullptr || aligned(a.k_weight, 16));
   };
-  const int vec = fits(16) ? 16 : fits(8) ? 8 : 0;
+  const int vec = fits(16) ? 16 : fits(8) ? 8 : es == 2 && fits(4) ? 4 : 0;
   if (vec != 0) {
     const bool pool_f32 = p.pool_dtype == B200_DTYPE_F32;
     if (a.dtype == B200_DTYPE_F32) {

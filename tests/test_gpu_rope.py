@@ -55,7 +55,8 @@ SIZES = [  # t, hq, hkv, d, rot
     (5, 8, 2, 80, 40),     # 16-bit rows in chunks of 8 bytes
     (4, 33, 1, 72, 24),
     (3, 4, 2, 84, 44),     # fp32 rows in chunks of 8 bytes
-    (5, 6, 2, 80, 20),
+    (5, 6, 2, 80, 20),     # and 16-bit rows in chunks of 4
+    (4, 3, 2, 120, 12),
     (6, 2, 1, 64, 2),      # one pair: the element path
     (3, 2, 1, 10, 6),      # rows that are not whole chunks
     (2, 3, 1, 254, 100),
@@ -95,7 +96,7 @@ def test_norm_rope_layouts(layout, wdtype, index):
     assert_close(ko, norm_rope(k, pos, table, kw, 1e-3), BF16, 64, False, "k")
 
 
-@pytest.mark.parametrize("size", [(5, 32, 8, 128, 128), (7, 8, 2, 80, 40), (3, 2, 1, 10, 6)], ids=str)
+@pytest.mark.parametrize("size", [(5, 32, 8, 128, 128), (7, 8, 2, 80, 40), (7, 8, 2, 80, 20), (3, 2, 1, 10, 6)], ids=str)
 def test_norm_rope_in_place_gives_the_same(size):
     from b200attn import qk_norm_rope_b200
 
@@ -111,6 +112,8 @@ def test_norm_rope_in_place_gives_the_same(size):
                                                     ((3001, 20, 4, 80, 32), F32, True),
                                                     ((2600, 32, 8, 80, 40), BF16, False),
                                                     ((2700, 12, 4, 80, 20), F32, True),
+                                                    ((2500, 14, 4, 80, 20), BF16, True),
+                                                    ((2500, 14, 4, 88, 36), F16, False),
                                                     ((2999, 9, 3, 64, 64), F16, False)], ids=str)
 def test_many_tokens_equal_few(size, dtype, interleaved):
     """Large calls give a warp more rows; every row comes out the same."""
