@@ -25,7 +25,6 @@ _TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 _SIZE = {"bf16": 2, "f16": 2, "f32": 4}
 _DEVICE = "cuda"
 _EPS = 1e-6
-_PACKAGE = str(Path(__file__).resolve().parents[1] / "mini-gpt-inference_b200")
 
 
 def listed():
@@ -212,8 +211,9 @@ def run(s):
 
 
 def _run_own(s, op):
-    if _PACKAGE not in sys.path:
-        sys.path.insert(0, _PACKAGE)
+    package = str(Path(__file__).resolve().parents[1] / "mini-gpt-inference_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
     import b200attn
 
     if op == "norm_rope":
