@@ -32,7 +32,8 @@
 // TMEM (512 columns): S_w / P_w at 128 w, O_w at 256 + 128 w.
 // V rows behind the prefix are cleared in shared memory before they are
 // used: unwritten pool rows can hold NaN, and 0 * NaN is NaN.
-// Every wait is bounded; after one runs out all roles leave.
+// Every wait is bounded and a whole warp's decision; after one runs out all
+// roles leave.
 //
 // Measured (32 query heads of 128 over 8 key heads): 256 sequences over 16384
 // keys 73 us, of which 53 us are 28 tile pairs of 1.9 us a CTA (the products
@@ -85,6 +86,18 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A whole warp's bounded wait: all lanes get one answer.  What a warp does next
+// (votes, elections, TMEM access) needs every lane, and lanes that poll for
+// themselves may pass the limit, or see another role's abort flag, on different
+// sides of it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+}
+// The same; no also where a role has given up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const volatile int32_t* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity) && *abort_flag == 0) != 0;
 }
 
 // Waits for this thread's TMEM loads; the 32 values cannot be used earlier.
@@ -351,14 +364,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv, ++it) {
             const int st = static_cast<int>(it % NS);
-            int good = 1;
-            if (lane == 0) good = mbar_wait(&empty[st], ((it / NS) & 1u) ^ 1u) ? 1 : 0;
-            good = __shfl_sync(0xffffffffu, good, 0);
-            if (!good || *abort_flag) {
-              if (!good && lane == 0) give_up();
-              ok = false;
-              break;
-            }
+            ok = warp_wait(&empty[st], ((it / NS) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
             if (lane == 0)
               mbar_arrive_expect_tx(&full[st], static_cast<uint32_t>(nb * L::HALVES * box_bytes));
             __syncwarp();
@@ -372,13 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // Copies in flight land before the CTA ends.
-      if (lane == 0) {
-        for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i)
-          if (!mbar_wait(&full[i % NS], (i / NS) & 1u)) {
-            give_up();
-            break;
-          }
-      }
+      for (uint32_t i = it > NS ? it - NS : 0; i < it; ++i) ok = warp_wait(&full[i % NS], (i / NS) & 1u) && ok;
+      if (!ok && lane == 0) give_up();
     } else if (warp == 1) {
       // ------------------------------------------------------------ products
       // The whole warp, so that descriptors stay in uniform registers (one lane
@@ -394,16 +396,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t np0 = 0, np1 = 0;  // P tiles of group w awaited so far
         uint32_t nq0 = 0, nq1 = 0;  // Q tiles awaited so far
         bool ok = true;
-        auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-          return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
-        };
-        auto wait_entry = [&](uint32_t e) { return wait_all(&full[e % NS], (e / NS) & 1u); };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity, abort_flag); };
+        auto wait_entry = [&](uint32_t e) { return wait(&full[e % NS], (e / NS) & 1u); };
         Segments sg(p);
         while (ok && sg.next()) {
           const int n = sg.n;
           const bool two = !one && unit_rows(sg.unit) + kBM < s.rows;  // row tile 1 is there
-          ok = wait_all(&q_full[0], nq0++ & 1u) && (!two || wait_all(&q_full[1], nq1++ & 1u)) &&
-               *abort_flag == 0;
+          ok = wait(&q_full[0], nq0++ & 1u) && (!two || wait(&q_full[1], nq1++ & 1u));
           // Step t: P V of tile t, then S of tile t + lead for the same group, which
           // frees the columns in that order.  Two row tiles: both groups, one tile
           // ahead; one row tile: the groups alternate, two tiles ahead.
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int w = one ? t & 1 : i;
               const bool last = i == groups - 1;
               if (t >= 0) {
-                ok = wait_all(&p_full[w], (w ? np1 : np0) & 1u) && (i > 0 || wait_entry(ev));
+                ok = wait(&p_full[w], (w ? np1 : np0) & 1u) && (i > 0 || wait_entry(ev));
                 if (!ok) break;
                 (w ? np1 : np0) += 1;
                 tc_fence_after();
@@ -448,13 +447,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (last) mma_commit(&empty[ek % NS]);
               }
             }
-            ok = ok && *abort_flag == 0;
           }
           first += 2 * n;
         }
         if (!ok && lane == 0) give_up();
         mma_commit(idle);  // every product issued has ended before TMEM is freed
-        if (!wait_all(idle, 0) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
+        if (!warp_wait(idle, 0) && lane == 0) report(s.status, B200_DEV_WAIT_TIMEOUT);
         __syncwarp();
       }
     } else {
@@ -492,10 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int k = 0; k < cnt; ++k, ++tiles) {
         const int jj = one ? 2 * k + w : k;  // tile within the segment
-        if (!mbar_wait(&s_full[w], tiles & 1u) || *abort_flag) {
-          ok = false;
-          break;
-        }
+        ok = warp_wait(&s_full[w], tiles & 1u, abort_flag);
+        if (!ok) break;
         tc_fence_after();
         const int left = static_cast<int>(  // keys from here on
             min(s.prefix - static_cast<int64_t>(sg.j0 + jj) * kBN, static_cast<int64_t>(kBN)));
@@ -574,10 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (left < kBN && (one || w == 0)) {
           const uint32_t e = first + 2 * jj + 1;
-          if (!mbar_wait(&full[e % NS], (e / NS) & 1u)) {
-            ok = false;
-            break;
-          }
+          ok = warp_wait(&full[e % NS], (e / NS) & 1u, abort_flag);
+          if (!ok) break;
           if (r >= left) {
             uint8_t* vrow = smem + L::RING + (e % NS) * L::TILE + r * 128;
 #pragma unroll
@@ -593,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[w]);
       }
       if (ok && cnt > 0) {
-        ok = mbar_wait(&o_full[w], oseg & 1u) && *abort_flag == 0;
+        ok = warp_wait(&o_full[w], oseg & 1u, abort_flag);
         ++oseg;
         tc_fence_after();
       }
@@ -611,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(merge_full);
-        ok = mbar_wait(merge_full, mseg & 1u) && *abort_flag == 0;
+        ok = warp_wait(merge_full, mseg & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
         uint32_t x0, y0, x1, y1;
@@ -664,21 +658,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // O, Q and ml may be written again once both groups are done with them.
         tc_fence_before();
         mbar_arrive(merge_done);
-        ok = mbar_wait(merge_done, mseg & 1u) && *abort_flag == 0;
+        ok = warp_wait(merge_done, mseg & 1u, abort_flag);
         tc_fence_after();
         ++mseg;
       } else if (one ? w == 0 : group_live) {
         // The next Q goes over what the group's warps stage their rows in.
         mbar_arrive(&drained[w]);
-        ok = mbar_wait(&drained[w], dseg & 1u) && *abort_flag == 0;
+        ok = warp_wait(&drained[w], dseg & 1u, abort_flag);
         ++dseg;
       }
       first += 2 * n;
     }
-    if (!ok) {
-      report(s.status, B200_DEV_WAIT_TIMEOUT);
-      *abort_flag = 1;
-    }
+    if (!ok) give_up();
   }
   tc_fence_before();
   __syncthreads();

@@ -1,0 +1,31 @@
+"""Waits of the shared-prefix decode's tcgen05 kernel, read from its source: a
+wait that runs out cannot be made to happen here, and what follows it must
+hold for whole warps."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import b200attn
+
+SOURCE = Path(b200attn.__file__).parents[1] / "csrc" / "shared_prefix_tc.cu"
+
+
+def _code() -> str:
+    text = SOURCE.read_text()
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def test_every_wait_is_a_vote_of_the_warp():
+    """A lane that leaves a loop by its own poll of a barrier, or its own look at
+    the abort flag, would leave the others at a full-mask vote without it."""
+    code = _code()
+    helpers = re.findall(r"__device__ __forceinline__ bool warp_wait\([^{]*\{[^}]*\}", code)
+    assert len(helpers) == 2
+    for h in helpers:
+        assert re.search(r"return __all_sync\(0xffffffffu, mbar_wait\(bar, parity\)", h)
+        code = code.replace(h, "")
+    assert "mbar_wait(" not in code
+    # Outside the helpers the flag is only set.
+    uses = re.findall(r"\*abort_flag[^;]*;", code)
+    assert sorted(u.replace(" ", "") for u in uses) == ["*abort_flag=0;", "*abort_flag=1;"]
