@@ -111,6 +111,11 @@ __device__ __forceinline__ void wait_ld32(float* v) {
         "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
 
+// The same for the pair of each of two groups.
+__device__ __forceinline__ void wait_ld4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(a), "+r"(b), "+r"(c), "+r"(d));
+}
+
 // Weights 2^(v scale - ref) of 32 scores as bf16 pairs; returns their sum
 // before the rounding.  LO: also what the rounding left, as bf16 pairs.
 template <bool LO>
@@ -611,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t x0, y0, x1, y1;
         tmem_ld2(tmem + lanes, x0, y0);
         tmem_ld2(tmem + 128 + lanes, x1, y1);
-        tmem_wait_ld();
+        wait_ld4(x0, y0, x1, y1);
         const float2 a0 = make_float2(__uint_as_float(x0), __uint_as_float(y0));
         const float2 a1 = make_float2(__uint_as_float(x1), __uint_as_float(y1));
         m = fmaxf(a0.x, a1.x);
@@ -637,11 +642,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (both) {
             float o1[32];
             tmem_ld32(o0 + 128 + c, o1);
-            tmem_wait_ld();
+            wait_ld32(o);
+            wait_ld32(o1);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = o[e] * f0 + o1[e] * f1;
           } else {
-            tmem_wait_ld();
+            wait_ld32(o);
           }
           out.put(c, o);
           if ((c + 32) % W == 0) out.flush(c + 32 - W);

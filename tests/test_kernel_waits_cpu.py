@@ -29,3 +29,16 @@ def test_every_wait_is_a_vote_of_the_warp():
     # Outside the helpers the flag is only set.
     uses = re.findall(r"\*abort_flag[^;]*;", code)
     assert sorted(u.replace(" ", "") for u in uses) == ["*abort_flag=0;", "*abort_flag=1;"]
+
+
+def test_every_tmem_load_is_held_by_its_wait():
+    """The registers of a load are operands of the wait behind it: a wait that
+    names none lets the compiler move their use ahead of it."""
+    code = _code()
+    assert "tmem_wait_ld(" not in code
+    waited = set(re.findall(r"\w+", " ".join(re.findall(r"\bwait_ld(?:4|32)\(([^;]*)\);", code))))
+    loads = re.findall(r"\btmem_ld(2|32)\(([^;]*)\);", code)
+    assert len(loads) >= 8
+    for kind, args in loads:
+        for name in [x.strip().split("[")[0] for x in args.split(",")][-2 if kind == "2" else -1:]:
+            assert name in waited, args
