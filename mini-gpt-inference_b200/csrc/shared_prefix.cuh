@@ -71,6 +71,17 @@ TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms);
 int launch_shared_prefix_tc(const SharedParams& s, const b200_kv_pool_t& pool, const TcSplit& t,
                             int zero_count, cudaStream_t stream);
 
+// Two floats as bf16 rounded towards zero (their upper halves).  Where several
+// bf16 pieces add up to a number, all but the last are chopped like this: what is
+// left then has the number's sign, and kKeepSign of the number, less than f32
+// itself rounds off, keeps it from being zero, so that every piece times an
+// infinity is the same infinity.  (Pieces rounded to nearest leave rests of
+// either sign or none: inf - inf, 0 * inf.)
+constexpr float kKeepSign = 0x1p-30f;
+__device__ __forceinline__ uint32_t chop_bf16(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+
 // Keys [*k0, *k1) of part `split` of a sequence with n own keys; returns the
 // number of parts (at least 1, also for n = 0).
 __device__ __forceinline__ int own_range(const SharedParams& p, int64_t n, int split, int64_t* k0,

@@ -109,7 +109,7 @@ struct OwnSmem {
 // QP: bf16 pieces that a query element is the exact sum of: 1 for bf16, 2 for
 // f16 (11 bits), 3 for f32 (24 bits).  A piece is another product, and there is
 // time for them.  The weights take part in as many pieces, and at least in two:
-// what is left of them is 2^-16, with three 2^-24.
+// what is left of them is at most 2^-16, with three 2^-24.
 template <int DP, bool PREFIX, int QP>
 __global__ void __launch_bounds__(kWarps * 32)
     shared_own_mma_kernel(const __grid_constant__ CUtensorMap tmk,
@@ -323,17 +323,21 @@ __global__ void __launch_bounds__(kWarps * 32)
     }
     const float ref0 = m[0] == -INFINITY ? 0.f : m[0];
     const float ref1 = m[1] == -INFINITY ? 0.f : m[1];
-    float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
-    float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
+    const float p0 = ex2(x[0] - ref0), p1 = ex2(x[1] - ref1);
+    const float p2 = ex2(x[2] - ref0), p3 = ex2(x[3] - ref1);
     l[0] += p0 + p2;
     l[1] += p1 + p3;
+    float r0 = p0, r1 = p1, r2 = p2, r3 = p3;  // what the pieces so far leave
 #pragma unroll
     for (int w = 0; w < PP; ++w) {
-      const uint32_t h0 = pack_bf16(p0, p1), h1 = pack_bf16(p2, p3);
+      const bool last = w == PP - 1;
+      const uint32_t h0 = last ? pack_bf16(r0, r1) : chop_bf16(r0, r1);
+      const uint32_t h1 = last ? pack_bf16(r2, r3) : chop_bf16(r2, r3);
       pb[w][0] = transpose8x8(h0);
       pb[w][1] = transpose8x8(h1);
       const float2 f0 = bf16x2_to_float2(h0), f1 = bf16x2_to_float2(h1);
-      p0 -= f0.x, p1 -= f0.y, p2 -= f1.x, p3 -= f1.y;
+      r0 = fmaf(p0, kKeepSign, r0 - f0.x), r1 = fmaf(p1, kKeepSign, r1 - f0.y);
+      r2 = fmaf(p2, kKeepSign, r2 - f1.x), r3 = fmaf(p3, kKeepSign, r3 - f1.y);
     }
     // V rows of masked keys may hold anything, and 0 * NaN is NaN.
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;

@@ -117,10 +117,11 @@ __device__ __forceinline__ void wait_ld4(uint32_t& a, uint32_t& b, uint32_t& c, 
 }
 
 // Weights 2^(v scale - ref) of 32 scores as bf16 pairs; returns their sum
-// before the rounding.  LO: also what the rounding left, as bf16 pairs.
+// before the rounding.  LO: rounded towards zero, and also what that left.
 template <bool LO>
 __device__ __forceinline__ float weights32(const float* v, float scale, float ref, uint32_t* pk, uint32_t* lo) {
   const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-ref, -ref), one2 = make_float2(1.f, 1.f);
+  const float2 minus2 = make_float2(-1.f, -1.f), keep2 = make_float2(kKeepSign, kKeepSign);
   float2 q[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) q[e] = ffma2(make_float2(v[2 * e], v[2 * e + 1]), sc2, nm2);
@@ -128,10 +129,12 @@ __device__ __forceinline__ float weights32(const float* v, float scale, float re
   for (int e = 0; e < 16; ++e) q[e] = make_float2(ex2(q[e].x), ex2(q[e].y));
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
-    pk[e] = pack_bf16(q[e].x, q[e].y);
     if constexpr (LO) {
-      const float2 hi = bf16x2_to_float2(pk[e]);
-      lo[e] = pack_bf16(q[e].x - hi.x, q[e].y - hi.y);
+      pk[e] = chop_bf16(q[e].x, q[e].y);
+      const float2 rest = ffma2(q[e], keep2, ffma2(bf16x2_to_float2(pk[e]), minus2, q[e]));
+      lo[e] = pack_bf16(rest.x, rest.y);
+    } else {
+      pk[e] = pack_bf16(q[e].x, q[e].y);
     }
   }
 #pragma unroll
