@@ -106,9 +106,9 @@ struct OwnSmem {
 
 // DP: head dimension rounded up to 64 or 128.
 // PREFIX: the keys are a part of the prefix's, the rows all sequences'.
-// QP: bf16 pieces that a query element is the exact sum of: 1 for bf16, 2 for
-// f16 (11 bits), 3 for f32 (24 bits).  A piece is another product, and there is
-// time for them.  The weights take part in as many pieces, and at least in two:
+// QP: bf16 pieces that a query element is the sum of: 1 for bf16, 2 for f16 (11
+// bits), 3 for f32 (24 bits), in all its bits (and 2^-30 of it at most where a
+// piece would be zero).  A piece is another product, and there is time for them.  The weights take part in as many pieces, and at least in two:
 // what is left of them is at most 2^-16, with three 2^-24.
 template <int DP, bool PREFIX, int QP>
 __global__ void __launch_bounds__(kWarps * 32)
@@ -239,12 +239,13 @@ __global__ void __launch_bounds__(kWarps * 32)
           qf[0][i][u] = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(p.q) + at);
         } else {
           constexpr int type = QP == 1 ? B200_DTYPE_BF16 : QP == 2 ? B200_DTYPE_F16 : B200_DTYPE_F32;
-          float x = load_elem(p.q, at, type), y = load_elem(p.q, at + p.qs2, type);
+          const float x = load_elem(p.q, at, type), y = load_elem(p.q, at + p.qs2, type);
+          float rx = x, ry = y;  // what the pieces so far leave
 #pragma unroll
           for (int c = 0; c < QP; ++c) {
-            qf[c][i][u] = pack_bf16(x, y);
+            qf[c][i][u] = chop_bf16(rx, ry);
             const float2 f = bf16x2_to_float2(qf[c][i][u]);
-            x -= f.x, y -= f.y;
+            rx = fmaf(x, kKeepSign, rx - f.x), ry = fmaf(y, kKeepSign, ry - f.y);
           }
         }
       }

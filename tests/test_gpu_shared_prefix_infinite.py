@@ -93,3 +93,29 @@ def test_infinities_of_both_signs_are_no_number(size, types):
     cpu.pool.v[0][_row(cpu, 0, size[5] - 2)][:, 5] = -INF
     want = _check(cpu, _run(cpu), _weights(types, size))
     assert want[..., 5].isnan().all()
+
+
+@_all
+def test_a_key_with_an_infinite_element(size, types):
+    """Its score is -inf for about half of the rows, which it gives no weight,
+    and +inf for the others, which have no softmax."""
+    cpu = case(*size, *types, seed=63)
+    cpu.pool.k[0][_row(cpu, 0, 7)][:, 11] = INF
+    cpu.pool.k[0][_row(cpu, 0, size[5] - 1)][:, 40] = -INF
+    cpu.q[..., 40] = -cpu.q[..., 11]  # every infinite score of a row has one sign
+    for i in range(size[0]):
+        cpu.pool.k[0][_row(cpu, i, size[5] + 1)][:, 11] = INF
+    want = _check(cpu, _run(cpu), _weights(types, size))
+    odd = want.isnan().any(-1)
+    assert odd.any() and not odd.all()
+
+
+@ALL[0]
+@pytest.mark.parametrize("types", [(F32, BF16), (F32, F32)], ids=str)
+def test_queries_next_to_the_largest_number(size, types):
+    """Queries beyond bf16's largest number are finite in float32; keys small enough
+    keep their scores of ordinary size."""
+    cpu = case(*size, *types, seed=65)
+    cpu.q[..., 4] = 3.4e38
+    cpu.pool.k[..., 4] = (cpu.pool.k[..., 4].float().sign() * 2.0 ** -125).to(types[1])
+    _check(cpu, _run(cpu), False)
