@@ -43,6 +43,7 @@
 // quarter by quarter, of weights by polynomial on the FMA pipes, and turns of
 // the two groups at the exponential unit were all built and measured: 2 to 2.6
 // us a tile pair.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -505,8 +506,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             min(s.prefix - static_cast<int64_t>(sg.j0 + jj) * kBN, static_cast<int64_t>(kBN)));
         if (warp_live) {
           // The weights are taken relative to the row's reference m as it stands,
-          // and their sum tells whether that was far too low (or a score is not
-          // a number); the rare warp with such a row finds a new one and does
+          // and their sum tells whether that was far too low, or none yet (or a
+          // score is not a number); the rare warp with such a row finds a new one and does
           // the tile again.  The first tile has no reference yet.  What runs
           // once or rarely is rolled up: cold instructions cost more than
           // loops here (unrolled, the first two tiles of a CTA took 11 us).
@@ -556,7 +557,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               m = m_new;
             }
-            const float ref = m == -INFINITY ? 0.f : m;
+            // A row that has met no weight yet has no reference either: the lowest
+            // number in its place makes the sum of any weight infinite, and is as
+            // good as any where all scores are still -inf.
+            const float ref = m == -INFINITY ? -FLT_MAX : m;
             float v[2][32];
             add = 0.f;
             tmem_ld32(ts, v[0]);

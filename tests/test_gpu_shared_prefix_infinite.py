@@ -119,3 +119,19 @@ def test_queries_next_to_the_largest_number(size, types):
     cpu.q[..., 4] = 3.4e38
     cpu.pool.k[..., 4] = (cpu.pool.k[..., 4].float().sign() * 2.0 ** -125).to(types[1])
     _check(cpu, _run(cpu), False)
+
+
+@pytest.mark.parametrize("shift", [0.0, 6.0, -40.0])
+@_all
+def test_whole_key_tiles_without_weight(size, types, shift):
+    """Scores of -inf over most of the prefix's key tiles, so that parts begin
+    with them or hold nothing else; the others' scores are moved by ``shift``."""
+    cpu = case(*size, *types, seed=64)
+    d = size[3]
+    cpu.q[..., 2] = 1.0
+    k = cpu.pool.k[0]
+    at = torch.arange(cpu.prefix)
+    rows = cpu.table[at // cpu.block], at % cpu.block
+    none = (at // 128 % 4 != 3) & (at != 5)
+    k[rows[0], rows[1], :, 2] = torch.where(none, -INF, shift * d ** 0.5)[:, None].to(k.dtype)
+    _check(cpu, _run(cpu), _weights(types, size))
