@@ -377,23 +377,24 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     const int per_sm = rows <= 8 || eights * prefix < (int64_t(1) << 18) ? 2 : 3;
     int64_t parts = std::min({per_sm * num_sms / eights, ceil_div(prefix, 64),
                               std::max({int64_t(16), std::min<int64_t>(ceil_div(prefix, 256), 32),
-                                        std::min<int64_t>(ceil_div(prefix, 1024), 64)})});
+                                        std::min<int64_t>(ceil_div(prefix, 1024), kPrefixParts)})});
     parts = std::max(parts, std::min<int64_t>(ceil_div(prefix, 4096), 32));
     pl.prefix_per = ceil_div(ceil_div(prefix, parts), 16) * 16;
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   } else if (prefix > 0) {
     const int64_t units = ceil_div(rows, 64) * Hkv;
     int64_t parts = std::min<int64_t>(ceil_div(2 * num_sms, units), ceil_div(prefix, 4 * kKeys));
-    parts = std::max<int64_t>(1, std::min<int64_t>(parts, 64));
+    parts = std::max<int64_t>(1, std::min<int64_t>(parts, kPrefixParts));
     pl.prefix_per = ceil_div(ceil_div(prefix, parts), kKeys) * kKeys;
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   }
-  // Own keys: enough parts to fill the GPU, none much longer than 1024 keys.
+  // Own keys: enough parts to fill the GPU, of about 1024 keys at most while
+  // there are no more than kOwnParts of them (131072 own keys: 4096 each).
   pl.row_chunks = static_cast<int>(ceil_div(rep, kOwnRows));
   pl.own_min = mma ? 128 : 64;
   const int64_t units = B * Hkv * pl.row_chunks;
   int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));
-  splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(32)});
+  splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(kOwnParts)});
   pl.own_splits = static_cast<int>(std::max<int64_t>(splits, 1));
   const size_t slots = static_cast<size_t>(Hkv * rows) * (pl.np + pl.own_splits);
   pl.acc_bytes = round256(slots * D * sizeof(float));
@@ -488,6 +489,8 @@ int launch_shared_prefix(const b200_shared_prefix_args_t& a, cudaStream_t stream
              a.workspace_bytes);
     return fail(B200_ERR_WORKSPACE, buf);
   }
+  if (pl.np > kPrefixParts || pl.own_splits > kOwnParts)
+    return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
   SharedParams p{};
   p.q = a.q;
   p.out = a.out;

@@ -47,6 +47,9 @@ struct SharedParams {
   float qscale;  // log2(e) / sqrt(D)
 };
 
+// The most parts of a row: of the prefix and of its own keys.
+constexpr int kPrefixParts = 64, kOwnParts = 32;
+
 // Own keys and join, bf16 pool, kOwnRows rows of a key head to a CTA.  (16 rows
 // take twice the registers and a longer code that has to be fetched first: 16
 // query heads to each of 4 key heads, 64 sequences behind 4096 keys 45 us, two
@@ -129,12 +132,13 @@ int launch_own(void (*kern)(Params...), int64_t grid, int block, int smem, cudaS
 
 // The joined rows row0 .. row0 + nrows - 1 (at most 8) of key head g, by a block
 // of 128 threads: sum_s 2^(m_s - M) acc_s / sum_s 2^(m_s - M) l_s over the
-// prefix's slots and the first `parts` own ones (at most 96 in all).  `sm`:
+// prefix's slots and the first `parts` own ones.  `sm`:
 // kJoinFloats of shared memory that the block is done with.  Four elements of a
 // row are a thread's, or, where the rows are short or few, several threads' that
 // share the parts out; the first loads are on their way before the factors are
 // known.
-constexpr int kJoinParts = 96, kJoinAhead = 8;
+constexpr int kJoinParts = kPrefixParts + kOwnParts, kJoinAhead = 8;
+static_assert(kJoinParts % 32 == 0, "a lane's parts");
 constexpr int kJoinFloats = 8 * kJoinParts + 128 * 4;
 __device__ __forceinline__ void join_rows(const SharedParams& p, int g, int row0, int nrows, int parts,
                                           float* sm) {

@@ -40,7 +40,7 @@ constexpr int kWarps = 4;
 constexpr int kStep = 16;      // keys a warp takes at a time
 constexpr int kAhead = 8;      // parts of a row that the join loads together (4 and 16: 1 to 5 % slower at
                                // many parts, and at many short joins)
-constexpr int kMaxSlots = 102;  // parts of a row: 65 of the prefix, 32 own ones, 4 warps
+constexpr int kMaxSlots = kPrefixParts + kOwnParts + kWarps;  // parts of a row, and the warps' states
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -506,8 +506,6 @@ int launch_one(const OwnParams& op, const b200_kv_pool_t& pool, const DeviceInfo
            cudaStream_t stream) {
   const SharedParams& p = op.s;
   const int64_t grid = static_cast<int64_t>(PREFIX ? p.np : p.B * p.own_splits) * p.row_chunks * p.Hkv;
-  if (p.np + p.own_splits + kWarps > kMaxSlots)
-    return fail(B200_ERR_UNSUPPORTED, "shared prefix: too many parts");
   const int smem = OwnSmem<DP, PREFIX, QP>::BYTES + 1024;
   CUtensorMap tk, tv;
   const uint64_t dims[3] = {static_cast<uint64_t>(pool.head_dim), static_cast<uint64_t>(pool.num_heads),

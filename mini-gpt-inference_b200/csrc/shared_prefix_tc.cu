@@ -736,7 +736,7 @@ TcSplit shared_tc_split(int64_t rows, int64_t Hkv, int64_t prefix, int num_sms) 
   t.unit_tiles = static_cast<int>(ceil_div(prefix, kBN));
   t.units = Hkv * t.unit_pairs;
   const int64_t shares = std::max(std::min<int64_t>(ceil_div(t.unit_tiles, 2), 32),
-                                  std::min<int64_t>(ceil_div(t.unit_tiles, 4), 64));
+                                  std::min<int64_t>(ceil_div(t.unit_tiles, 4), kPrefixParts));
   t.ctas = static_cast<int>(std::min<int64_t>(num_sms, t.units * shares));
   // The most CTAs that share a unit (an upper bound where the units are many).
   int64_t most = 1;
