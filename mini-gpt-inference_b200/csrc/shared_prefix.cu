@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(128) shared_own_elem_kernel(const __grid_const
   if (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S) {
     if (split == 0) {
       if (threadIdx.x == 0) report(p.status, B200_DEV_BAD_LENGTH);
+      if (p.out == p.q) wait_for_previous();  // it reads these rows
       for (int i = threadIdx.x; i < nrows * p.D; i += 128)
         store_elem(p.out, b * p.os0 + (g * p.rep + chunk * R + i / p.D) * p.os1 + (i % p.D) * p.os2,
                    p.out_dtype, 0.f);

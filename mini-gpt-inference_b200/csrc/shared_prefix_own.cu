@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (!PREFIX && (ctx < 1 || ctx < p.prefix || ctx > p.table_width * p.S)) {
     if (split == 0) {
       if (threadIdx.x == 0) report(p.status, B200_DEV_BAD_LENGTH);
+      if (p.out == p.q) wait_for_previous();  // it reads these rows
       for (int i = threadIdx.x; i < nrows * p.D; i += kWarps * 32)
         store_elem(p.out, b * p.os0 + (head0 + i / p.D) * p.os1 + (i % p.D) * p.os2, p.out_dtype, 0.f);
     }

@@ -146,3 +146,26 @@ def test_bad_own_pages_touch_no_other_sequence(rows):
     assert int(status) == _lib.DEV_BAD_BLOCK
     rest = [i for i in range(rows[0]) if i != 28]
     assert torch.equal(out[rest], want[rest])
+
+
+@HEADS
+@pytest.mark.parametrize("rows", [(40, 16, 4, 2900), (70, 8, 2, 5003), (20, 16, 16, 3001)], ids=str)
+def test_out_in_place_of_padding_rows_that_are_no_numbers(rows, d):
+    """Rows that hold anything, and get their zeros where their queries stood, leave
+    the other rows' results as they are, bit for bit."""
+    cpu = _case(rows, d, 80)
+    at = torch.arange(rows[3])
+    k = cpu.pool.k.float()
+    k[0, cpu.table[at // 16], at % 16, :, 0] += (at / rows[3] * 30 * d ** 0.5)[:, None]
+    cpu.pool.k = k.to(BF16)
+    cpu.q[..., 0] = 1
+    bad = torch.arange(0, rows[0], 6)
+    cpu.q[bad] = float("nan")
+    cpu.lens[bad] = 0
+    c = to_device(cpu)
+    want = _run(c)
+    assert not want[bad].any() and want.isfinite().all()
+    for _ in range(30):
+        c.q.copy_(cpu.q)
+        _run(c, out=c.q)
+        assert torch.equal(c.q, want)

@@ -42,3 +42,15 @@ def test_every_tmem_load_is_held_by_its_wait():
     for kind, args in loads:
         for name in [x.strip().split("[")[0] for x in args.split(",")][-2 if kind == "2" else -1:]:
             assert name in waited, args
+
+
+def test_zero_rows_in_place_of_queries_wait_for_the_prefix():
+    """The own-key kernels run beside the prefix's, which reads q; a row without a
+    valid length is written without its parts, so that nothing else orders it
+    behind those reads where out is q."""
+    for name in ("shared_prefix.cu", "shared_prefix_own.cu"):
+        code = re.sub(r"//[^\n]*", "", SOURCE.with_name(name).read_text())
+        bad = code.split("B200_DEV_BAD_LENGTH);")
+        assert len(bad) == 2
+        wait, store = bad[1].find("if (p.out == p.q) wait_for_previous();"), bad[1].find("store_elem(")
+        assert 0 <= wait < store
