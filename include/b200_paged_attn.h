@@ -393,6 +393,7 @@ typedef struct {
 } b200_shared_prefix_args_t;
 
 B200_API int b200_shared_prefix_decode(const b200_shared_prefix_args_t* args, void* stream);
+/* Its workspace bytes on the current device; 0 for sizes that the call refuses. */
 B200_API size_t b200_shared_prefix_decode_workspace_size(int64_t batch, int64_t num_q_heads,
                                                 int64_t num_kv_heads, int64_t head_dim,
                                                 int64_t prefix_len, int64_t table_width,

@@ -157,21 +157,27 @@ int check_rope(const b200_qk_norm_rope_args_t& a) {
   return B200_OK;
 }
 
+// What the launch and the workspace query are planned from; num_kv_heads >= 1.
+int check_shared_sizes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t prefix_len,
+                       int64_t table_width) {
+  B200_CHECK(batch >= 1 && num_q_heads >= 1, B200_ERR_INVALID_ARGUMENT, "q dimensions must be nonzero");
+  B200_CHECK(num_q_heads % num_kv_heads == 0, B200_ERR_INVALID_ARGUMENT,
+             "the query heads must be a multiple of the pool's heads");
+  B200_CHECK(batch < (int64_t(1) << 24) && num_q_heads < (int64_t(1) << 16) &&
+                 batch * num_q_heads < (int64_t(1) << 26),
+             B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
+  B200_CHECK(table_width >= 1, B200_ERR_INVALID_ARGUMENT, "block_tables need at least one block column");
+  B200_CHECK(prefix_len >= 0, B200_ERR_INVALID_ARGUMENT, "prefix_len must be >= 0");
+  B200_CHECK(prefix_len < (int64_t(1) << 30) && table_width < (int64_t(1) << 30),
+             B200_ERR_UNSUPPORTED, "shared prefix: contexts too long");
+  return B200_OK;
+}
+
 int check_shared(const b200_shared_prefix_args_t& a) {
   int rc = check_pool(a.pool, a.layer_idx);
   if (rc != B200_OK) return rc;
-  B200_CHECK(a.batch >= 1 && a.num_q_heads >= 1, B200_ERR_INVALID_ARGUMENT,
-             "q dimensions must be nonzero");
-  B200_CHECK(a.num_q_heads % a.pool.num_heads == 0, B200_ERR_INVALID_ARGUMENT,
-             "the query heads must be a multiple of the pool's heads");
-  B200_CHECK(a.batch < (int64_t(1) << 24) && a.num_q_heads < (int64_t(1) << 16) &&
-                 a.batch * a.num_q_heads < (int64_t(1) << 26),
-             B200_ERR_UNSUPPORTED, "shared prefix: too many query rows");
-  B200_CHECK(a.table_width >= 1, B200_ERR_INVALID_ARGUMENT,
-             "block_tables need at least one block column");
-  B200_CHECK(a.prefix_len >= 0, B200_ERR_INVALID_ARGUMENT, "prefix_len must be >= 0");
-  B200_CHECK(a.prefix_len < (int64_t(1) << 30) && a.table_width < (int64_t(1) << 30),
-             B200_ERR_UNSUPPORTED, "shared prefix: contexts too long");
+  rc = check_shared_sizes(a.batch, a.num_q_heads, a.pool.num_heads, a.prefix_len, a.table_width);
+  if (rc != B200_OK) return rc;
   B200_CHECK(a.q != nullptr && a.out != nullptr, B200_ERR_INVALID_ARGUMENT,
              "q and out must be non-null");
   B200_CHECK(valid_dtype(a.q_dtype) && valid_dtype(a.out_dtype), B200_ERR_INVALID_ARGUMENT,
@@ -354,8 +360,9 @@ size_t b200_shared_prefix_decode_workspace_size(int64_t batch, int64_t num_q_hea
                                                 int64_t prefix_len, int64_t table_width,
                                                 int64_t block_size, b200_dtype_t kv_dtype,
                                                 b200_dtype_t q_dtype) {
-  if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1 || prefix_len < 0 ||
-      table_width < 1 || block_size < 1)
+  clear_error();
+  if (num_kv_heads < 1 || head_dim < 1 || head_dim > 128 || !is_pow2(block_size) || block_size > 256 ||
+      check_shared_sizes(batch, num_q_heads, num_kv_heads, prefix_len, table_width) != B200_OK)
     return 0;
   return shared_prefix_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, prefix_len,
                                        table_width, block_size, kv_dtype, q_dtype, sm_count());
