@@ -59,16 +59,17 @@ def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
     return gap >= row_x and gap + row_y <= step_x
 
 
-def _check_out(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None:
+def _check_out(out: torch.Tensor, like: torch.Tensor, name: str, others) -> None:
     """An output is ``like``'s shape, dtype and device, and see _check_place."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have the shape, dtype and device of its input")
-    _check_place(out, like, name, inputs)
+    _check_place(out, like, name, others)
 
 
-def _check_place(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> None:
-    """An output writes no element twice, and is either exactly ``like`` or
-    apart from every input."""
+def _check_place(out: torch.Tensor, like: torch.Tensor, name: str, others=()) -> None:
+    """An output writes no element twice, is either exactly its input ``like``
+    or apart from it, and is apart from the others (one tensor given as two
+    inputs would be written as the one and read as the other)."""
     if out.numel() == 0:
         return
     # A permutation of contiguous rows, or rows apart: no element twice.
@@ -77,11 +78,10 @@ def _check_place(out: torch.Tensor, like: torch.Tensor, name: str, inputs) -> No
         if stride <= extent:
             raise ValueError(f"{name} must not overlap itself")
         extent += stride * (n - 1)
-    for t in inputs:
-        same = (t is like and t.dtype == out.dtype and t.data_ptr() == out.data_ptr()
-                and t.stride() == out.stride())
-        if not same and not _apart(out, t):
-            raise ValueError(f"{name} must be its input itself or not overlap the inputs")
+    same = (like.dtype == out.dtype and like.data_ptr() == out.data_ptr()
+            and like.stride() == out.stride())
+    if not (same or _apart(out, like)) or not all(_apart(out, t) for t in others):
+        raise ValueError(f"{name} must be its input itself or not overlap the inputs")
 
 
 def _rope_fields(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out,
@@ -130,7 +130,7 @@ def _rope_fields(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleav
         raise ValueError("eps must be positive")
     sp = 0 if status is None else _status_ptr(status, index)
     if q_out is not None:
-        _check_out(q_out, q, "q_out", (q, k) if v is None else (q, k, v))
+        _check_out(q_out, q, "q_out", (k,) if v is None else (k, v))
         qs = q_out.stride()
     else:
         q_out = q.new_empty((t, hq, d))
@@ -139,7 +139,7 @@ def _rope_fields(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleav
     ks = (0, 0, 0)
     if v is None:
         if k_out is not None:
-            _check_out(k_out, k, "k_out", (q, k, q_out))
+            _check_out(k_out, k, "k_out", (q, q_out))
             ks = k_out.stride()
         else:
             k_out = k.new_empty((t, hkv, d))

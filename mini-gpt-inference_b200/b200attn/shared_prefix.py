@@ -93,7 +93,7 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     elif out.shape != (b, hq, d) or out.dtype not in _DTYPES or out.get_device() != index:
         raise ValueError("out must be a [B,Hq,D] tensor on the q device")
     else:
-        _check_place(out, q, "out", (q,))
+        _check_place(out, q, "out")
     qd = _DTYPES[q.dtype]
     # A workspace of the call's own, from the allocator of the current stream
     # (or of the graph being captured): calls on other streams, and other
