@@ -65,7 +65,7 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     index = q.get_device()
     pool_fields = _pool_fields(pool, index, layer_idx)
     _, _, _, _, block, h, pd, kv_dtype = pool_fields
-    if pd != d or hq % h:
+    if pd != d or h == 0 or hq % h:
         raise ValueError("the KV pool needs q's head dimension and a divisor of its heads")
     if block_tables.ndim != 2:
         raise ValueError("block_tables must have shape [B,M]")

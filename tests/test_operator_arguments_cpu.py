@@ -35,3 +35,13 @@ def test_one_tensor_as_k_and_v_of_an_append_in_place():
     with pytest.raises(ValueError, match="not overlap the inputs"):
         rope_kv_append_b200(_Cuda(x), torch.zeros(3, 2, 32), x, pool, torch.arange(3),
                             torch.zeros(3, dtype=torch.int64), rope_table(8, 32), 0, q_out=x)
+
+
+def test_a_pool_without_heads():
+    from b200attn import shared_prefix_decode_b200
+
+    pool = SimpleNamespace(k=torch.zeros(1, 2, 16, 0, 32), v=torch.zeros(1, 2, 16, 0, 32), block_size=16)
+    tables = torch.zeros(3, 2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="head dimension"):
+        shared_prefix_decode_b200(_Cuda(torch.zeros(3, 8, 32)), pool, tables[0], 16, tables,
+                                  torch.full((3,), 17), 0)
