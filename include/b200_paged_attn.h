@@ -358,6 +358,9 @@ B200_API int b200_rope_kv_append(const b200_rope_kv_append_args_t* args, void* s
  * pool's num_heads.  prefix_len 0 is a plain paged decode.
  * A sequence whose length is < 1, < prefix_len or > M*S gets zero rows and
  * sets B200_DEV_BAD_LENGTH (a padding row of a fixed-size batch, say).
+ * The launch and the workspace are sized by M: of tables much wider than the
+ * sequences need, pass the columns that the longest one does (table_width; the
+ * row stride stays).
  * `workspace`: b200_shared_prefix_decode_workspace_size() bytes, 256-byte
  * aligned; its contents need not be initialised and are the call's own until
  * it has run.

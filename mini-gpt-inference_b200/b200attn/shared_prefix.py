@@ -44,6 +44,10 @@ def shared_prefix_decode_b200(q: torch.Tensor, pool, prefix_table, prefix_len: i
     are not read); context_lengths: [B], prefix included.  The new token's K/V
     are already in the pool (``rope_kv_append_b200`` or ``kv_scatter_b200``).
 
+    The launch and its workspace are sized by M, since the lengths are the
+    device's: of tables much wider than the sequences need, pass a view of the
+    columns that the longest one does, ``block_tables[:, :n]``.
+
     Where a prefix ends inside a block, position ``prefix_len`` is row
     ``prefix_len % S`` of the sequence's own block of that column.
     ``prefix_len`` 0 is a plain paged decode.  A sequence shorter than the

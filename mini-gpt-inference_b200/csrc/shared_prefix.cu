@@ -390,12 +390,19 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
     pl.np = static_cast<int>(ceil_div(prefix, pl.prefix_per));
   }
   // Own keys: enough parts to fill the GPU, of about 1024 keys at most while
-  // there are no more than kOwnParts of them (131072 own keys: 4096 each).
+  // there are no more than kOwnParts of them (131072 own keys: 4096 each).  The
+  // lengths are the device's, and a part that a sequence does not need is a CTA
+  // that reads its length and ends, so that tables much wider than the lengths cost
+  // time: at most 28 rounds of the four CTAs to an SM.  (256 sequences of 8 heads
+  // with up to 128 own keys and tables for 131072: 83 us, with 32 parts 154, tables
+  // for no more than the lengths 61; one of them with 16384 own keys, tables for
+  // 32768: 89 and 149; one with 100000: 309 and 195.)
   pl.row_chunks = static_cast<int>(ceil_div(rep, kOwnRows));
   pl.own_min = mma ? 128 : 64;
   const int64_t units = B * Hkv * pl.row_chunks;
   int64_t splits = std::max<int64_t>(ceil_div(2 * num_sms, units), ceil_div(max_own, 1024));
-  splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(kOwnParts)});
+  splits = std::min<int64_t>({splits, ceil_div(max_own, pl.own_min), int64_t(kOwnParts),
+                              std::max<int64_t>(28 * 4 * num_sms / units, 1)});
   pl.own_splits = static_cast<int>(std::max<int64_t>(splits, 1));
   const size_t slots = static_cast<size_t>(Hkv * rows) * (pl.np + pl.own_splits);
   pl.acc_bytes = round256(slots * D * sizeof(float));

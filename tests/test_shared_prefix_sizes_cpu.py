@@ -54,3 +54,14 @@ def test_sizes_at_the_limits():
                    dict(batch=1, hq=1, hkv=1, prefix=0, width=1), dict(batch=1023, hq=65535, hkv=65535),
                    dict(width=(1 << 30) - 1)):
             assert size(*_with(kv=kv, q=q, **kw)) > 0
+
+
+def test_wide_tables_do_not_multiply_the_parts_of_a_large_batch():
+    """A row's own parts cost workspace, and CTAs, by the table's width: few in a
+    large batch, all 32 in a small one."""
+    size = _lib.load().b200_shared_prefix_decode_workspace_size
+    part = lambda b: b * 32 * (128 + 2) * 4  # noqa: E731
+    wide, tight = (size(*_with(batch=256, width=w)) for w in (8192, (4096 + 128) // 16))
+    assert 0 < wide - tight <= 7 * part(256) + 1024
+    wide, tight = (size(*_with(batch=16, width=w)) for w in (8192, (4096 + 128) // 16))
+    assert wide - tight >= 28 * part(16)
