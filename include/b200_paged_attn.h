@@ -361,6 +361,14 @@ B200_API int b200_rope_kv_append(const b200_rope_kv_append_args_t* args, void* s
  * The launch and the workspace are sized by M: of tables much wider than the
  * sequences need, pass the columns that the longest one does (table_width; the
  * row stride stays).
+ * Scores, weights and sums are f32 (f16 and f32 queries of a bf16 pool keep all
+ * their bits).  With bf16 queries of a bf16 pool and more than 128 query rows to
+ * a key head (B * Hq / H) the prefix's weights are rounded to bf16 for their
+ * product with V, half a step, 2^-8, each; elsewhere they keep 2^-16 or better.
+ * Entries behind a context, or that no sequence owns, may hold anything.
+ * Infinities and NaN that are read act as in the formula (a score of -inf has no
+ * weight, an infinite value gives an infinity) while the key's weight is above
+ * 2^-100 of its row's largest; below, the key may count as one without a weight.
  * `workspace`: b200_shared_prefix_decode_workspace_size() bytes, 256-byte
  * aligned; its contents need not be initialised and are the call's own until
  * it has run.

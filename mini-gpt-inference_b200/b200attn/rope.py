@@ -201,7 +201,8 @@ def rope_kv_append_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool,
     A slot outside the pool, or a position outside the table, skips that
     token's k and v and sets DEV_BAD_SLOT / DEV_BAD_POSITION in ``status``.
     Slots of one call are distinct, except those that nothing reads (padding
-    rows that share a scratch slot).
+    rows that share a scratch slot); q, k and v are not views of the pool's
+    slots that the call writes.
     """
     _inference_only(q, k, v, cos_sin, q_weight, k_weight)
     lib = _lib.load()

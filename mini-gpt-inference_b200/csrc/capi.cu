@@ -137,7 +137,8 @@ int check_rope(const b200_qk_norm_rope_args_t& a) {
              "q and k dimensions must be nonzero");
   B200_CHECK(a.head_dim <= 256 && a.num_q_heads + 2 * a.num_kv_heads < (int64_t(1) << 20),
              B200_ERR_UNSUPPORTED, "rotation: head_dim must be <= 256 (and heads < 2^20)");
-  // One CTA per token: the grid's x extent bounds T.
+  // The element kernel has one CTA per token, and the grid's x extent bounds T (the
+  // vector kernel takes very many tokens in several launches).
   B200_CHECK(a.num_tokens < (int64_t(1) << 31) - 1, B200_ERR_UNSUPPORTED,
              "rotation: num_tokens must be < 2^31 - 1");
   B200_CHECK(a.q != nullptr && a.k != nullptr && a.q_out != nullptr && a.cos_sin != nullptr &&

@@ -358,7 +358,9 @@ SharedPlan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pref
   // (4 sequences of 8 x 4 heads over 2048 keys: 10 us against 15; over 32768: 32
   // against 43; 1 of 32 x 1: 83 against 116).  Above, it is as long as little is
   // read: 64 rows to each of 8 heads, 1024 keys 13 us against 17, 2048 the same,
-  // 8192 30 against 23.
+  // 8192 30 against 23.  Queries of other types have no tensor-tile form, however
+  // many: eight rows at a time they take 245 (f16) and 280 us (f32) at 1024 rows to
+  // each of 8 heads behind 4096 keys, by f32 arithmetic 694.
   const int64_t eights = ceil_div(rows, kOwnRows) * Hkv;
   pl.few = mma && prefix > 0 &&
            (q_dtype != B200_DTYPE_BF16 || rows <= 16 || eights * prefix < (int64_t(1) << 17));
