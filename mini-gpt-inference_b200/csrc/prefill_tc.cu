@@ -451,11 +451,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t key = key0 + (static_cast<int64_t>(b) << p.rb_shift);
       const int64_t raw = raw_next;
       raw_next = entry(j + 1);
-      int ok = 1;
-      if (lane == 0) ok = mbar_wait(&empty[st], (use & 1u) ^ 1u) ? 1 : 0;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok || *reinterpret_cast<volatile int32_t*>(abort_flag)) {
-        if (lane == 0 && !ok) {
+      // Lane 0 waits, and looks at the abort flag, for the warp: lanes that look
+      // for themselves may see it set on different sides of a look.
+      int state = 0;  // 1: another role has given up, 2: the wait ran out
+      if (lane == 0)
+        state = !mbar_wait(&empty[st], (use & 1u) ^ 1u)                ? 2
+                : *reinterpret_cast<volatile int32_t*>(abort_flag) != 0 ? 1
+                                                                        : 0;
+      state = __shfl_sync(0xffffffffu, state, 0);
+      if (state != 0) {
+        if (lane == 0 && state == 2) {
           report(p.status, B200_DEV_WAIT_TIMEOUT);
           *abort_flag = 1;
         }
@@ -600,11 +605,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nk = g.cnt[w];
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    // A whole warp's wait: what follows (votes, TMEM access) needs every lane.
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;
+    };
     for (int k = 0; k < nk; ++k) {
       const int j = g.tile(w, k);
       const int sb = k & 1;          // barrier parity of this tile
       const int buf = k % kNBuf;     // S buffer of this tile
-      if (!mbar_wait(&s_full[w * 2 + sb], static_cast<uint32_t>(k >> 1) & 1u)) {
+      if (!warp_wait(&s_full[w * 2 + sb], static_cast<uint32_t>(k >> 1) & 1u)) {
         ok = false;
         break;
       }
@@ -676,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // P.V(k-1) must have completed before O is rescaled (only then is
         // the softmax held back by the MMAs of an earlier tile).
         const int kp = k - 1;
-        if (!mbar_wait(&o_done[w * 2 + (kp & 1)], static_cast<uint32_t>(kp >> 1) & 1u)) {
+        if (!warp_wait(&o_done[w * 2 + (kp & 1)], static_cast<uint32_t>(kp >> 1) & 1u)) {
           ok = false;
           break;
         }
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first_w = g.split ? (j & 1) : (j < g.nkt[0] ? 0 : 1);
       if (w == first_w && valid < kBN) {
         // V of this tile must have landed before its rows are cleared.
-        if (!mbar_wait(&v_full[j % kVStages], static_cast<uint32_t>(j / kVStages) & 1u)) {
+        if (!warp_wait(&v_full[j % kVStages], static_cast<uint32_t>(j / kVStages) & 1u)) {
           ok = false;
           break;
         }
@@ -720,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // The last P.V completing implies all earlier ones have (issue order).
     if (nk > 0 && ok &&
-        !mbar_wait(&o_done[w * 2 + ((nk - 1) & 1)], static_cast<uint32_t>((nk - 1) >> 1) & 1u))
+        !warp_wait(&o_done[w * 2 + ((nk - 1) & 1)], static_cast<uint32_t>((nk - 1) >> 1) & 1u))
       ok = false;
     if (!ok) {
       if (r == 0) report(p.status, B200_DEV_WAIT_TIMEOUT);
@@ -743,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       tc_fence_after();
-      write = write && w == 0 && *reinterpret_cast<volatile int32_t*>(abort_flag) == 0;
+      write = write && w == 0 && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int32_t*>(abort_flag) != 0);
       if (write) {
         uint32_t mb, lb;
         tmem_ld2(tmem_s(1, 0) + lane_base, mb, lb);

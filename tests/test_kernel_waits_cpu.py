@@ -54,3 +54,15 @@ def test_zero_rows_in_place_of_queries_wait_for_the_prefix():
         assert len(bad) == 2
         wait, store = bad[1].find("if (p.out == p.q) wait_for_previous();"), bad[1].find("store_elem(")
         assert 0 <= wait < store
+
+
+def test_waits_of_the_prefill_are_votes_too():
+    """Single lanes wait for themselves only inside lane 0's branches."""
+    code = re.sub(r"//[^\n]*", "", SOURCE.with_name("prefill_tc.cu").read_text())
+    softmax = code[code.index("const int w = wg;"):]
+    helper = "return __all_sync(0xffffffffu, mbar_wait(bar, parity)) != 0;"
+    assert softmax.count(helper) == 1 and "mbar_wait(" not in softmax.replace(helper, "")
+    # Reads of the flag: lane 0's, for its warp, and a vote.
+    reads = re.findall(r"[^;{}]*\*reinterpret_cast<volatile int32_t\*>\(abort_flag\)[^;]*;", code)
+    assert len(reads) == 2
+    assert "if (lane == 0)" in reads[0] and "__any_sync(0xffffffffu," in reads[1]
