@@ -149,7 +149,7 @@ __device__ __forceinline__ float p_pass(uint32_t srow, float scale, float neg_m,
                   make_float2(0.f, 0.f)};
   float sv[2][32];
   tmem_ld32(srow, sv[0]);
-  tmem_wait_ld();
+  wait_ld32(sv[0]);
 #pragma unroll
   for (int c = 0; c < kBN; c += 32) {
     const int cur = (c >> 5) & 1;
@@ -168,7 +168,7 @@ __device__ __forceinline__ float p_pass(uint32_t srow, float scale, float neg_m,
       pk[e >> 1] = pack_bf16(p0, p1);
     }
     tmem_st16(srow + (c >> 1), pk);
-    if (c + 32 < kBN) tmem_wait_ld();
+    if (c + 32 < kBN) wait_ld32(sv[cur ^ 1]);
   }
   return ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
 }
@@ -633,7 +633,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         {
 #pragma unroll
           for (int c = 0; c < kBN; c += 32) tmem_ld32(tmem_s(w, buf) + lane_base + c, sv + c);
-          tmem_wait_ld();
+          wait_ld32(sv);
+#pragma unroll
+          for (int c = 32; c < kBN; c += 32) waited32(sv + c);
           // Eight independent chains of three-input max, then a tree.
           float mp[8];
           if (need_mask) {
@@ -695,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < D; c += 32) {
             float o[32];
             tmem_ld32(tmem_o(w) + lane_base + c, o);
-            tmem_wait_ld();
+            wait_ld32(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] *= alpha;
             tmem_st32(tmem_o(w) + lane_base + c, o);
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (write) {
         uint32_t mb, lb;
         tmem_ld2(tmem_s(1, 0) + lane_base, mb, lb);
-        tmem_wait_ld();
+        wait_ld2(mb, lb);
         const float m1 = __uint_as_float(mb), l1 = __uint_as_float(lb);
         const float mm = fmaxf(m, m1);
         // (Under a key split over CTAs a row may see no key of this CTA's
@@ -787,11 +789,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (g.split) {
             float o1[32];
             tmem_ld32(tmem_o(1) + lane_base + c, o1);
-            tmem_wait_ld();
+            wait_ld32(o);
+            waited32(o1);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = o[e] * a_self + o1[e] * a_other;
           } else {
-            tmem_wait_ld();
+            wait_ld32(o);
           }
 #pragma unroll
           for (int e = 0; e < 32; ++e) prow[(c + e) * kRows] = o[e];
@@ -869,11 +872,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (g.split) {
           float o1[32];
           tmem_ld32(tmem_o(1) + lane_base + c, o1);
-          tmem_wait_ld();
+          wait_ld32(o);
+          waited32(o1);
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = o[e] * ws + o1[e] * wo;
         } else {
-          tmem_wait_ld();
+          wait_ld32(o);
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] *= ws;
         }

@@ -153,7 +153,8 @@ __device__ __forceinline__ void epi_store64(uint32_t taddr, uint8_t* stage, __nv
   __syncwarp();  // tcgen05.ld is warp-collective; the staging rows are free
   tmem_ld32(taddr, v);
   tmem_ld32(taddr + 32u, v + 32);
-  tmem_wait_ld();
+  wait_ld32(v);
+  waited32(v + 32);
   uint4* srow = reinterpret_cast<uint4*>(stage + lane * kEpiPitch);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (c >= bn) break;
       float* cur = v[i & 1];
       if (mine_ok) {
-        tmem_wait_ld();
+        wait_ld32(cur);
         if (c + 32 < bn) tmem_ld32(trow + static_cast<uint32_t>(c + 32), v[(i + 1) & 1]);
       } else {
 #pragma unroll

@@ -103,22 +103,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const 
   return __all_sync(0xffffffffu, mbar_wait(bar, parity) && *abort_flag == 0) != 0;
 }
 
-// Waits for this thread's TMEM loads; the 32 values cannot be used earlier.
-__device__ __forceinline__ void wait_ld32(float* v) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
-        "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
-        "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
-        "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
-}
-
-// The same for the pair of each of two groups.
-__device__ __forceinline__ void wait_ld4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(a), "+r"(b), "+r"(c), "+r"(d));
-}
-
 // Weights 2^(v scale - ref) of 32 scores as bf16 pairs; returns their sum
 // before the rounding.  LO: rounded towards zero, and also what that left.
 template <bool LO>

@@ -66,3 +66,12 @@ def test_waits_of_the_prefill_are_votes_too():
     reads = re.findall(r"[^;{}]*\*reinterpret_cast<volatile int32_t\*>\(abort_flag\)[^;]*;", code)
     assert len(reads) == 2
     assert "if (lane == 0)" in reads[0] and "__any_sync(0xffffffffu," in reads[1]
+
+
+def test_no_kernel_waits_for_tmem_without_its_registers():
+    for path in SOURCE.parent.glob("*.cu*"):
+        code = re.sub(r"//[^\n]*", "", path.read_text())
+        for m in re.finditer(r'"tcgen05\.wait::ld[^"]*"([^;]*);', code):
+            assert '"+f"(' in m[1] or '"+r"(' in m[1], (path.name, m[0])
+        if "tmem_ld" in code and path.suffix == ".cu":
+            assert re.search(r"\bwait_ld(?:2|4|32)\(", code), path.name
